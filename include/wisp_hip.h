@@ -205,6 +205,53 @@ size_t wisp_moe_fp8_work_bytes(int T, int K, int H, int I, int nslots);
 int wisp_quant_fp8_groups(const void* x, int dtype, int rows, int cols, int group, uint8_t* q,
                           float* scales, wisp_stream_t stream);
 
+/* MXFP4: a row's values in blocks of 32, each value a 4-bit E2M1 code (two to
+ * a byte, the earlier value in the low half), each block one E8M0 scale byte
+ * s: value = E2M1(code) * 2^(s - 127), s = 255: NaN.  No reference
+ * counterpart (the reference pages bf16 and block-FP8 experts).
+ *
+ * x [rows, cols] (WISP_F32 or WISP_BF16, rows contiguous) -> codes
+ * [rows, cols / 2], scales [rows, cols / 32].  A block's scale is
+ * 2^(floor(log2 max|v|) - 2), no smaller than 2^-127; values are rounded to
+ * the nearest code, ties to the even one, and saturate at 6.  A block that
+ * holds an infinity or a NaN gets scale 255 and zero codes.  cols must be a
+ * multiple of 32, x 16-byte and codes 4-byte aligned. */
+int wisp_quant_mxfp4(const void* x, int dtype, int64_t rows, int cols, uint8_t* codes,
+                     uint8_t* scales, wisp_stream_t stream);
+
+/* The values of codes and scales in dtype (WISP_F32 or WISP_BF16): exact,
+ * except that a magnitude of 2^128 or more is an infinity. */
+int wisp_dequant_mxfp4(const uint8_t* codes, const uint8_t* scales, int64_t rows, int cols,
+                       void* out, int dtype, wisp_stream_t stream);
+
+/* wisp_moe_experts over MXFP4 weights: x, act and out are bfloat16; sums are
+ * float32, act and out are rounded once.  W13 of slot s: codes at
+ * w13 + s*w13_stride ([2I, H/2]), scales at s13 + s*s13_stride ([2I, H/32]);
+ * W2 [H, I/2] and s2 [H, I/32] likewise; strides in bytes.  H and I must be
+ * multiples of 32, H*I below 2^31, weights and their strides 16-byte aligned.
+ * A slot outside [0, nslots) contributes zero.  act: T*K*I elements; work:
+ * device, 256-byte aligned, wisp_moe_mxfp4_work_bytes(T, K, H, nslots)
+ * bytes. */
+int wisp_moe_experts_mxfp4(const void* x, int T, int H, int I, int K, const float* topk_w,
+                           const int32_t* slots, int nslots, const void* w13, size_t w13_stride,
+                           const void* s13, size_t s13_stride, const void* w2, size_t w2_stride,
+                           const void* s2, size_t s2_stride, void* act, void* out, void* work,
+                           size_t work_bytes, wisp_stream_t stream);
+
+/* The whole MoE layer over E resident MXFP4 experts: wisp_route_topk_softmax
+ * on logits [T, E], then wisp_moe_experts_mxfp4 with expert e in slot e.
+ * topk_w and topk_ids [T, K] receive the routing. */
+int wisp_moe_layer_mxfp4(const void* x, const void* logits, int logits_dtype, int T, int H, int I,
+                         int E, int K, int renormalize, float* topk_w, int32_t* topk_ids,
+                         const void* w13, size_t w13_stride, const void* s13, size_t s13_stride,
+                         const void* w2, size_t w2_stride, const void* s2, size_t s2_stride,
+                         void* act, void* out, void* work, size_t work_bytes,
+                         wisp_stream_t stream);
+
+/* Bytes of the work buffer of the MXFP4 experts (pair lists and fp32 per-pair
+ * outputs). */
+size_t wisp_moe_mxfp4_work_bytes(int T, int K, int H, int nslots);
+
 /* Bytes of the device array wisp_moe_experts_noalloc works in, per GPU, in
  * a default build; building with WISP_NOALLOC_SCRATCH_MIB=n sets n MiB, and
  * wisp_noalloc_scratch_bytes() returns the size the library was built with.

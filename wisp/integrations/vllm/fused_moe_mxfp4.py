@@ -1,0 +1,198 @@
+"""MXFP4 experts for MI355X: quantising weights to 4-bit microscaled floating
+point, reading them back, and the MoE layer over such weights.
+
+The reference pages bf16 and block-FP8 experts only; this format has no
+counterpart there.  An expert in MXFP4 is 17/32 of a byte a weight: 3.76 times
+fewer bytes over the host link and from HBM than in bf16, 1.88 times fewer
+than in FP8.
+
+Format.  A row's values in blocks of 32; each value a 4-bit E2M1 code (two to a
+byte, the earlier value in the low half), each block one E8M0 scale byte ``s``;
+a value is ``E2M1(code) * 2**(s - 127)``, ``s == 255`` is NaN.  Weights are
+``uint8`` tensors: codes ``w13 [E, 2I, H/2]``, ``w2 [E, H, I/2]``, scales
+``s13 [E, 2I, H/32]``, ``s2 [E, H, I/32]``.  Activations are bfloat16; products
+are summed in float32; the SwiGLU result and the output are rounded to bfloat16
+once each.
+"""
+from __future__ import annotations
+
+import functools
+
+import torch
+
+from wisp_amd import _lib
+from wisp_amd._lib import check, lib
+from .fused_moe import _check_out, _require_device
+
+BLOCK = 32
+_DTYPES = {torch.float32: _lib.WISP_F32, torch.bfloat16: _lib.WISP_BF16}
+
+
+def _on_device(fn):
+    """Runs ``fn`` with its first argument's GPU as the current device, on
+    that device's current stream."""
+    first = fn.__code__.co_varnames[0]
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        t = args[0] if args else kwargs.get(first)
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError(f"wisp.mxfp4: {fn.__name__} takes device tensors")
+        if t.device.index == torch.cuda.current_device():
+            return fn(*args, **kwargs)
+        with torch.cuda.device(t.device):
+            return fn(*args, **kwargs)
+    return call
+
+
+@_on_device
+def quantize_mxfp4(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``w [..., C]`` (float32 or bfloat16, C a multiple of 32) -> codes
+    ``[..., C/2]`` and scales ``[..., C/32]``.  A block's scale is
+    ``2**(floor(log2(max|w|)) - 2)``; values are rounded to the nearest code
+    (ties to the even one) and saturate at 6 times the scale.  A block with an
+    infinity or a NaN reads back as NaNs."""
+    if w.dtype not in _DTYPES:
+        raise NotImplementedError(f"wisp.mxfp4: cannot quantise {w.dtype} (float32 and bfloat16)")
+    if w.dim() < 1 or w.shape[-1] % BLOCK:
+        raise ValueError("wisp.mxfp4: the last dimension must be a multiple of 32")
+    w = w.contiguous()
+    if w.data_ptr() % 16:
+        w = w.clone()
+    C = w.shape[-1]
+    codes = torch.empty((*w.shape[:-1], C // 2), dtype=torch.uint8, device=w.device)
+    scales = torch.empty((*w.shape[:-1], C // BLOCK), dtype=torch.uint8, device=w.device)
+    if w.numel():
+        check(lib().wisp_quant_mxfp4(w.data_ptr(), _DTYPES[w.dtype], w.numel() // C, C,
+                                     codes.data_ptr(), scales.data_ptr(), _lib.stream_handle()),
+              "quantize_mxfp4")
+    return codes, scales
+
+
+@_on_device
+def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor,
+                     dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values of codes ``[..., C/2]`` and scales ``[..., C/32]`` as
+    ``[..., C]`` in ``dtype`` (bfloat16 or float32; both hold them exactly)."""
+    if dtype not in _DTYPES:
+        raise NotImplementedError(f"wisp.mxfp4: cannot read back as {dtype} "
+                                  "(float32 and bfloat16)")
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError("wisp.mxfp4: codes and scales are uint8")
+    if codes.dim() < 1 or scales.shape != (*codes.shape[:-1], codes.shape[-1] // 16) or \
+            codes.shape[-1] % 16:
+        raise ValueError(f"wisp.mxfp4: codes {tuple(codes.shape)} and scales "
+                         f"{tuple(scales.shape)} disagree (16 bytes of codes a scale)")
+    _require_device(scales, codes.device, "scales")
+    codes, scales = codes.contiguous(), scales.contiguous()
+    if codes.data_ptr() % 4:
+        codes = codes.clone()
+    C = 2 * codes.shape[-1]
+    out = torch.empty((*codes.shape[:-1], C), dtype=dtype, device=codes.device)
+    if out.numel():
+        check(lib().wisp_dequant_mxfp4(codes.data_ptr(), scales.data_ptr(), out.numel() // C, C,
+                                       out.data_ptr(), _DTYPES[dtype], _lib.stream_handle()),
+              "dequantize_mxfp4")
+    return out
+
+
+def _check_weights(x, w13, w2, s13, s2) -> tuple[int, int, int]:
+    """``(E, H, I)`` of MXFP4 expert tensors beside activations ``x [T, H]``."""
+    if x.dtype != torch.bfloat16:
+        raise NotImplementedError("wisp.mxfp4: activations must be bfloat16")
+    if x.dim() != 2 or w13.dim() != 3 or w2.dim() != 3:
+        raise ValueError("wisp.mxfp4: x is [T, H], w13 [E, 2I, H/2], w2 [E, H, I/2]")
+    H = x.shape[1]
+    E, I = w13.shape[0], 2 * w2.shape[2]
+    dev = x.device
+    for t, name, shape in ((w13, "w13", (E, 2 * I, H // 2)), (w2, "w2", (E, H, I // 2)),
+                           (s13, "s13", (E, 2 * I, H // BLOCK)), (s2, "s2", (E, H, I // BLOCK))):
+        if t.dtype != torch.uint8 or t.shape != shape:
+            raise ValueError(f"wisp.mxfp4: {name} must be a uint8 {shape} tensor")
+        if t.device != dev:
+            _require_device(t, dev, name)
+        st = t.stride()
+        if st[2] != 1 or st[1] != shape[2]:
+            raise ValueError(f"wisp.mxfp4: each expert of {name} must be contiguous")
+    return E, H, I
+
+
+def _buffers(x, T, K, H, I, nslots):
+    """act and the work buffer of one call, in one allocation of its own (so
+    that calls on other streams, or captured into other graphs, share
+    nothing): ``(tensor, act address, work address, work bytes)``."""
+    act = -(-T * K * I * 2 // 256) * 256
+    nbytes = lib().wisp_moe_mxfp4_work_bytes(T, K, H, nslots)
+    buf = torch.empty(act + nbytes, dtype=torch.uint8, device=x.device)
+    p = buf.data_ptr()
+    return buf, p, p + act, nbytes
+
+
+def _output(x, out):
+    if out is None:
+        return torch.empty_like(x)
+    _check_out(out, x)
+    return out
+
+
+@_on_device
+def experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, slots: torch.Tensor, w13: torch.Tensor,
+                  w2: torch.Tensor, s13: torch.Tensor, s2: torch.Tensor,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """SwiGLU experts over MXFP4 weights with the routing-order combine:
+    ``out[t] = sum_k topk_w[t, k] * expert(slots[t, k], x[t])``.  ``x [T, H]``
+    bfloat16, ``topk_w [T, K]`` float32, ``slots [T, K]`` int32; a slot outside
+    ``[0, E)`` (say -1) contributes nothing."""
+    E, H, I = _check_weights(x, w13, w2, s13, s2)
+    T = x.shape[0]
+    if slots.dim() != 2 or slots.shape[0] != T or topk_w.shape != slots.shape or \
+            slots.dtype != torch.int32 or topk_w.dtype != torch.float32:
+        raise ValueError(f"wisp.mxfp4: topk_w float32 and slots int32 must be [{T}, K]")
+    _require_device(slots, x.device, "slots")
+    _require_device(topk_w, x.device, "topk_w")
+    K = slots.shape[1]
+    x, slots, topk_w = x.contiguous(), slots.contiguous(), topk_w.contiguous()
+    out = _output(x, out)
+    if T == 0:
+        return out
+    buf, act, work, nbytes = _buffers(x, T, K, H, I, E)
+    check(lib().wisp_moe_experts_mxfp4(
+        x.data_ptr(), T, H, I, K, topk_w.data_ptr(), slots.data_ptr(), E, w13.data_ptr(),
+        w13.stride(0), s13.data_ptr(), s13.stride(0), w2.data_ptr(), w2.stride(0), s2.data_ptr(),
+        s2.stride(0), act, out.data_ptr(), work, nbytes, _lib.stream_handle()), "experts_mxfp4")
+    return out
+
+
+@_on_device
+def route_and_experts_mxfp4(x: torch.Tensor, router_logits: torch.Tensor, top_k: int,
+                            renormalize: bool, w13: torch.Tensor, w2: torch.Tensor,
+                            s13: torch.Tensor, s2: torch.Tensor,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """The whole MoE layer, all MXFP4 experts resident in device tensors:
+    softmax routing of ``router_logits [T, E]`` (top-k by logit, ties to the
+    lower id), then :func:`experts_mxfp4` with slot = expert id."""
+    E, H, I = _check_weights(x, w13, w2, s13, s2)
+    T, K = x.shape[0], int(top_k)
+    if router_logits.shape != (T, E):
+        raise ValueError(f"wisp.mxfp4: router_logits must be [{T}, {E}]")
+    if not 1 <= K <= E:
+        raise ValueError(f"wisp.mxfp4: top_k={top_k} outside [1, {E}]")
+    _require_device(router_logits, x.device, "router_logits")
+    if router_logits.dtype not in _DTYPES:
+        router_logits = router_logits.float()
+    x, router_logits = x.contiguous(), router_logits.contiguous()
+    out = _output(x, out)
+    if T == 0:
+        return out
+    buf, act, work, nbytes = _buffers(x, T, K, H, I, E)
+    routing = torch.empty(2 * T * K, dtype=torch.int32, device=x.device)
+    check(lib().wisp_moe_layer_mxfp4(
+        x.data_ptr(), router_logits.data_ptr(), _DTYPES[router_logits.dtype], T, H, I, E, K,
+        int(bool(renormalize)), routing.data_ptr(), routing.data_ptr() + 4 * T * K,
+        w13.data_ptr(), w13.stride(0), s13.data_ptr(), s13.stride(0), w2.data_ptr(), w2.stride(0),
+        s2.data_ptr(), s2.stride(0), act, out.data_ptr(), work, nbytes, _lib.stream_handle()),
+        "route_and_experts_mxfp4")
+    return out
+
+
+__all__ = ["quantize_mxfp4", "dequantize_mxfp4", "experts_mxfp4", "route_and_experts_mxfp4"]

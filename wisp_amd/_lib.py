@@ -103,6 +103,14 @@ SIGNATURES = {
                                     _vp]),
     "wisp_quant_fp8_groups": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
     "wisp_moe_fp8_work_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "wisp_quant_mxfp4": (_i32, [_vp, _i32, _i64, _i32, _vp, _vp, _vp]),
+    "wisp_dequant_mxfp4": (_i32, [_vp, _vp, _i64, _i32, _vp, _i32, _vp]),
+    "wisp_moe_experts_mxfp4": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _sz, _vp,
+                                      _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _vp]),
+    "wisp_moe_layer_mxfp4": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp,
+                                    _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz,
+                                    _vp]),
+    "wisp_moe_mxfp4_work_bytes": (_sz, [_i32, _i32, _i32, _i32]),
     "wisp_layer_create": (_i32, [C.POINTER(LayerDesc), C.POINTER(_vp)]),
     "wisp_layer_destroy": (_i32, [_vp]),
     "wisp_layer_set_scratch": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp]),

@@ -25,6 +25,8 @@ SOURCES = [
     "experts_gemv.hip",
     "experts_mfma.hip",
     "experts_fp8.hip",
+    "experts_mxfp4.hip",
+    "quant_mxfp4.hip",
     "pagein.hip",
     "packed.hip",
     "prefetch.hip",

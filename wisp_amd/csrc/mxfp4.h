@@ -1,0 +1,42 @@
+// MXFP4 on gfx950: E2M1 codes (two to a byte, the earlier value in the low
+// half) with one E8M0 scale byte s per block of 32 values of a row; a value is
+// E2M1(code) * 2^(s - 127), s = 255 is NaN.
+//
+// The conversions are single instructions that take the scale as a float
+// whose exponent field is s.  Checked on MI355X over every byte and scale
+// (reading back) and every finite bf16 value (quantising): exact, rounded to
+// nearest with ties to the even code, saturating at 6, subnormal results and
+// scales included.  A value read back is exact in bf16 too: two significant
+// bits, and no exponent below bf16's subnormals.
+#pragma once
+
+#include "common.h"
+
+namespace wisp {
+namespace mx {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kBlock = 32;        // values of one scale
+constexpr int kBlockBytes = 16;   // their codes
+
+// The conversions' scale operand for byte `q` (0..3) of a word of scale bytes.
+__device__ inline float scale_of(uint32_t word, int q) {
+  return __uint_as_float(((word >> (8 * q)) & 0xffu) << 23);
+}
+
+// The eight bf16 values of a word of codes.
+__device__ __attribute__((always_inline)) inline bf16x8 bf16_of(uint32_t codes, float scale) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+}  // namespace mx
+}  // namespace wisp
