@@ -228,7 +228,9 @@ int wisp_dequant_mxfp4(const uint8_t* codes, const uint8_t* scales, int64_t rows
  * float32, act and out are rounded once.  W13 of slot s: codes at
  * w13 + s*w13_stride ([2I, H/2]), scales at s13 + s*s13_stride ([2I, H/32]);
  * W2 [H, I/2] and s2 [H, I/32] likewise; strides in bytes.  H and I must be
- * multiples of 32, H*I below 2^31, weights and their strides 16-byte aligned.
+ * multiples of 32, H*I below 2^31, weights and their strides 16-byte aligned,
+ * scales and their strides 4-byte aligned (the aligned words that hold an
+ * expert's scale bytes are read whole).
  * A slot outside [0, nslots) contributes zero.  act: T*K*I elements; work:
  * device, 256-byte aligned, wisp_moe_mxfp4_work_bytes(T, K, H, nslots)
  * bytes. */

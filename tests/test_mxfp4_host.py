@@ -56,6 +56,7 @@ def _experts(lib, T=2, H=64, I=32, K=2, nslots=4, w13s=None, s13s=None, w2s=None
     (dict(x=P + 2), UNSUPPORTED), (dict(out=P + 8), UNSUPPORTED), (dict(w13=P + 4), UNSUPPORTED),
     (dict(w13s=64 * 32 + 8), UNSUPPORTED), (dict(w13s=64 * 32 - 16), INVALID),
     (dict(w2s=64 * 16 - 16), INVALID), (dict(s13s=64), INVALID), (dict(s2s=32), INVALID),
+    (dict(s13s=130), UNSUPPORTED), (dict(s2s=66), UNSUPPORTED),
     (dict(work=None), INVALID), (dict(work=P + 16), INVALID), (dict(work_bytes=64), INVALID),
     (dict(T=1 << 26, K=64), INVALID),
 ])

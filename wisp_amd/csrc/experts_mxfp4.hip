@@ -24,21 +24,23 @@ using mx::bf16x8;
 using mx::f32x4;
 using mx::u32x4;
 
-constexpr int kChunk = 128;               // k columns of a step: four blocks of each row
-constexpr int kTokBytes = kChunk * 2;     // of a token row
+constexpr int kChunk = 128;               // k columns of a chunk: four blocks of each row
+constexpr int kSub = 2;                   // chunks of a stage
+constexpr int kStageK = kSub * kChunk;    // k columns of a stage: 128 bytes of a row's codes
+constexpr int kTokBytes = kChunk * 2;     // of a token row, a chunk
 constexpr int kTokPerCopy = 1024 / kTokBytes;
 
-// A block of WR x WT waves: wave (wr, wt) holds NG tiles of 16 weight rows
-// and the NT token tiles of 16 from wt * NT on.
-template <int WR_, int WT_, int NG_, int NT_>
+// A block of WR waves: each holds NG tiles of 16 weight rows against NT token
+// tiles of 16.
+template <int WR_, int NG_, int NT_>
 struct Shape {
-  static constexpr int WR = WR_, WT = WT_, NG = NG_, NT = NT_;
-  static constexpr int kWaves = WR * WT;
+  static constexpr int WR = WR_, NG = NG_, NT = NT_;
   static constexpr int kRows = WR * NG * 16;
-  static constexpr int kToks = WT * NT * 16;
-  static constexpr int kCopies = kToks / kTokPerCopy / kWaves;  // per wave and chunk
-  static_assert(kCopies * kTokPerCopy * kWaves == kToks, "token copies split evenly");
-  static constexpr int kStage = kToks * kTokBytes;
+  static constexpr int kToks = NT * 16;                   // of a pass
+  static constexpr int NC = kToks / kTokPerCopy / WR;     // token copies of a wave and chunk
+  static_assert(NC * kTokPerCopy * WR == kToks, "token copies split evenly");
+  static constexpr int kPart = kToks * kTokBytes;         // a chunk's tokens
+  static constexpr int kWaveW = NG * 16 * 128;            // a wave's codes of a stage
 };
 
 struct GroupedArgs {
@@ -53,13 +55,6 @@ struct GroupedArgs {
   void* out;
 };
 
-// The weights of one chunk: a lane's block of each of its row tiles.
-template <int NG>
-struct Weights {
-  u32x4 w[NG];
-  uint32_t s[NG];
-};
-
 // bf16(silu(g) * u) of four consecutive columns, one 8-byte store at p.
 __device__ inline void store_act4(uint16_t* p, const f32x4& g, const f32x4& u) {
   uint32_t h[4];
@@ -68,98 +63,174 @@ __device__ inline void store_act4(uint16_t* p, const f32x4& g, const f32x4& u) {
   *reinterpret_cast<uint2*>(p) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
-// Grid (panel, slot).  Lane l of a wave feeds row l % 16 of a tile, block
-// l / 16 of the chunk: its 16 bytes of codes are the operands of four matrix
-// instructions, step j over k = 32 (l / 16) + 8 j .. + 7.  Token rows are
-// staged in LDS, 256 bytes of each a chunk, 16-byte piece b of row r at
-// position b ^ (r % 16).
-template <typename Sh, bool kW13, bool kTail>
-__global__ __launch_bounds__(64 * Sh::kWaves) void mx_grouped_kernel(GroupedArgs a) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-  constexpr int NG = Sh::NG, NT = Sh::NT;
-  const int s = blockIdx.y;
-  const int M = a.counts[s];
-  if (M == 0) return;
-  const int32_t* list = a.lists + (size_t)s * a.P;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int wr = wave / Sh::WT, wt = wave % Sh::WT, q = lane >> 4;
-  const int Kdim = kW13 ? a.H : a.I, nblk = Kdim / mx::kBlock;
-  const int chunks = (nblk + 3) / 4;
-  // first output column of row tile g, and how many columns there are
-  const int N = kW13 ? a.I : a.H;
-  constexpr int per = kW13 ? NG / 2 : NG;  // tiles of output columns
-  const int n0 = (blockIdx.x * Sh::WR + wr) * per * 16;
-  const uint8_t* W = a.W + (size_t)s * a.w_stride;
-  const uint8_t* S = a.S + (size_t)s * a.s_stride;
-  uint32_t row[NG];
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    const int n = min(n0 + g % per * 16, N - 16);  // tiles past the end repeat the last
-    row[g] = (uint32_t)((g < per ? 0 : a.I) + n + (lane & 15)) * (uint32_t)nblk;
+// One block's products for the tokens of one slot, a pass of up to kToks of
+// them at a time, in stages of 256 k columns.
+//
+// Weights go through registers one stage ahead: eight lanes read the 128
+// bytes of a row (lanes that each read a row of their own, as the matrix
+// operand wants them, cost the address unit 64 cycles a load instead of 16
+// and hold a stream of weights at 3 TB/s), then into the wave's own part of
+// LDS, 16-byte block b of row r at position b ^ (r % 8), and back in operand
+// order: lane l holds row l % 16 of a tile, block l / 16 of a chunk, the
+// operands of four matrix instructions, step j over
+// k = 32 (l / 16) + 8 j .. + 7.  Lane l loads the scales of the wave's row l.
+//
+// Token rows are copied to LDS asynchronously one chunk ahead, 256 bytes of
+// each, 16-byte piece b of row r at position b ^ (r % 16).
+//
+// kOdd: rows that are not whole stages.  Blocks past a row's end read as
+// zeros, and each lane loads its own blocks' scales.
+template <typename Sh, bool kW13, bool kOdd>
+struct Tile {
+  static constexpr int NG = Sh::NG, NT = Sh::NT, NC = Sh::NC;
+  static constexpr int per = kW13 ? NG / 2 : NG;  // tiles of output columns of a wave
+  static constexpr int NL = 2 * NG;               // code loads of a stage
+  static constexpr int NS = kOdd ? kSub * NG : kSub;  // words of scales
+  static constexpr int kLoads = NL + (kOdd ? NS : 1);
+  static_assert(NG == 4, "a lane for each weight row of the wave");
+  const GroupedArgs& a;
+  unsigned char* tlds;
+  unsigned char* wlds;  // this wave's
+  const int32_t* list;
+  int wave, lane, q, Kdim, nblk, chunks, N, n0;
+  mx::Buffer W, S;    // the slot's codes and scales
+  uint32_t tile0[NG]; // first weight row of each tile (wave-uniform)
+
+  // Byte of the scale of this lane's block of chunk c in tile g (kOdd).
+  __device__ __attribute__((always_inline)) uint32_t scale_at(int g, int c) const {
+    return (tile0[g] + (lane & 15)) * (uint32_t)nblk + max(min(c * 4 + q, nblk - 1), 0);
   }
-  auto load = [&](int c, Weights<NG>& b) {
-    const int blk = kTail ? min(c * 4 + q, nblk - 1) : c * 4 + q;
+
+  // A stage's codes, row 8 (n % 2) + l / 8 of tile n / 2, and scale words.
+  struct Weights {
+    u32x4 w[NL];
+    uint32_t s[NS];
+  };
+  __device__ __attribute__((always_inline)) void load(int c, Weights& b) const {
+    const uint32_t rowb = (uint32_t)nblk * mx::kBlockBytes;
+    const int blk = c * 4 + (lane & 7);
+    // (nothing past a row's end, also in the stage after the last)
+    const uint32_t v = blk < nblk ? (uint32_t)(lane >> 3) * rowb + blk * mx::kBlockBytes : 1u << 31;
+#pragma unroll
+    for (int n = 0; n < NL; ++n)
+      b.w[n] = mx::load16_nt(W, v, (tile0[n / 2] + n % 2 * 8) * rowb);
+    if constexpr (kOdd) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        b.s[i] = mx::load4(S, scale_at(i / kSub, c + i % kSub) & ~3u);
+      }
+    } else {
+      const uint32_t at = (tile0[0] + (lane & 15)) * (uint32_t)nblk;
+      uint32_t row = at;
+#pragma unroll
+      for (int g = 1; g < NG; ++g)
+        row = q == g ? at + (tile0[g] - tile0[0]) * (uint32_t)nblk : row;
+      const auto two = mx::load8(S, c < chunks ? row + c * 4 : 1u << 31);
+      b.s[0] = two[0], b.s[1] = two[1];
+    }
+  }
+
+  // Token copies of a pass: this lane's source pieces of chunk 0.
+  struct Tokens {
+    const unsigned char* src[NC];
+    int piece[NC];  // with kOdd
+  };
+  __device__ __attribute__((always_inline)) void copy(int c, const Tokens& t,
+                                                      unsigned char* stage) const {
+    if (c >= chunks) return;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      // (pieces past a row's end repeat its last; their products are not used)
+      const int b = kOdd ? min(c * 16 + t.piece[i], Kdim / 8 - 1) - t.piece[i] : c * 16;
+      dma::dma16(t.src[i] + (ptrdiff_t)b * 16, stage + (i * Sh::WR + wave) * 1024);
+    }
+  }
+
+  // Half h of the stage from chunk c on, its tokens in rds; the copies of the
+  // next chunk's tokens into wrs are under way meanwhile, and with h = 0 the
+  // next stage's weights into w.  (wrs and rds are distinct, which the
+  // compiler has to know.  It also tells only eight copy instructions of a
+  // kernel apart, and waits for all copies before an LDS read if there are
+  // more: hence one place for all copies, with a turn of the loop for the
+  // first.)
+  template <int h>
+  __device__ __attribute__((always_inline)) void half(int c, unsigned char* __restrict__ wrs,
+                                                      const unsigned char* __restrict__ rds,
+                                                      const Tokens& tok, const uint32_t (&s)[NS],
+                                                      Weights& w, f32x4 (&acc)[NG][NT]) const {
+    // this chunk's tokens have landed: all loads but the youngest, the weights
+    dma::wait_vm<h == 0 ? 0 : kLoads>();
+    dma::lds_barrier();
+    if (c + h >= -1) copy(c + h + 1, tok, wrs);
+    if constexpr (h == 0) load(c + kSub, w);
+    if (c + h < 0 || c + h >= chunks) return;
+    u32x4 codes[NG];
+    uint32_t scale[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      b.w[g] = __builtin_nontemporal_load(
-          reinterpret_cast<const u32x4*>(W + (size_t)(row[g] + blk) * mx::kBlockBytes));
-      b.s[g] = S[row[g] + blk];
+      codes[g] = *reinterpret_cast<const u32x4*>(wlds + (g * 16 + (lane & 15)) * 128 +
+                                                 (((h * 4 + q) ^ (lane & 7)) << 4));
+      scale[g] = kOdd ? mx::scale_of(s[g * kSub + h], scale_at(g, c + h) & 3)
+                      : mx::scale_of(__shfl((int)s[h], g * 16 + (lane & 15)), q);
     }
-  };
-  for (int m0 = 0; m0 < M; m0 += Sh::kToks) {
-    const int mrows = min(M - m0, Sh::kToks);
-    const unsigned char* src[Sh::kCopies];
-    int piece[Sh::kCopies];
+    const bool none = kOdd && (c + h) * 4 + q >= nblk;
 #pragma unroll
-    for (int i = 0; i < Sh::kCopies; ++i) {
-      const int r = (i * Sh::kWaves + wave) * kTokPerCopy + (lane >> 4);
-      const int p = list[m0 + min(r, mrows - 1)];
-      src[i] = reinterpret_cast<const unsigned char*>(a.A + (size_t)(kW13 ? p / a.K : p) * Kdim);
-      piece[i] = (lane & 15) ^ (r & 15);
-    }
-    auto copy = [&](int c, unsigned char* stage) {
+    for (int j = 0; j < 4; ++j) {
+      bf16x8 t[NT];
 #pragma unroll
-      for (int i = 0; i < Sh::kCopies; ++i) {
-        const int b = kTail ? min(c * 16 + piece[i], Kdim / 8 - 1) : c * 16 + piece[i];
-        dma::dma16(src[i] + (size_t)b * 16, stage + (i * Sh::kWaves + wave) * 1024);
+      for (int i = 0; i < NT; ++i) {
+        t[i] = *reinterpret_cast<const bf16x8*>(rds + (i * 16 + (lane & 15)) * kTokBytes +
+                                                (((q * 4 + j) ^ (lane & 15)) << 4));
+        if (none) t[i] = bf16x8{};  // what is there may be an infinity
       }
-    };
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const bf16x8 v = mx::bf16_of(codes[g][j], __uint_as_float(scale[g]));
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          acc[g][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, t[i], acc[g][i], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  __device__ __attribute__((always_inline)) void step(int c, const Tokens& tok, Weights& w,
+                                                      f32x4 (&acc)[NG][NT]) const {
+    uint32_t s[NS];
+    if (c >= 0) {
+#pragma unroll
+      for (int n = 0; n < NL; ++n) {
+        const int r = n * 8 + (lane >> 3);
+        *reinterpret_cast<u32x4*>(wlds + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = w.w[n];
+      }
+#pragma unroll
+      for (int i = 0; i < NS; ++i) s[i] = w.s[i];
+    }
+    half<0>(c, tlds + Sh::kPart, tlds, tok, s, w, acc);
+    half<1>(c, tlds, tlds + Sh::kPart, tok, s, w, acc);
+  }
+
+  __device__ __attribute__((always_inline)) void pass(int m0, int mrows) const {
+    Weights w;
+    Tokens tok;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int r = (i * Sh::WR + wave) * kTokPerCopy + (lane >> 4);
+      const int p = list[m0 + min(r, mrows - 1)];
+      tok.piece[i] = (lane & 15) ^ (r & 15);
+      tok.src[i] = reinterpret_cast<const unsigned char*>(
+          a.A + (size_t)(kW13 ? p / a.K : p) * Kdim + tok.piece[i] * 8);
+    }
     f32x4 acc[NG][NT];
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
       for (int t = 0; t < NT; ++t) acc[g][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Weights<NG> w;
-    for (int c = 0; c < chunks; ++c) {
-      copy(c, lds);
-      load(c, w);
-      dma::wait_vm<0>();
-      dma::lds_barrier();
-      const bool none = kTail && c * 4 + q >= nblk;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        bf16x8 t[NT];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          const int r = (wt * NT + i) * 16 + (lane & 15);
-          t[i] = *reinterpret_cast<const bf16x8*>(lds + r * kTokBytes +
-                                                  (((q * 4 + j) ^ (lane & 15)) << 4));
-          if (none) t[i] = bf16x8{};
-        }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const bf16x8 v =
-              mx::bf16_of(none ? 0u : w.w[g][j], __uint_as_float((none ? 0u : w.s[g]) << 23));
-#pragma unroll
-          for (int i = 0; i < NT; ++i)
-            acc[g][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, t[i], acc[g][i], 0, 0, 0);
-        }
-      }
-      dma::lds_barrier();
-    }
+#pragma unroll 1
+    for (int c = -kSub; c < chunks; c += kSub) step(c, tok, w, acc);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const int r = (wt * NT + i) * 16 + (lane & 15);
+      const int r = i * 16 + (lane & 15);
       if (r >= mrows) continue;
       const int p = list[m0 + r];
 #pragma unroll
@@ -173,21 +244,64 @@ __global__ __launch_bounds__(64 * Sh::kWaves) void mx_grouped_kernel(GroupedArgs
       }
     }
   }
+};
+
+// Grid (panel, slot).
+template <typename Sh, bool kW13, bool kOdd>
+__global__ __launch_bounds__(64 * Sh::WR) __attribute__((amdgpu_waves_per_eu(Sh::NT < 4 ? 3 : 2))) void
+mx_grouped_kernel(GroupedArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char tlds[];
+  __shared__ __attribute__((aligned(16))) unsigned char wlds[Sh::WR * Sh::kWaveW];
+  const int s = blockIdx.y;
+  const int M = a.counts[s];
+  if (M == 0) return;
+  Tile<Sh, kW13, kOdd> t{a, tlds};
+  t.list = a.lists + (size_t)s * a.P;
+  t.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  t.wlds = wlds + t.wave * Sh::kWaveW;
+  t.lane = threadIdx.x & 63;
+  t.q = t.lane >> 4;
+  t.Kdim = kW13 ? a.H : a.I, t.nblk = t.Kdim / mx::kBlock;
+  t.chunks = (t.nblk + 3) / 4;
+  t.N = kW13 ? a.I : a.H;
+  t.n0 = (blockIdx.x * Sh::WR + t.wave) * t.per * 16;
+  const uint32_t blocks = (uint32_t)(kW13 ? 2 * a.I : a.H) * (uint32_t)t.nblk;
+  t.W = mx::buffer(a.W + (size_t)s * a.w_stride, blocks * mx::kBlockBytes);
+  t.S = mx::buffer(a.S + (size_t)s * a.s_stride, (blocks + 3) & ~3u);
+#pragma unroll
+  for (int g = 0; g < Sh::NG; ++g)  // (tiles past the end repeat the last)
+    t.tile0[g] = (g < t.per ? 0 : a.I) + min(t.n0 + g % t.per * 16, t.N - 16);
+#pragma unroll 1
+  for (int m0 = 0; m0 < M; m0 += Sh::kToks) t.pass(m0, min(M - m0, Sh::kToks));
 }
 
-using Mid = Shape<4, 1, 4, 4>;
+template <typename Sh, bool kW13, bool kOdd>
+hipError_t launch_grouped(const GroupedArgs& a, dim3 grid, hipStream_t st, hipEvent_t e0,
+                          hipEvent_t e1) {
+  constexpr unsigned lds = 2 * Sh::kPart;
+  static_assert(lds + Sh::WR * Sh::kWaveW <= 160 * 1024, "LDS per block");
+  static std::atomic<uint64_t> big{0};
+  const hipError_t e =
+      allow_lds(&mx_grouped_kernel<Sh, kW13, kOdd>, lds + Sh::WR * Sh::kWaveW, lds, &big);
+  if (e != hipSuccess) return e;
+  launch_timed_lds(mx_grouped_kernel<Sh, kW13, kOdd>, grid, dim3(64 * Sh::WR), lds, st, e0, e1, a);
+  return hipSuccess;
+}
 
 template <bool kW13>
-void launch_grouped(const GroupedArgs& a, int nslots, hipStream_t st, hipEvent_t e0,
-                    hipEvent_t e1) {
-  const int cols = kW13 ? a.I : a.H, per = kW13 ? Mid::kRows / 2 : Mid::kRows;
-  const dim3 grid((cols + per - 1) / per, nslots);
-  if ((kW13 ? a.H : a.I) % kChunk)
-    launch_timed_lds(mx_grouped_kernel<Mid, kW13, true>, grid, dim3(64 * Mid::kWaves), Mid::kStage,
-                     st, e0, e1, a);
-  else
-    launch_timed_lds(mx_grouped_kernel<Mid, kW13, false>, grid, dim3(64 * Mid::kWaves),
-                     Mid::kStage, st, e0, e1, a);
+hipError_t launch_product(const GroupedArgs& a, int nslots, hipStream_t st, hipEvent_t e0,
+                          hipEvent_t e1) {
+  const int spread = std::min(a.P, nslots);
+  auto go = [&](auto shape) {
+    using Sh = decltype(shape);
+    constexpr int per = Sh::kRows / (kW13 ? 2 : 1);
+    const dim3 grid(((kW13 ? a.I : a.H) + per - 1) / per, nslots);
+    return (kW13 ? a.H : a.I) % kStageK ? launch_grouped<Sh, kW13, true>(a, grid, st, e0, e1)
+                                        : launch_grouped<Sh, kW13, false>(a, grid, st, e0, e1);
+  };
+  if (a.P <= 8 * spread) return go(Shape<4, 4, 1>{});
+  if (a.P <= 20 * spread) return go(Shape<4, 4, 2>{});
+  return go(Shape<4, 4, 4>{});
 }
 
 // Work buffer: the layout of the bf16 grouped GEMM's (pair lists, counts, y).
@@ -236,8 +350,10 @@ int experts_mxfp4(const void* x, int T, int H, int I, int K, const float* topk_w
                         w13_stride, (const uint8_t*)s13, s13_stride, act};
   const GroupedArgs a2{(const uint16_t*)act, H, I, K, P, lists, counts, (const uint8_t*)w2,
                        w2_stride, (const uint8_t*)s2, s2_stride, (char*)work + wk.y};
-  launch_grouped<true>(a13, nslots, st, ev ? ev->ev[0] : nullptr, ev ? ev->ev[1] : nullptr);
-  launch_grouped<false>(a2, nslots, st, ev ? ev->ev[2] : nullptr, ev ? ev->ev[3] : nullptr);
+  WISP_HIP_TRY((launch_product<true>(a13, nslots, st, ev ? ev->ev[0] : nullptr,
+                                     ev ? ev->ev[1] : nullptr)));
+  WISP_HIP_TRY((launch_product<false>(a2, nslots, st, ev ? ev->ev[2] : nullptr,
+                                      ev ? ev->ev[3] : nullptr)));
   WISP_HIP_TRY(hipGetLastError());
   return experts_mfma_combine(T, H, K, topk_w, slots, nslots, work, out, st);
 }
@@ -259,8 +375,10 @@ int check_call(const void* x, int T, int H, int I, int K, int nslots, const void
   }
   const char* why = mxfp4_unsupported(H, I, K);
   if (!why && ((uintptr_t)w13 % 16 || (uintptr_t)w2 % 16 || w13_stride % 16 || w2_stride % 16 ||
-               (uintptr_t)x % 16 || (uintptr_t)act % 16 || (uintptr_t)out % 16))
-    why = "weights, their strides and the activations must be 16-byte aligned";
+               (uintptr_t)x % 16 || (uintptr_t)act % 16 || (uintptr_t)out % 16 ||
+               (uintptr_t)s13 % 4 || (uintptr_t)s2 % 4 || s13_stride % 4 || s2_stride % 4))
+    why = "weights, their strides and the activations must be 16-byte aligned, scales and their "
+          "strides 4-byte";
   if (why) {
     wisp_set_last_error(why, where);
     return WISP_ERR_UNSUPPORTED;

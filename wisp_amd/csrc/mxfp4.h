@@ -19,14 +19,16 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBlock = 32;        // values of one scale
 constexpr int kBlockBytes = 16;   // their codes
 
-// The conversions' scale operand for byte `q` (0..3) of a word of scale bytes.
-__device__ inline float scale_of(uint32_t word, int q) {
-  return __uint_as_float(((word >> (8 * q)) & 0xffu) << 23);
+// The bits of the conversions' scale operand for byte `q` (0..3) of a word of
+// scale bytes.
+__device__ inline uint32_t scale_of(uint32_t word, int q) {
+  return ((word >> (8 * q)) & 0xffu) << 23;
 }
 
 // The eight bf16 values of a word of codes.
@@ -38,5 +40,31 @@ __device__ __attribute__((always_inline)) inline bf16x8 bf16_of(uint32_t codes, 
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// A range of less than 2^31 bytes of device memory, read by 32-bit byte
+// offsets (`off`, a lane's, plus `base`, the wave's, which lies in the range);
+// a read at or past the range's end gives zeros and touches no memory.
+#ifdef __HIP_DEVICE_COMPILE__
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __attribute__((always_inline)) inline Buffer buffer(const void* p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00027000);
+}
+__device__ __attribute__((always_inline)) inline u32x4 load16_nt(Buffer b, uint32_t off,
+                                                                   uint32_t base) {
+  // nt: each byte is read once
+  return __builtin_amdgcn_raw_buffer_load_b128(b, (int)off, (int)base, 2);
+}
+__device__ __attribute__((always_inline)) inline u32x2 load8(Buffer b, uint32_t off) {
+  return __builtin_amdgcn_raw_buffer_load_b64(b, (int)off, 0, 0);
+}
+__device__ __attribute__((always_inline)) inline uint32_t load4(Buffer b, uint32_t off) {
+  return __builtin_amdgcn_raw_buffer_load_b32(b, (int)off, 0, 0);
+}
+#else  // the host pass does not know these builtins
+struct Buffer {};
+__device__ inline Buffer buffer(const void*, uint32_t) { return {}; }
+__device__ inline u32x4 load16_nt(Buffer, uint32_t, uint32_t) { return {}; }
+__device__ inline u32x2 load8(Buffer, uint32_t) { return {}; }
+__device__ inline uint32_t load4(Buffer, uint32_t) { return 0; }
+#endif
 }  // namespace mx
 }  // namespace wisp
