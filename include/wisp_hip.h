@@ -232,7 +232,7 @@ int wisp_dequant_mxfp4(const uint8_t* codes, const uint8_t* scales, int64_t rows
  * scales and their strides 4-byte aligned (the aligned words that hold an
  * expert's scale bytes are read whole).
  * A slot outside [0, nslots) contributes zero.  act: T*K*I elements; work:
- * device, 256-byte aligned, wisp_moe_mxfp4_work_bytes(T, K, H, nslots)
+ * device, 256-byte aligned, wisp_moe_mxfp4_work_bytes(T, K, H, I, nslots)
  * bytes. */
 int wisp_moe_experts_mxfp4(const void* x, int T, int H, int I, int K, const float* topk_w,
                            const int32_t* slots, int nslots, const void* w13, size_t w13_stride,
@@ -251,8 +251,8 @@ int wisp_moe_layer_mxfp4(const void* x, const void* logits, int logits_dtype, in
                          wisp_stream_t stream);
 
 /* Bytes of the work buffer of the MXFP4 experts (pair lists and fp32 per-pair
- * outputs). */
-size_t wisp_moe_mxfp4_work_bytes(int T, int K, int H, int nslots);
+ * outputs; for a few tokens act in float32).  Not monotone in T. */
+size_t wisp_moe_mxfp4_work_bytes(int T, int K, int H, int I, int nslots);
 
 /* Bytes of the device array wisp_moe_experts_noalloc works in, per GPU, in
  * a default build; building with WISP_NOALLOC_SCRATCH_MIB=n sets n MiB, and

@@ -105,27 +105,24 @@ def _check_weights(x, w13, w2, s13, s2) -> tuple[int, int, int]:
     H = x.shape[1]
     E, I = w13.shape[0], 2 * w2.shape[2]
     dev = x.device
-    for t, name, shape in ((w13, "w13", (E, 2 * I, H // 2)), (w2, "w2", (E, H, I // 2)),
-                           (s13, "s13", (E, 2 * I, H // BLOCK)), (s2, "s2", (E, H, I // BLOCK))):
-        if t.dtype != torch.uint8 or t.shape != shape:
-            raise ValueError(f"wisp.mxfp4: {name} must be a uint8 {shape} tensor")
+    for t, name, rows, cols in ((w13, "w13", 2 * I, H // 2), (w2, "w2", H, I // 2),
+                                (s13, "s13", 2 * I, H // BLOCK), (s2, "s2", H, I // BLOCK)):
+        if t.dtype != torch.uint8 or t.shape != (E, rows, cols):
+            raise ValueError(f"wisp.mxfp4: {name} must be a uint8 {(E, rows, cols)} tensor")
         if t.device != dev:
             _require_device(t, dev, name)
-        st = t.stride()
-        if st[2] != 1 or st[1] != shape[2]:
+        if not t.is_contiguous() and (t.stride(2) != 1 or t.stride(1) != cols):
             raise ValueError(f"wisp.mxfp4: each expert of {name} must be contiguous")
     return E, H, I
 
 
-def _buffers(x, T, K, H, I, nslots):
-    """act and the work buffer of one call, in one allocation of its own (so
-    that calls on other streams, or captured into other graphs, share
-    nothing): ``(tensor, act address, work address, work bytes)``."""
-    act = -(-T * K * I * 2 // 256) * 256
-    nbytes = lib().wisp_moe_mxfp4_work_bytes(T, K, H, nslots)
-    buf = torch.empty(act + nbytes, dtype=torch.uint8, device=x.device)
-    p = buf.data_ptr()
-    return buf, p, p + act, nbytes
+@functools.lru_cache(maxsize=256)
+def _layout(T: int, K: int, H: int, I: int, nslots: int) -> tuple[int, int, int]:
+    """Byte offset of a call's routing and work buffer behind its act, and the
+    work buffer's size."""
+    routing = -(-T * K * I * 2 // 256) * 256
+    work = routing + -(-T * K * 8 // 256) * 256
+    return routing, work, lib().wisp_moe_mxfp4_work_bytes(T, K, H, I, nslots)
 
 
 def _output(x, out):
@@ -155,11 +152,15 @@ def experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, slots: torch.Tensor, w1
     out = _output(x, out)
     if T == 0:
         return out
-    buf, act, work, nbytes = _buffers(x, T, K, H, I, E)
+    # one allocation of the call's own, so that calls on other streams, or
+    # captured into other graphs, share nothing
+    _, work, nbytes = _layout(T, K, H, I, E)
+    buf = torch.empty(work + nbytes, dtype=torch.uint8, device=x.device)
+    p = buf.data_ptr()
     check(lib().wisp_moe_experts_mxfp4(
         x.data_ptr(), T, H, I, K, topk_w.data_ptr(), slots.data_ptr(), E, w13.data_ptr(),
         w13.stride(0), s13.data_ptr(), s13.stride(0), w2.data_ptr(), w2.stride(0), s2.data_ptr(),
-        s2.stride(0), act, out.data_ptr(), work, nbytes, _lib.stream_handle()), "experts_mxfp4")
+        s2.stride(0), p, out.data_ptr(), p + work, nbytes, _lib.stream_handle()), "experts_mxfp4")
     return out
 
 
@@ -184,13 +185,14 @@ def route_and_experts_mxfp4(x: torch.Tensor, router_logits: torch.Tensor, top_k:
     out = _output(x, out)
     if T == 0:
         return out
-    buf, act, work, nbytes = _buffers(x, T, K, H, I, E)
-    routing = torch.empty(2 * T * K, dtype=torch.int32, device=x.device)
+    routing, work, nbytes = _layout(T, K, H, I, E)
+    buf = torch.empty(work + nbytes, dtype=torch.uint8, device=x.device)  # as above
+    p = buf.data_ptr()
     check(lib().wisp_moe_layer_mxfp4(
         x.data_ptr(), router_logits.data_ptr(), _DTYPES[router_logits.dtype], T, H, I, E, K,
-        int(bool(renormalize)), routing.data_ptr(), routing.data_ptr() + 4 * T * K,
+        int(bool(renormalize)), p + routing, p + routing + 4 * T * K,
         w13.data_ptr(), w13.stride(0), s13.data_ptr(), s13.stride(0), w2.data_ptr(), w2.stride(0),
-        s2.data_ptr(), s2.stride(0), act, out.data_ptr(), work, nbytes, _lib.stream_handle()),
+        s2.data_ptr(), s2.stride(0), p, out.data_ptr(), p + work, nbytes, _lib.stream_handle()),
         "route_and_experts_mxfp4")
     return out
 

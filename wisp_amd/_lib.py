@@ -110,7 +110,7 @@ SIGNATURES = {
     "wisp_moe_layer_mxfp4": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp,
                                     _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz,
                                     _vp]),
-    "wisp_moe_mxfp4_work_bytes": (_sz, [_i32, _i32, _i32, _i32]),
+    "wisp_moe_mxfp4_work_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32]),
     "wisp_layer_create": (_i32, [C.POINTER(LayerDesc), C.POINTER(_vp)]),
     "wisp_layer_destroy": (_i32, [_vp]),
     "wisp_layer_set_scratch": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp]),
@@ -186,5 +186,8 @@ def ptr(t) -> int | None:
 
 def stream_handle(stream=None) -> int:
     import torch
-    s = torch.cuda.current_stream() if stream is None else stream
-    return s.cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    # the raw handle: a torch.cuda.Stream object costs several microseconds,
+    # as long as a small call's kernels
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())

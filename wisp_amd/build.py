@@ -26,6 +26,7 @@ SOURCES = [
     "experts_mfma.hip",
     "experts_fp8.hip",
     "experts_mxfp4.hip",
+    "experts_mxfp4_few.hip",
     "quant_mxfp4.hip",
     "pagein.hip",
     "packed.hip",

@@ -17,6 +17,13 @@ namespace wisp {
 int experts_mfma_combine(int T, int H, int K, const float* topk_w, const int32_t* slots,
                          int nslots, const void* work, void* out, hipStream_t st);
 size_t mfma_work_bytes(int T, int K, int H, int nslots);
+bool mxfp4_few(int T, int K, int H, int I);
+size_t mxfp4_few_bytes(int P, int I);
+int mxfp4_few_layer(const void* x, const void* logits, int logits_dtype, int renorm,
+                    int64_t* forward, int T, int H, int I, int K, float* topk_w, int32_t* slots,
+                    int nslots, const void* w13, size_t w13_stride, const void* s13,
+                    size_t s13_stride, const void* w2, size_t w2_stride, const void* s2,
+                    size_t s2_stride, void* act, void* out, hipStream_t st, const StageEvents* ev);
 
 namespace {
 
@@ -317,8 +324,9 @@ struct Work {
 
 }  // namespace
 
-size_t mxfp4_work_bytes(int T, int K, int H, int nslots) {
-  return mfma_work_bytes(T, K, H, nslots);
+size_t mxfp4_work_bytes(int T, int K, int H, int I, int nslots) {
+  if (T < 1 || K < 1 || H < 1 || I < 1 || nslots < 1) return 0;
+  return mxfp4_few(T, K, H, I) ? mxfp4_few_bytes(T * K, I) : mfma_work_bytes(T, K, H, nslots);
 }
 
 // Why the MXFP4 kernels do not cover a call, or null.
@@ -330,17 +338,30 @@ const char* mxfp4_unsupported(int H, int I, int K) {
   return nullptr;
 }
 
+namespace {
+
+int check_work(int T, int K, int H, int I, int nslots, const void* work, size_t work_bytes) {
+  if (nslots <= 65535 && work && work_bytes >= mxfp4_work_bytes(T, K, H, I, nslots) &&
+      (uintptr_t)work % 256 == 0)
+    return WISP_OK;
+  wisp_set_last_error("work buffer missing, misaligned or too small", "MXFP4 experts");
+  return WISP_ERR_INVALID;
+}
+
+}  // namespace
+
 int experts_mxfp4(const void* x, int T, int H, int I, int K, const float* topk_w,
                   const int32_t* slots, int nslots, const void* w13, size_t w13_stride,
                   const void* s13, size_t s13_stride, const void* w2, size_t w2_stride,
                   const void* s2, size_t s2_stride, void* act, void* out, void* work,
                   size_t work_bytes, hipStream_t st, const StageEvents* ev) {
   if (T == 0) return WISP_OK;
-  if (nslots > 65535 || !work || work_bytes < mxfp4_work_bytes(T, K, H, nslots) ||
-      ((uintptr_t)work) % 256) {
-    wisp_set_last_error("work buffer missing, misaligned or too small", "MXFP4 experts");
-    return WISP_ERR_INVALID;
-  }
+  const int rc = check_work(T, K, H, I, nslots, work, work_bytes);
+  if (rc != WISP_OK) return rc;
+  if (mxfp4_few(T, K, H, I))
+    return mxfp4_few_layer(x, nullptr, 0, 0, nullptr, T, H, I, K, const_cast<float*>(topk_w),
+                           const_cast<int32_t*>(slots), nslots, w13, w13_stride, s13, s13_stride,
+                           w2, w2_stride, s2, s2_stride, work, out, st, ev);
   const int P = T * K;
   const Work wk(P, nslots);
   int32_t* lists = (int32_t*)((char*)work + wk.lists);
@@ -394,8 +415,8 @@ int check_call(const void* x, int T, int H, int I, int K, int nslots, const void
 
 }  // namespace
 
-extern "C" size_t wisp_moe_mxfp4_work_bytes(int T, int K, int H, int nslots) {
-  return wisp::mxfp4_work_bytes(T, K, H, nslots);
+extern "C" size_t wisp_moe_mxfp4_work_bytes(int T, int K, int H, int I, int nslots) {
+  return wisp::mxfp4_work_bytes(T, K, H, I, nslots);
 }
 
 extern "C" int wisp_moe_experts_mxfp4(const void* x, int T, int H, int I, int K,
@@ -430,6 +451,14 @@ extern "C" int wisp_moe_layer_mxfp4(const void* x, const void* logits, int logit
   int rc = check_call(x, T, H, I, K, E, w13, w13_stride, s13, s13_stride, w2, w2_stride, s2,
                       s2_stride, act, out, where);
   if (rc != WISP_OK) return rc;
+  if (T > 0 && E <= kMaxExperts && K <= E && logits && topk_w && topk_ids &&
+      (logits_dtype == WISP_F32 || logits_dtype == WISP_BF16) && mxfp4_few(T, K, H, I)) {
+    rc = check_work(T, K, H, I, E, work, work_bytes);
+    if (rc != WISP_OK) return rc;
+    return mxfp4_few_layer(x, logits, logits_dtype, renormalize, nullptr, T, H, I, K, topk_w,
+                           topk_ids, E, w13, w13_stride, s13, s13_stride, w2, w2_stride, s2,
+                           s2_stride, work, out, (hipStream_t)stream, nullptr);
+  }
   rc = wisp_route_topk_softmax(logits, logits_dtype, T, E, K, renormalize, topk_w, topk_ids,
                                nullptr, stream);
   if (rc != WISP_OK) return rc;

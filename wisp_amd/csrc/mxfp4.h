@@ -40,6 +40,33 @@ __device__ __attribute__((always_inline)) inline bf16x8 bf16_of(uint32_t codes, 
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// The same values two and two, and as float32.
+struct Pairs {
+  bf16x2 p[4];
+};
+__device__ __attribute__((always_inline)) inline Pairs pairs_of(uint32_t codes, float scale) {
+  return Pairs{{__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0),
+                __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1),
+                __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2),
+                __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3)}};
+}
+__device__ __attribute__((always_inline)) inline void f32_of(uint32_t codes, float scale,
+                                                             float (&f)[8]) {
+  const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 0);
+  const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 1);
+  const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 2);
+  const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 3);
+  f[0] = a[0], f[1] = a[1], f[2] = b[0], f[3] = b[1];
+  f[4] = c[0], f[5] = c[1], f[6] = d[0], f[7] = d[1];
+}
+
+// c + a[0] * b[0] + a[1] * b[1] in float32, b's two bf16 values in a word.
+__device__ __attribute__((always_inline)) inline float dot2(bf16x2 a, uint32_t b, float c) {
+  bf16x2 v;
+  __builtin_memcpy(&v, &b, 4);
+  return __builtin_amdgcn_fdot2_f32_bf16(a, v, c, false);
+}
+
 // A range of less than 2^31 bytes of device memory, read by 32-bit byte
 // offsets (`off`, a lane's, plus `base`, the wave's, which lies in the range);
 // a read at or past the range's end gives zeros and touches no memory.
