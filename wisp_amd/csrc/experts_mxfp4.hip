@@ -11,6 +11,7 @@
 
 #include "dma_pipeline.h"
 #include "mxfp4.h"
+#include "tile_pipeline.h"
 
 namespace wisp {
 
@@ -27,7 +28,6 @@ int mxfp4_few_layer(const void* x, const void* logits, int logits_dtype, int ren
 
 namespace {
 
-using mx::bf16x8;
 using mx::f32x4;
 using mx::u32x4;
 
@@ -62,11 +62,24 @@ struct GroupedArgs {
   void* out;
 };
 
+// g / (1 + e^-g), its last few float32 bits apart: act is rounded to bf16.
+// (The exponential's argument is clamped where e^-g is 0 or infinite anyway,
+// so that an infinite g gives what the formula does.)
+__device__ inline float silu_fast(float g) {
+  constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596299e-8f, kLn2 = 0.693147182f;
+  const float n = __builtin_amdgcn_fmed3f(-g, -104.f, 89.f);
+  const float t = n * kLog2e;
+  const float low = fmaf(n, kLog2e, -t) + n * kLog2eLow;  // what t's rounding left
+  float e = __builtin_amdgcn_exp2f(t);
+  e = fmaf(e * kLn2, low, e);
+  return g * __builtin_amdgcn_rcpf(1.f + e);
+}
+
 // bf16(silu(g) * u) of four consecutive columns, one 8-byte store at p.
 __device__ inline void store_act4(uint16_t* p, const f32x4& g, const f32x4& u) {
   uint32_t h[4];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) h[q] = bf16_rne(silu(g[q]) * u[q]);
+  for (int q = 0; q < 4; ++q) h[q] = bf16_rne(silu_fast(g[q]) * u[q]);
   *reinterpret_cast<uint2*>(p) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
@@ -77,7 +90,7 @@ __device__ inline void store_act4(uint16_t* p, const f32x4& g, const f32x4& u) {
 // bytes of a row (lanes that each read a row of their own, as the matrix
 // operand wants them, cost the address unit 64 cycles a load instead of 16
 // and hold a stream of weights at 3 TB/s), then into the wave's own part of
-// LDS, 16-byte block b of row r at position b ^ (r % 8), and back in operand
+// LDS, 16-byte block b of row r at position b ^ (r / 2 % 8), and back in operand
 // order: lane l holds row l % 16 of a tile, block l / 16 of a chunk, the
 // operands of four matrix instructions, step j over
 // k = 32 (l / 16) + 8 j .. + 7.  Lane l loads the scales of the wave's row l.
@@ -176,26 +189,26 @@ struct Tile {
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       codes[g] = *reinterpret_cast<const u32x4*>(wlds + (g * 16 + (lane & 15)) * 128 +
-                                                 (((h * 4 + q) ^ (lane & 7)) << 4));
+                                                 (((h * 4 + q) ^ (lane >> 1 & 7)) << 4));
       scale[g] = kOdd ? mx::scale_of(s[g * kSub + h], scale_at(g, c + h) & 3)
                       : mx::scale_of(__shfl((int)s[h], g * 16 + (lane & 15)), q);
     }
     const bool none = kOdd && (c + h) * 4 + q >= nblk;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      bf16x8 t[NT];
+      u32x4 t[NT];
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        t[i] = *reinterpret_cast<const bf16x8*>(rds + (i * 16 + (lane & 15)) * kTokBytes +
+        t[i] = *reinterpret_cast<const u32x4*>(rds + (i * 16 + (lane & 15)) * kTokBytes +
                                                 (((q * 4 + j) ^ (lane & 15)) << 4));
-        if (none) t[i] = bf16x8{};  // what is there may be an infinity
+        if (none) t[i] = u32x4{};  // what is there may be an infinity
       }
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const bf16x8 v = mx::bf16_of(codes[g][j], __uint_as_float(scale[g]));
+        const u32x4 v = mx::bf16_of(codes[g][j], __uint_as_float(scale[g]));
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-          acc[g][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, t[i], acc[g][i], 0, 0, 0);
+          acc[g][i] = mx::mfma(v, t[i], acc[g][i]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -208,7 +221,7 @@ struct Tile {
 #pragma unroll
       for (int n = 0; n < NL; ++n) {
         const int r = n * 8 + (lane >> 3);
-        *reinterpret_cast<u32x4*>(wlds + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = w.w[n];
+        *reinterpret_cast<u32x4*>(wlds + r * 128 + (((lane & 7) ^ (r >> 1 & 7)) << 4)) = w.w[n];
       }
 #pragma unroll
       for (int i = 0; i < NS; ++i) s[i] = w.s[i];
@@ -282,6 +295,254 @@ mx_grouped_kernel(GroupedArgs a) {
   for (int m0 = 0; m0 < M; m0 += Sh::kToks) t.pass(m0, min(M - m0, Sh::kToks));
 }
 
+// ---------------------------------------------------------------------------
+// Large calls: the same products in tiles of 256 weight rows (w13: 128 gate
+// and 128 up rows) by up to 192 tokens of a slot, eight waves in persistent
+// blocks, one per CU: wave (wr, wt) holds 64 rows against the token tiles wt,
+// wt + 2, ... of 16.  Stages are single chunks; the last chunk of a tile
+// already loads the first of the next.  The matrix instructions and the k
+// order of every output are those of the kernel above, so the bytes are too.
+// ---------------------------------------------------------------------------
+struct Big {
+  static constexpr int WR = 4, WT = 2, NG = 4, NT = 6;
+  static constexpr int kWaves = WR * WT;
+  static constexpr int kRows = WR * NG * 16;
+  static constexpr int kToks = WT * NT * 16;
+  static constexpr int NC = kToks / kTokPerCopy / kWaves;  // token copies of a wave and chunk
+  static constexpr int kPart = kToks * kTokBytes;
+  static constexpr int kWaveW = NG * 16 * 64;              // a wave's codes of a chunk
+  static constexpr int kW = 2 * kPart;
+  static constexpr int kTable = kW + kWaves * kWaveW;
+  static constexpr int kLds = kTable + (int)sizeof(tile::Table);
+};
+
+template <bool kW13>
+struct BigTile {
+  static constexpr int NG = Big::NG, NT = Big::NT, NC = Big::NC;
+  static constexpr int per = kW13 ? NG / 2 : NG;
+  const GroupedArgs& a;
+  unsigned char* lds;
+  unsigned char* wlds;
+  int wave, lane, wr, wt, q, Kdim, nblk, chunks, N;
+
+  tile::Range tokens;
+  struct Source {
+    uint32_t src[NC];  // this lane's piece of each token copy's row
+    mx::Buffer W, S;
+    uint32_t tile0[NG];
+    uint32_t scale;  // byte of the first scale of the wave's row `lane`
+  };
+  struct Weights {
+    u32x4 w[NG];
+    uint32_t s;
+  };
+
+  __device__ __attribute__((always_inline)) int row0(const tile::Work& w) const {
+    return (w.panel * Big::WR + wr) * per * 16;
+  }
+  // The pairs behind this wave's token copies: lane 4 i + n holds that of row
+  // n of copy i.
+  __device__ __attribute__((always_inline)) int pairs(const tile::Work& w) const {
+    static_assert(NC * kTokPerCopy <= 64, "a lane for each row of a wave's copies");
+    const int r = ((lane >> 2) * Big::kWaves + wave) * kTokPerCopy + (lane & 3);
+    return a.lists[(size_t)w.slot * a.P + w.m0 + min(r, w.mrows - 1)];
+  }
+  __device__ __attribute__((always_inline)) void source(const tile::Work& w, int pr,
+                                                        Source& s) const {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int r = (i * Big::kWaves + wave) * kTokPerCopy + q;
+      const int p = __shfl(pr, i * kTokPerCopy + q);
+      s.src[i] = (uint32_t)(kW13 ? p / a.K : p) * (uint32_t)(Kdim * 2) +
+                 (((lane & 15) ^ (r & 15)) << 4);
+    }
+    const uint32_t blocks = (uint32_t)(kW13 ? 2 * a.I : a.H) * (uint32_t)nblk;
+    s.W = mx::buffer(a.W + (size_t)w.slot * a.w_stride, blocks * mx::kBlockBytes);
+    s.S = mx::buffer(a.S + (size_t)w.slot * a.s_stride, blocks);
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+      s.tile0[g] = (g < per ? 0 : a.I) + min(row0(w) + g % per * 16, N - 16);
+    uint32_t row = s.tile0[0];
+#pragma unroll
+    for (int g = 1; g < NG; ++g) row = q == g ? s.tile0[g] : row;
+    s.scale = (row + (lane & 15)) * (uint32_t)nblk;
+  }
+  // Chunk c's token copy i into a stage.
+  __device__ __attribute__((always_inline)) void copy(int i, int c, const Source& s,
+                                                      unsigned char* stage) const {
+    tile::copy16(tokens, s.src[i], c * kTokBytes, stage + (i * Big::kWaves + wave) * 1024);
+  }
+  // Chunk c's codes of row tile g, four lanes for the 64 bytes of a row; its
+  // scales, lane l those of the wave's row l.
+  __device__ __attribute__((always_inline)) void load(int g, int c, const Source& s,
+                                                      Weights& b) const {
+    const uint32_t rowb = (uint32_t)nblk * mx::kBlockBytes;
+    const uint32_t v = (uint32_t)(lane >> 2) * rowb + (c * 4 + (lane & 3)) * mx::kBlockBytes;
+    b.w[g] = mx::load16(s.W, v, s.tile0[g] * rowb);
+  }
+  __device__ __attribute__((always_inline)) void load_scales(int c, const Source& s,
+                                                             Weights& b) const {
+    b.s = mx::load4(s.S, s.scale + c * 4);
+  }
+
+  // A wave's codes of a chunk in operand order, their scales, and the operands
+  // of step 0.
+  struct Operands {
+    u32x4 codes[NG], v0[NG];
+    float scale[NG];
+  };
+  // Through the wave's own LDS: 16-byte block b of row r at position
+  // b ^ (r / 4 % 4).
+  __device__ __attribute__((always_inline)) void put(const Weights& w) const {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const int r = g * 16 + (lane >> 2);
+      *reinterpret_cast<u32x4*>(wlds + r * 64 + (((lane & 3) ^ (r >> 2 & 3)) << 4)) = w.w[g];
+    }
+  }
+  __device__ __attribute__((always_inline)) void get(uint32_t s, Operands& o) const {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const int r = g * 16 + (lane & 15);
+      o.codes[g] = *reinterpret_cast<const u32x4*>(wlds + r * 64 + ((q ^ (r >> 2 & 3)) << 4));
+      o.scale[g] = __uint_as_float(mx::scale_of(__shfl((int)s, r), q));
+    }
+  }
+
+  // One chunk's products from stage rds and operands o, with the loads of
+  // chunk c of `src`.  While the matrix instructions of step j run, the token
+  // and weight operands of step j + 1 are made, and during the last step the
+  // weight operands of the next chunk, so that only its first token operands
+  // are waited for behind the barrier.  The loads go out a few at a time: all
+  // together they fill the address unit's queue, and the wave waits there
+  // instead of computing (80 of 476 us at the Qwen3 8192-token chunk's w13).
+  // For the same reason nothing here is skipped for a tile that is not full:
+  // a branch's LDS reads are all waited for where it ends.
+  __device__ __attribute__((always_inline)) void step(unsigned char* __restrict__ wrs,
+                                                      const unsigned char* __restrict__ rds, int c,
+                                                      const Source& src, Weights& w, Operands& o,
+                                                      f32x4 (&acc)[NG][NT]) const {
+    u32x4 t[NT], v1[NG];
+    auto token = [&](int i, int j) {
+      return *reinterpret_cast<const u32x4*>(
+          rds + ((i * Big::WT + wt) * 16 + (lane & 15)) * kTokBytes +
+          (((q * 4 + j) ^ (lane & 15)) << 4));
+    };
+#pragma unroll
+    for (int i = 0; i < NT; ++i) t[i] = token(i, 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u32x4(&v)[NG] = j & 1 ? v1 : o.v0;
+      u32x4(&vn)[NG] = j & 1 ? o.v0 : v1;
+      if (j == 3) {
+        put(w);
+        get(w.s, o);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) acc[g][i] = mx::mfma(v[g], t[i], acc[g][i]);
+        if (j < 3) t[i] = token(i, j + 1);
+        if (j < 3 ? i < NG : i >= NT - NG) {
+          const int g = j < 3 ? i : i - (NT - NG);
+          vn[g] = mx::bf16_of(o.codes[g][(j + 1) & 3], o.scale[g]);
+        }
+        // weights in step 0, token copies in steps 0 to 1
+        if (j == 0 && i < NG) load(i, c, src, w);
+        if (j == 0 && i == NG) load_scales(c, src, w);
+        if (j == 0 && i == NG + 1) copy(0, c, src, wrs);
+        if (j == 1 && i < NC - 1) copy(i + 1, c, src, wrs);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+};
+
+template <bool kW13>
+__global__ __launch_bounds__(64 * Big::kWaves)
+__attribute__((amdgpu_waves_per_eu(2, 2))) void mx_tile_kernel(GroupedArgs a, int nslots) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  tile::Table* tab = reinterpret_cast<tile::Table*>(lds + Big::kTable);
+  BigTile<kW13> t{a, lds};
+  t.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  t.lane = threadIdx.x & 63;
+  t.wr = t.wave / Big::WT, t.wt = t.wave % Big::WT, t.q = t.lane >> 4;
+  t.wlds = lds + Big::kW + t.wave * Big::kWaveW;
+  t.Kdim = kW13 ? a.H : a.I, t.nblk = t.Kdim / mx::kBlock, t.chunks = t.nblk / 4;
+  t.N = kW13 ? a.I : a.H;
+  t.tokens = {a.A, (uint32_t)(kW13 ? a.P / a.K : a.P) * (uint32_t)(t.Kdim * 2)};
+  constexpr int cols = kW13 ? Big::kRows / 2 : Big::kRows;
+  const int npanels = (t.N + cols - 1) / cols;
+  if (t.wave == 0) tile::fill_table(tab, a.counts, nslots, Big::kToks);
+  __syncthreads();
+  int j = 0;
+  auto take = [&](tile::Work& w) {
+    const bool found = tile::find_work(tab, tile::work_of(blockIdx.x, j++), nslots, npanels, &w);
+    w.slot = __builtin_amdgcn_readfirstlane(w.slot);
+    w.panel = __builtin_amdgcn_readfirstlane(w.panel);
+    w.m0 = __builtin_amdgcn_readfirstlane(w.m0);
+    w.mrows = __builtin_amdgcn_readfirstlane(w.mrows);
+    return (bool)__builtin_amdgcn_readfirstlane(found);
+  };
+  tile::Work cur, next;
+  if (!take(cur)) return;
+  typename BigTile<kW13>::Source src;
+  typename BigTile<kW13>::Weights w = {};
+  int stage = 0;
+  bool have = true;  // `next` is a work
+  next = cur;
+  f32x4 acc[Big::NG][Big::NT];
+  int np = t.pairs(next);
+  typename BigTile<kW13>::Operands o = {};
+  // Turn c computes chunk c of `cur` and loads chunk c + 1, or the first of
+  // `next` (of `cur` once more if there is none).  What the first turn
+  // computes, from zero operands, is dropped.
+  for (int c = t.chunks - 1, first = 1;;) {
+    const bool last = c + 1 == t.chunks;
+    if (last && have) t.source(next, np, src);
+    dma::wait_vm<0>();
+    dma::lds_barrier();
+    t.step(lds + (stage ^ 1) * Big::kPart, lds + stage * Big::kPart, last ? 0 : c + 1, src, w, o,
+           acc);
+    stage ^= 1;
+    if (!last) {
+      ++c;
+      continue;
+    }
+    if (!first) {
+      const int32_t* list = a.lists + (size_t)cur.slot * a.P + cur.m0;
+      const int n0 = t.row0(cur);
+#pragma unroll
+      for (int i = 0; i < Big::NT; ++i) {
+        const int r = (i * Big::WT + t.wt) * 16 + (t.lane & 15);
+        if (r >= cur.mrows) continue;
+        const int p = list[r];
+#pragma unroll
+        for (int g = 0; g < t.per; ++g) {
+          const int n = n0 + g * 16;
+          if (n >= t.N) break;
+          if constexpr (kW13)
+            store_act4((uint16_t*)a.out + (size_t)p * t.N + n + t.q * 4, acc[g][i],
+                       acc[g + t.per][i]);
+          else
+            *reinterpret_cast<f32x4*>((float*)a.out + (size_t)p * t.N + n + t.q * 4) = acc[g][i];
+        }
+      }
+    }
+    if (!have) break;
+    cur = next;
+    have = take(next);
+    if (have) np = t.pairs(next);
+    c = 0;
+    first = 0;
+#pragma unroll
+    for (int g = 0; g < Big::NG; ++g)
+#pragma unroll
+      for (int i = 0; i < Big::NT; ++i) acc[g][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+}
+
 template <typename Sh, bool kW13, bool kOdd>
 hipError_t launch_grouped(const GroupedArgs& a, dim3 grid, hipStream_t st, hipEvent_t e0,
                           hipEvent_t e1) {
@@ -306,6 +567,18 @@ hipError_t launch_product(const GroupedArgs& a, int nslots, hipStream_t st, hipE
     return (kW13 ? a.H : a.I) % kStageK ? launch_grouped<Sh, kW13, true>(a, grid, st, e0, e1)
                                         : launch_grouped<Sh, kW13, false>(a, grid, st, e0, e1);
   };
+  // (the tiles' token offsets are 32 bits wide)
+  const uint64_t bytes = (uint64_t)(kW13 ? a.P / a.K : a.P) * (kW13 ? a.H : a.I) * 2;
+  if (a.P >= 64 * spread && (kW13 ? a.H : a.I) % kChunk == 0 && nslots <= kMaxExperts &&
+      bytes < 1ull << 32) {
+    static std::atomic<uint64_t> big{0};
+    static_assert(Big::kLds <= 160 * 1024, "LDS per block");
+    const hipError_t e = allow_lds(&mx_tile_kernel<kW13>, Big::kLds, Big::kLds, &big);
+    if (e != hipSuccess) return e;
+    launch_timed_lds(mx_tile_kernel<kW13>, dim3(tile::kBlocks), dim3(64 * Big::kWaves), Big::kLds,
+                     st, e0, e1, a, nslots);
+    return hipSuccess;
+  }
   if (a.P <= 8 * spread) return go(Shape<4, 4, 1>{});
   if (a.P <= 20 * spread) return go(Shape<4, 4, 2>{});
   return go(Shape<4, 4, 4>{});

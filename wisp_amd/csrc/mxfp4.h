@@ -31,13 +31,21 @@ __device__ inline uint32_t scale_of(uint32_t word, int q) {
   return ((word >> (8 * q)) & 0xffu) << 23;
 }
 
-// The eight bf16 values of a word of codes.
-__device__ __attribute__((always_inline)) inline bf16x8 bf16_of(uint32_t codes, float scale) {
-  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0);
-  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1);
-  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2);
-  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3);
-  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+// The eight bf16 values of a word of codes, two to a word: half an operand row
+// of the matrix instruction.  (Operands are held as words: the compiler takes
+// a bf16 vector that lives across a branch apart, value by value.)
+__device__ __attribute__((always_inline)) inline u32x4 bf16_of(uint32_t codes, float scale) {
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
+}
+
+// acc + a (16 rows x 32 of k) . b (32 of k x 16 columns).
+__device__ __attribute__((always_inline)) inline f32x4 mfma(const u32x4& a, const u32x4& b,
+                                                            const f32x4& acc) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
 }
 
 // The same values two and two, and as float32.
@@ -62,9 +70,7 @@ __device__ __attribute__((always_inline)) inline void f32_of(uint32_t codes, flo
 
 // c + a[0] * b[0] + a[1] * b[1] in float32, b's two bf16 values in a word.
 __device__ __attribute__((always_inline)) inline float dot2(bf16x2 a, uint32_t b, float c) {
-  bf16x2 v;
-  __builtin_memcpy(&v, &b, 4);
-  return __builtin_amdgcn_fdot2_f32_bf16(a, v, c, false);
+  return __builtin_amdgcn_fdot2_f32_bf16(a, __builtin_bit_cast(bf16x2, b), c, false);
 }
 
 // A range of less than 2^31 bytes of device memory, read by 32-bit byte
@@ -80,6 +86,10 @@ __device__ __attribute__((always_inline)) inline u32x4 load16_nt(Buffer b, uint3
   // nt: each byte is read once
   return __builtin_amdgcn_raw_buffer_load_b128(b, (int)off, (int)base, 2);
 }
+__device__ __attribute__((always_inline)) inline u32x4 load16(Buffer b, uint32_t off,
+                                                                uint32_t base) {
+  return __builtin_amdgcn_raw_buffer_load_b128(b, (int)off, (int)base, 0);
+}
 __device__ __attribute__((always_inline)) inline u32x2 load8(Buffer b, uint32_t off) {
   return __builtin_amdgcn_raw_buffer_load_b64(b, (int)off, 0, 0);
 }
@@ -90,6 +100,7 @@ __device__ __attribute__((always_inline)) inline uint32_t load4(Buffer b, uint32
 struct Buffer {};
 __device__ inline Buffer buffer(const void*, uint32_t) { return {}; }
 __device__ inline u32x4 load16_nt(Buffer, uint32_t, uint32_t) { return {}; }
+__device__ inline u32x4 load16(Buffer, uint32_t, uint32_t) { return {}; }
 __device__ inline u32x2 load8(Buffer, uint32_t) { return {}; }
 __device__ inline uint32_t load4(Buffer, uint32_t) { return 0; }
 #endif

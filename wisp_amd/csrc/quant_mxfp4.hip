@@ -69,12 +69,7 @@ __global__ __launch_bounds__(256) void quant_mxfp4_kernel(const T* __restrict__ 
 }
 
 __device__ inline void store8(uint16_t* p, uint32_t codes, float scale) {
-  union {
-    mx::bf16x8 v;
-    uint4 u;
-  } b;
-  b.v = mx::bf16_of(codes, scale);
-  *reinterpret_cast<uint4*>(p) = b.u;
+  *reinterpret_cast<mx::u32x4*>(p) = mx::bf16_of(codes, scale);
 }
 __device__ inline void store8(float* p, uint32_t codes, float scale) {
   const mx::f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 0);
