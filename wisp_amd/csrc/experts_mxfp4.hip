@@ -13,6 +13,9 @@
 #include "mxfp4.h"
 #include "tile_pipeline.h"
 
+#ifndef BIGNT
+#define BIGNT 4
+#endif
 namespace wisp {
 
 int experts_mfma_combine(int T, int H, int K, const float* topk_w, const int32_t* slots,
@@ -115,6 +118,7 @@ struct Tile {
   int wave, lane, q, Kdim, nblk, chunks, N, n0;
   mx::Buffer W, S;    // the slot's codes and scales
   uint32_t tile0[NG]; // first weight row of each tile (wave-uniform)
+  uint32_t scale0;    // byte of the first scale of the wave's row `lane`
 
   // Byte of the scale of this lane's block of chunk c in tile g (kOdd).
   __device__ __attribute__((always_inline)) uint32_t scale_at(int g, int c) const {
@@ -126,26 +130,20 @@ struct Tile {
     u32x4 w[NL];
     uint32_t s[NS];
   };
-  __device__ __attribute__((always_inline)) void load(int c, Weights& b) const {
+  __device__ __attribute__((always_inline)) void load_codes(int n, int c, Weights& b) const {
     const uint32_t rowb = (uint32_t)nblk * mx::kBlockBytes;
     const int blk = c * 4 + (lane & 7);
     // (nothing past a row's end, also in the stage after the last)
     const uint32_t v = blk < nblk ? (uint32_t)(lane >> 3) * rowb + blk * mx::kBlockBytes : 1u << 31;
-#pragma unroll
-    for (int n = 0; n < NL; ++n)
-      b.w[n] = mx::load16_nt(W, v, (tile0[n / 2] + n % 2 * 8) * rowb);
+    b.w[n] = mx::load16_nt(W, v, (tile0[n / 2] + n % 2 * 8) * rowb);
+  }
+  __device__ __attribute__((always_inline)) void load_scales(int c, Weights& b) const {
     if constexpr (kOdd) {
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
+      for (int i = 0; i < NS; ++i)
         b.s[i] = mx::load4(S, scale_at(i / kSub, c + i % kSub) & ~3u);
-      }
     } else {
-      const uint32_t at = (tile0[0] + (lane & 15)) * (uint32_t)nblk;
-      uint32_t row = at;
-#pragma unroll
-      for (int g = 1; g < NG; ++g)
-        row = q == g ? at + (tile0[g] - tile0[0]) * (uint32_t)nblk : row;
-      const auto two = mx::load8(S, c < chunks ? row + c * 4 : 1u << 31);
+      const auto two = mx::load8(S, c < chunks ? scale0 + c * 4 : 1u << 31);
       b.s[0] = two[0], b.s[1] = two[1];
     }
   }
@@ -157,81 +155,114 @@ struct Tile {
   };
   __device__ __attribute__((always_inline)) void copy(int c, const Tokens& t,
                                                       unsigned char* stage) const {
-    if (c >= chunks) return;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      // (pieces past a row's end repeat its last; their products are not used)
-      const int b = kOdd ? min(c * 16 + t.piece[i], Kdim / 8 - 1) - t.piece[i] : c * 16;
+      // (before the first chunk the first, past a row's end its last piece
+      // once more: no product uses it)
+      const int b = kOdd ? min(max(c, 0) * 16 + t.piece[i], Kdim / 8 - 1) - t.piece[i]
+                         : max(min(c, chunks - 1), 0) * 16;
       dma::dma16(t.src[i] + (ptrdiff_t)b * 16, stage + (i * Sh::WR + wave) * 1024);
     }
   }
 
-  // Half h of the stage from chunk c on, its tokens in rds; the copies of the
-  // next chunk's tokens into wrs are under way meanwhile, and with h = 0 the
-  // next stage's weights into w.  (wrs and rds are distinct, which the
-  // compiler has to know.  It also tells only eight copy instructions of a
-  // kernel apart, and waits for all copies before an LDS read if there are
-  // more: hence one place for all copies, with a turn of the loop for the
-  // first.)
+  // A wave's codes of a chunk in operand order, their scales, and the operands
+  // of step 0.
+  struct Operands {
+    u32x4 codes[NG], v0[NG];
+    float scale[NG];
+  };
+  __device__ __attribute__((always_inline)) void put(const Weights& w) const {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int r = n * 8 + (lane >> 3);
+      *reinterpret_cast<u32x4*>(wlds + r * 128 + (((lane & 7) ^ (r >> 1 & 7)) << 4)) = w.w[n];
+    }
+  }
+  template <int h>
+  __device__ __attribute__((always_inline)) void get(int c, const uint32_t (&s)[NS],
+                                                     Operands& o) const {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const int r = g * 16 + (lane & 15);
+      o.codes[g] = *reinterpret_cast<const u32x4*>(
+          wlds + r * 128 + (((h * 4 + q) ^ (r >> 1 & 7)) << 4));
+      o.scale[g] = __uint_as_float(kOdd ? mx::scale_of(s[g * kSub + h], scale_at(g, c + h) & 3)
+                                        : mx::scale_of(__shfl((int)s[h], r), q));
+    }
+  }
+
+  // Half h of the stage from chunk c on, its tokens in rds; the next chunk's
+  // token copies, into wrs, are under way meanwhile, and with h = 0 the next
+  // stage's weights, into w.  While the matrix instructions of step j run, the
+  // operands of step j + 1 are made, and during the last step the weight
+  // operands of the next half.  (wrs and rds are distinct, which the compiler
+  // has to know.  It also tells only eight copy instructions of a kernel apart,
+  // and waits for all copies before an LDS read if there are more: hence one
+  // place for all copies, with a turn of the loop for the first.)
   template <int h>
   __device__ __attribute__((always_inline)) void half(int c, unsigned char* __restrict__ wrs,
                                                       const unsigned char* __restrict__ rds,
-                                                      const Tokens& tok, const uint32_t (&s)[NS],
-                                                      Weights& w, f32x4 (&acc)[NG][NT]) const {
+                                                      const Tokens& tok, uint32_t (&s)[NS],
+                                                      Weights& w, Operands& o,
+                                                      f32x4 (&acc)[NG][NT]) const {
     // this chunk's tokens have landed: all loads but the youngest, the weights
     dma::wait_vm<h == 0 ? 0 : kLoads>();
     dma::lds_barrier();
-    if (c + h >= -1) copy(c + h + 1, tok, wrs);
-    if constexpr (h == 0) load(c + kSub, w);
-    if (c + h < 0 || c + h >= chunks) return;
-    u32x4 codes[NG];
-    uint32_t scale[NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      codes[g] = *reinterpret_cast<const u32x4*>(wlds + (g * 16 + (lane & 15)) * 128 +
-                                                 (((h * 4 + q) ^ (lane >> 1 & 7)) << 4));
-      scale[g] = kOdd ? mx::scale_of(s[g * kSub + h], scale_at(g, c + h) & 3)
-                      : mx::scale_of(__shfl((int)s[h], g * 16 + (lane & 15)), q);
-    }
+    u32x4 t[NT], v1[NG];
+    // (what stands past a row's end may be an infinity)
     const bool none = kOdd && (c + h) * 4 + q >= nblk;
+    auto token = [&](int i, int j) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(rds + (i * 16 + (lane & 15)) * kTokBytes +
+                                                      (((q * 4 + j) ^ (lane & 15)) << 4));
+      return none ? u32x4{} : v;
+    };
+#pragma unroll
+    for (int i = 0; i < NT; ++i) t[i] = token(i, 0);
+    copy(c + h + 1, tok, wrs);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      u32x4 t[NT];
+      u32x4(&v)[NG] = j & 1 ? v1 : o.v0;
+      u32x4(&vn)[NG] = j & 1 ? o.v0 : v1;
+      if (j == 3) {
+        if constexpr (h == 1) {
+          put(w);
+#pragma unroll
+          for (int i = 0; i < NS; ++i) s[i] = w.s[i];
+          get<0>(c + kSub, s, o);
+        } else {
+          get<1>(c, s, o);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        t[i] = *reinterpret_cast<const u32x4*>(rds + (i * 16 + (lane & 15)) * kTokBytes +
-                                                (((q * 4 + j) ^ (lane & 15)) << 4));
-        if (none) t[i] = u32x4{};  // what is there may be an infinity
-      }
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const u32x4 v = mx::bf16_of(codes[g][j], __uint_as_float(scale[g]));
+        for (int g = 0; g < NG; ++g) acc[g][i] = mx::mfma(v[g], t[i], acc[g][i]);
+        if (j < 3) t[i] = token(i, j + 1);
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-          acc[g][i] = mx::mfma(v, t[i], acc[g][i]);
+        for (int g = i * NG / NT; g < (i + 1) * NG / NT; ++g)
+          if (j < 3 || i == NT - 1) vn[g] = mx::bf16_of(o.codes[g][(j + 1) & 3], o.scale[g]);
+        if (j == 3 && i == NT - 1) {
+#pragma unroll
+          for (int g = 0; g < i * NG / NT; ++g) vn[g] = mx::bf16_of(o.codes[g][0], o.scale[g]);
+        }
+        // (all loads at once would fill the address unit's queue)
+        if (h == 0 && j < 2) {
+#pragma unroll
+          for (int n = (j * NT + i) * NL / (2 * NT); n < (j * NT + i + 1) * NL / (2 * NT); ++n)
+            load_codes(n, c + kSub, w);
+          if (j == 1 && i == NT - 1) load_scales(c + kSub, w);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
-  }
-
-  __device__ __attribute__((always_inline)) void step(int c, const Tokens& tok, Weights& w,
-                                                      f32x4 (&acc)[NG][NT]) const {
-    uint32_t s[NS];
-    if (c >= 0) {
-#pragma unroll
-      for (int n = 0; n < NL; ++n) {
-        const int r = n * 8 + (lane >> 3);
-        *reinterpret_cast<u32x4*>(wlds + r * 128 + (((lane & 7) ^ (r >> 1 & 7)) << 4)) = w.w[n];
-      }
-#pragma unroll
-      for (int i = 0; i < NS; ++i) s[i] = w.s[i];
-    }
-    half<0>(c, tlds + Sh::kPart, tlds, tok, s, w, acc);
-    half<1>(c, tlds, tlds + Sh::kPart, tok, s, w, acc);
   }
 
   __device__ __attribute__((always_inline)) void pass(int m0, int mrows) const {
-    Weights w;
+    Weights w = {};
+    Operands o = {};
+    uint32_t s[NS] = {};
     Tokens tok;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -242,12 +273,18 @@ struct Tile {
           a.A + (size_t)(kW13 ? p / a.K : p) * Kdim + tok.piece[i] * 8);
     }
     f32x4 acc[NG][NT];
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-      for (int t = 0; t < NT; ++t) acc[g][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // The first turn loads; what it computes is dropped.
 #pragma unroll 1
-    for (int c = -kSub; c < chunks; c += kSub) step(c, tok, w, acc);
+    for (int c = -kSub; c < chunks; c += kSub) {
+      if (c <= 0) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) acc[g][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      half<0>(c, tlds + Sh::kPart, tlds, tok, s, w, o, acc);
+      half<1>(c, tlds, tlds + Sh::kPart, tok, s, w, o, acc);
+    }
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int r = i * 16 + (lane & 15);
@@ -268,7 +305,7 @@ struct Tile {
 
 // Grid (panel, slot).
 template <typename Sh, bool kW13, bool kOdd>
-__global__ __launch_bounds__(64 * Sh::WR) __attribute__((amdgpu_waves_per_eu(Sh::NT < 4 ? 3 : 2))) void
+__global__ __launch_bounds__(64 * Sh::WR) __attribute__((amdgpu_waves_per_eu(Sh::NT < 3 ? 3 : 2))) void
 mx_grouped_kernel(GroupedArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char tlds[];
   __shared__ __attribute__((aligned(16))) unsigned char wlds[Sh::WR * Sh::kWaveW];
@@ -291,6 +328,10 @@ mx_grouped_kernel(GroupedArgs a) {
 #pragma unroll
   for (int g = 0; g < Sh::NG; ++g)  // (tiles past the end repeat the last)
     t.tile0[g] = (g < t.per ? 0 : a.I) + min(t.n0 + g % t.per * 16, t.N - 16);
+  uint32_t row = t.tile0[0];
+#pragma unroll
+  for (int g = 1; g < Sh::NG; ++g) row = t.q == g ? t.tile0[g] : row;
+  t.scale0 = (row + (t.lane & 15)) * (uint32_t)t.nblk;
 #pragma unroll 1
   for (int m0 = 0; m0 < M; m0 += Sh::kToks) t.pass(m0, min(M - m0, Sh::kToks));
 }
@@ -303,8 +344,9 @@ mx_grouped_kernel(GroupedArgs a) {
 // already loads the first of the next.  The matrix instructions and the k
 // order of every output are those of the kernel above, so the bytes are too.
 // ---------------------------------------------------------------------------
-struct Big {
-  static constexpr int WR = 4, WT = 2, NG = 4, NT = 6;
+template <int NT_>
+struct BigShape {
+  static constexpr int WR = 4, WT = 2, NG = 4, NT = NT_;
   static constexpr int kWaves = WR * WT;
   static constexpr int kRows = WR * NG * 16;
   static constexpr int kToks = WT * NT * 16;
@@ -316,7 +358,7 @@ struct Big {
   static constexpr int kLds = kTable + (int)sizeof(tile::Table);
 };
 
-template <bool kW13>
+template <typename Big, bool kW13>
 struct BigTile {
   static constexpr int NG = Big::NG, NT = Big::NT, NC = Big::NC;
   static constexpr int per = kW13 ? NG / 2 : NG;
@@ -448,23 +490,24 @@ struct BigTile {
           const int g = j < 3 ? i : i - (NT - NG);
           vn[g] = mx::bf16_of(o.codes[g][(j + 1) & 3], o.scale[g]);
         }
-        // weights in step 0, token copies in steps 0 to 1
-        if (j == 0 && i < NG) load(i, c, src, w);
-        if (j == 0 && i == NG) load_scales(c, src, w);
-        if (j == 0 && i == NG + 1) copy(0, c, src, wrs);
-        if (j == 1 && i < NC - 1) copy(i + 1, c, src, wrs);
+        // one load behind each tile: the weights, then the token copies
+        const int n = j * NT + i;
+        static_assert(NG + 1 + NC <= 3 * NT, "the loads go out before step 3 needs them");
+        if (n < NG) load(n, c, src, w);
+        if (n == NG) load_scales(c, src, w);
+        if (n > NG && n <= NG + NC) copy(n - NG - 1, c, src, wrs);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
 };
 
-template <bool kW13>
+template <typename Big, bool kW13>
 __global__ __launch_bounds__(64 * Big::kWaves)
 __attribute__((amdgpu_waves_per_eu(2, 2))) void mx_tile_kernel(GroupedArgs a, int nslots) {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   tile::Table* tab = reinterpret_cast<tile::Table*>(lds + Big::kTable);
-  BigTile<kW13> t{a, lds};
+  BigTile<Big, kW13> t{a, lds};
   t.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   t.lane = threadIdx.x & 63;
   t.wr = t.wave / Big::WT, t.wt = t.wave % Big::WT, t.q = t.lane >> 4;
@@ -487,14 +530,14 @@ __attribute__((amdgpu_waves_per_eu(2, 2))) void mx_tile_kernel(GroupedArgs a, in
   };
   tile::Work cur, next;
   if (!take(cur)) return;
-  typename BigTile<kW13>::Source src;
-  typename BigTile<kW13>::Weights w = {};
+  typename BigTile<Big, kW13>::Source src;
+  typename BigTile<Big, kW13>::Weights w = {};
   int stage = 0;
   bool have = true;  // `next` is a work
   next = cur;
   f32x4 acc[Big::NG][Big::NT];
   int np = t.pairs(next);
-  typename BigTile<kW13>::Operands o = {};
+  typename BigTile<Big, kW13>::Operands o = {};
   // Turn c computes chunk c of `cur` and loads chunk c + 1, or the first of
   // `next` (of `cur` once more if there is none).  What the first turn
   // computes, from zero operands, is dropped.
@@ -556,6 +599,18 @@ hipError_t launch_grouped(const GroupedArgs& a, dim3 grid, hipStream_t st, hipEv
   return hipSuccess;
 }
 
+template <typename Big, bool kW13>
+hipError_t launch_tiles(const GroupedArgs& a, int nslots, hipStream_t st, hipEvent_t e0,
+                        hipEvent_t e1) {
+  static_assert(Big::kLds <= 160 * 1024, "LDS per block");
+  static std::atomic<uint64_t> big{0};
+  const hipError_t e = allow_lds(&mx_tile_kernel<Big, kW13>, Big::kLds, Big::kLds, &big);
+  if (e != hipSuccess) return e;
+  launch_timed_lds(mx_tile_kernel<Big, kW13>, dim3(tile::kBlocks), dim3(64 * Big::kWaves),
+                   Big::kLds, st, e0, e1, a, nslots);
+  return hipSuccess;
+}
+
 template <bool kW13>
 hipError_t launch_product(const GroupedArgs& a, int nslots, hipStream_t st, hipEvent_t e0,
                           hipEvent_t e1) {
@@ -570,17 +625,11 @@ hipError_t launch_product(const GroupedArgs& a, int nslots, hipStream_t st, hipE
   // (the tiles' token offsets are 32 bits wide)
   const uint64_t bytes = (uint64_t)(kW13 ? a.P / a.K : a.P) * (kW13 ? a.H : a.I) * 2;
   if (a.P >= 64 * spread && (kW13 ? a.H : a.I) % kChunk == 0 && nslots <= kMaxExperts &&
-      bytes < 1ull << 32) {
-    static std::atomic<uint64_t> big{0};
-    static_assert(Big::kLds <= 160 * 1024, "LDS per block");
-    const hipError_t e = allow_lds(&mx_tile_kernel<kW13>, Big::kLds, Big::kLds, &big);
-    if (e != hipSuccess) return e;
-    launch_timed_lds(mx_tile_kernel<kW13>, dim3(tile::kBlocks), dim3(64 * Big::kWaves), Big::kLds,
-                     st, e0, e1, a, nslots);
-    return hipSuccess;
-  }
+      bytes < 1ull << 32)
+    return launch_tiles<BigShape<BIGNT>, kW13>(a, nslots, st, e0, e1);
   if (a.P <= 8 * spread) return go(Shape<4, 4, 1>{});
   if (a.P <= 20 * spread) return go(Shape<4, 4, 2>{});
+  if (a.P <= 34 * spread) return go(Shape<4, 4, 3>{});
   return go(Shape<4, 4, 4>{});
 }
 
