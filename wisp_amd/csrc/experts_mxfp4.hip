@@ -6,6 +6,8 @@
 // becomes its bf16 value, which is exact, in registers on its way into the
 // instruction: one conversion instruction gives two values with their scale
 // applied.
+#include <math.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -13,9 +15,6 @@
 #include "mxfp4.h"
 #include "tile_pipeline.h"
 
-#ifndef BIGNT
-#define BIGNT 4
-#endif
 namespace wisp {
 
 int experts_mfma_combine(int T, int H, int K, const float* topk_w, const int32_t* slots,
@@ -338,7 +337,7 @@ mx_grouped_kernel(GroupedArgs a) {
 
 // ---------------------------------------------------------------------------
 // Large calls: the same products in tiles of 256 weight rows (w13: 128 gate
-// and 128 up rows) by up to 192 tokens of a slot, eight waves in persistent
+// and 128 up rows) by up to 128 or 192 tokens of a slot, eight waves in persistent
 // blocks, one per CU: wave (wr, wt) holds 64 rows against the token tiles wt,
 // wt + 2, ... of 16.  Stages are single chunks; the last chunk of a tile
 // already loads the first of the next.  The matrix instructions and the k
@@ -457,7 +456,8 @@ struct BigTile {
   // weight operands of the next chunk, so that only its first token operands
   // are waited for behind the barrier.  The loads go out a few at a time: all
   // together they fill the address unit's queue, and the wave waits there
-  // instead of computing (80 of 476 us at the Qwen3 8192-token chunk's w13).
+  // instead of computing (80 of 476 us at the Qwen3
+  // 8192-token chunk's w13).
   // For the same reason nothing here is skipped for a tile that is not full:
   // a branch's LDS reads are all waited for where it ends.
   __device__ __attribute__((always_inline)) void step(unsigned char* __restrict__ wrs,
@@ -599,6 +599,21 @@ hipError_t launch_grouped(const GroupedArgs& a, dim3 grid, hipStream_t st, hipEv
   return hipSuccess;
 }
 
+// How long a call's tiles of this shape take, in token tiles of a wave (a
+// chunk costs a wave about half a token tile besides its products): the
+// rounds of 256 blocks, for slots of the average length, give or take the
+// square root that a random router's have.  Measured, shapes of 128 / 192
+// tokens (us): w13 and w2 of the Qwen3 8192-token chunk (512 a slot) 491 /
+// 448 and 322 / 299, of the Mixtral 1000-token chunk (250 a slot) 541 / 626 and
+// 449 / 316 (w2's few panels: 298 tiles are two rounds, 256 one).
+template <typename Big>
+double tile_cost(int P, int spread, int panels) {
+  const double mean = (double)P / spread, dev = sqrt(mean);
+  double tiles = 0;
+  for (double m : {mean - dev, mean, mean + dev}) tiles += ceil(m / Big::kToks) / 3 * spread;
+  return ceil(tiles * panels / tile::kBlocks) * (Big::NT + 0.6);
+}
+
 template <typename Big, bool kW13>
 hipError_t launch_tiles(const GroupedArgs& a, int nslots, hipStream_t st, hipEvent_t e0,
                         hipEvent_t e1) {
@@ -625,8 +640,12 @@ hipError_t launch_product(const GroupedArgs& a, int nslots, hipStream_t st, hipE
   // (the tiles' token offsets are 32 bits wide)
   const uint64_t bytes = (uint64_t)(kW13 ? a.P / a.K : a.P) * (kW13 ? a.H : a.I) * 2;
   if (a.P >= 64 * spread && (kW13 ? a.H : a.I) % kChunk == 0 && nslots <= kMaxExperts &&
-      bytes < 1ull << 32)
-    return launch_tiles<BigShape<BIGNT>, kW13>(a, nslots, st, e0, e1);
+      bytes < 1ull << 32) {
+    const int panels = (int)(((kW13 ? a.I : a.H) + (kW13 ? 127 : 255)) / (kW13 ? 128 : 256));
+    return tile_cost<BigShape<4>>(a.P, spread, panels) < tile_cost<BigShape<6>>(a.P, spread, panels)
+               ? launch_tiles<BigShape<4>, kW13>(a, nslots, st, e0, e1)
+               : launch_tiles<BigShape<6>, kW13>(a, nslots, st, e0, e1);
+  }
   if (a.P <= 8 * spread) return go(Shape<4, 4, 1>{});
   if (a.P <= 20 * spread) return go(Shape<4, 4, 2>{});
   if (a.P <= 34 * spread) return go(Shape<4, 4, 3>{});
