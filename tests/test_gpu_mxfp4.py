@@ -176,7 +176,7 @@ SHAPES = [  # T, H, I, E, K
     (3, 1056, 352, 24, 3), (5, 64, 96, 70, 20), (8, 2048, 768, 16, 8), (16, 512, 256, 16, 8),
     (17, 256, 64, 5, 5), (33, 160, 128, 4, 1), (70, 160, 96, 4, 2), (77, 1056, 352, 24, 3),
     (200, 128, 192, 3, 1), (300, 512, 256, 16, 2), (600, 256, 416, 2, 2), (1100, 384, 288, 3, 2),
-    (130, 128, 128, 2, 1), (200, 256, 640, 3, 2), (401, 512, 128, 2, 2), (1300, 256, 384, 5, 1),
+    (12, 64, 4160, 6, 4), (20, 96, 3104, 4, 4), (40, 128, 9216, 3, 2), (130, 128, 128, 2, 1), (200, 256, 640, 3, 2), (401, 512, 128, 2, 2), (1300, 256, 384, 5, 1),
 ]
 
 

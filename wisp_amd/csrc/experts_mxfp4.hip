@@ -19,8 +19,7 @@ namespace wisp {
 
 int experts_mfma_combine(int T, int H, int K, const float* topk_w, const int32_t* slots,
                          int nslots, const void* work, void* out, hipStream_t st);
-size_t mfma_work_bytes(int T, int K, int H, int nslots);
-bool mxfp4_few(int T, int K, int H, int I);
+bool mxfp4_few(int T, int K, int H, int I, int nslots);
 size_t mxfp4_few_bytes(int P, int I);
 int mxfp4_few_layer(const void* x, const void* logits, int logits_dtype, int renorm,
                     int64_t* forward, int T, int H, int I, int K, float* topk_w, int32_t* slots,
@@ -62,6 +61,7 @@ struct GroupedArgs {
   const uint8_t* S;
   size_t s_stride;
   void* out;
+  int splits;  // of the k range (w2): split z writes its part of y, [P][H], at z * P * H
 };
 
 // g / (1 + e^-g), its last few float32 bits apart: act is rounded to bf16.
@@ -115,6 +115,7 @@ struct Tile {
   unsigned char* wlds;  // this wave's
   const int32_t* list;
   int wave, lane, q, Kdim, nblk, chunks, N, n0;
+  int from, to;       // this block's chunks, whole stages but for a row's end
   mx::Buffer W, S;    // the slot's codes and scales
   uint32_t tile0[NG]; // first weight row of each tile (wave-uniform)
   uint32_t scale0;    // byte of the first scale of the wave's row `lane`
@@ -132,8 +133,8 @@ struct Tile {
   __device__ __attribute__((always_inline)) void load_codes(int n, int c, Weights& b) const {
     const uint32_t rowb = (uint32_t)nblk * mx::kBlockBytes;
     const int blk = c * 4 + (lane & 7);
-    // (nothing past a row's end, also in the stage after the last)
-    const uint32_t v = blk < nblk ? (uint32_t)(lane >> 3) * rowb + blk * mx::kBlockBytes : 1u << 31;
+    // (nothing past the range's end, also in the stage after the last)
+    const uint32_t v = blk < min(nblk, to * 4) ? (uint32_t)(lane >> 3) * rowb + blk * mx::kBlockBytes : 1u << 31;
     b.w[n] = mx::load16_nt(W, v, (tile0[n / 2] + n % 2 * 8) * rowb);
   }
   __device__ __attribute__((always_inline)) void load_scales(int c, Weights& b) const {
@@ -272,15 +273,17 @@ struct Tile {
           a.A + (size_t)(kW13 ? p / a.K : p) * Kdim + tok.piece[i] * 8);
     }
     f32x4 acc[NG][NT];
+    auto clear = [&] {
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[g][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    clear();  // (the last split may be empty)
     // The first turn loads; what it computes is dropped.
 #pragma unroll 1
-    for (int c = -kSub; c < chunks; c += kSub) {
-      if (c <= 0) {
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-#pragma unroll
-          for (int t = 0; t < NT; ++t) acc[g][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
+    for (int c = from - kSub; c < to; c += kSub) {
+      if (c == from) clear();
       half<0>(c, tlds + Sh::kPart, tlds, tok, s, w, o, acc);
       half<1>(c, tlds, tlds + Sh::kPart, tok, s, w, o, acc);
     }
@@ -296,13 +299,14 @@ struct Tile {
         if constexpr (kW13)
           store_act4((uint16_t*)a.out + (size_t)p * N + n + q * 4, acc[g][i], acc[g + per][i]);
         else
-          *reinterpret_cast<f32x4*>((float*)a.out + (size_t)p * N + n + q * 4) = acc[g][i];
+          *reinterpret_cast<f32x4*>((float*)a.out + ((size_t)blockIdx.z * a.P + p) * N + n +
+                                    q * 4) = acc[g][i];
       }
     }
   }
 };
 
-// Grid (panel, slot).
+// Grid (panel, slot, split).
 template <typename Sh, bool kW13, bool kOdd>
 __global__ __launch_bounds__(64 * Sh::WR) __attribute__((amdgpu_waves_per_eu(Sh::NT < 3 ? 3 : 2))) void
 mx_grouped_kernel(GroupedArgs a) {
@@ -319,6 +323,9 @@ mx_grouped_kernel(GroupedArgs a) {
   t.q = t.lane >> 4;
   t.Kdim = kW13 ? a.H : a.I, t.nblk = t.Kdim / mx::kBlock;
   t.chunks = (t.nblk + 3) / 4;
+  const int stages = (t.chunks + kSub - 1) / kSub;
+  const int span = (stages + (int)gridDim.z - 1) / (int)gridDim.z * kSub;
+  t.from = blockIdx.z * span, t.to = min(t.from + span, t.chunks);
   t.N = kW13 ? a.I : a.H;
   t.n0 = (blockIdx.x * Sh::WR + t.wave) * t.per * 16;
   const uint32_t blocks = (uint32_t)(kW13 ? 2 * a.I : a.H) * (uint32_t)t.nblk;
@@ -599,6 +606,9 @@ hipError_t launch_grouped(const GroupedArgs& a, dim3 grid, hipStream_t st, hipEv
   return hipSuccess;
 }
 
+// Calls of at least this many pairs a slot take the block tiles.
+constexpr int kTilePairs = 64;
+
 // How long a call's tiles of this shape take, in token tiles of a wave (a
 // chunk costs a wave about half a token tile besides its products): the
 // rounds of 256 blocks, for slots of the average length, give or take the
@@ -633,13 +643,13 @@ hipError_t launch_product(const GroupedArgs& a, int nslots, hipStream_t st, hipE
   auto go = [&](auto shape) {
     using Sh = decltype(shape);
     constexpr int per = Sh::kRows / (kW13 ? 2 : 1);
-    const dim3 grid(((kW13 ? a.I : a.H) + per - 1) / per, nslots);
+    const dim3 grid(((kW13 ? a.I : a.H) + per - 1) / per, nslots, a.splits);
     return (kW13 ? a.H : a.I) % kStageK ? launch_grouped<Sh, kW13, true>(a, grid, st, e0, e1)
                                         : launch_grouped<Sh, kW13, false>(a, grid, st, e0, e1);
   };
   // (the tiles' token offsets are 32 bits wide)
   const uint64_t bytes = (uint64_t)(kW13 ? a.P / a.K : a.P) * (kW13 ? a.H : a.I) * 2;
-  if (a.P >= 64 * spread && (kW13 ? a.H : a.I) % kChunk == 0 && nslots <= kMaxExperts &&
+  if (a.splits == 1 && a.P >= kTilePairs * spread && (kW13 ? a.H : a.I) % kChunk == 0 && nslots <= kMaxExperts &&
       bytes < 1ull << 32) {
     const int panels = (int)(((kW13 ? a.I : a.H) + (kW13 ? 127 : 255)) / (kW13 ? 128 : 256));
     return tile_cost<BigShape<4>>(a.P, spread, panels) < tile_cost<BigShape<6>>(a.P, spread, panels)
@@ -652,14 +662,49 @@ hipError_t launch_product(const GroupedArgs& a, int nslots, hipStream_t st, hipE
   return go(Shape<4, 4, 4>{});
 }
 
-// Work buffer: the layout of the bf16 grouped GEMM's (pair lists, counts, y).
+// out[t, h] = bf16(sum_k w[t,k] * sum_z y[z, (t,k), h]), k and z ascending;
+// pairs without a slot are passed over.  Grid (ceil(H / 1024), T).
+__global__ __launch_bounds__(256) void mx_combine_kernel(const float* __restrict__ y, int splits,
+                                                         int P, int H, int K, int nslots,
+                                                         const float* __restrict__ topk_w,
+                                                         const int32_t* __restrict__ slots,
+                                                         uint16_t* __restrict__ out) {
+  const int t = blockIdx.y, h = (blockIdx.x * 256 + threadIdx.x) * 4;
+  if (h >= H) return;
+  f32x4 acc{0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < K; ++k) {
+    const int p = t * K + k, s = slots[p];
+    if (s < 0 || s >= nslots) continue;
+    f32x4 v{0.f, 0.f, 0.f, 0.f};
+    for (int z = 0; z < splits; ++z)
+      v += *reinterpret_cast<const f32x4*>(y + ((size_t)z * P + p) * H + h);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(topk_w[p], v[e], acc[e]);
+  }
+  *reinterpret_cast<uint2*>(out + (size_t)t * H + h) =
+      make_uint2(bf16_rne(acc[0]) | (uint32_t)bf16_rne(acc[1]) << 16,
+                 bf16_rne(acc[2]) | (uint32_t)bf16_rne(acc[3]) << 16);
+}
+
+// Splits of w2's k range: a call whose panels are too few to fill the GPU (16
+// of 256 rows at H 4096) splits it, into parts of at least four stages.  It
+// goes by the whole call alone, for the bytes depend on it.  Measured, 1 / 4
+// splits, Mixtral, 6 tokens: w2 100 / 49 us.
+int w2_splits(int T, int K, int H, int I, int nslots) {
+  if ((int64_t)T * K >= (int64_t)kTilePairs * nslots) return 1;
+  const double blocks = mx::distinct(T, K, nslots) * ((H + 255) / 256);
+  return std::max(1, std::min((int)ceil(512 / blocks), I / (4 * kStageK)));
+}
+
+// Work buffer (pair lists, counts, y).
 struct Work {
-  size_t lists, counts, y;
-  Work(int P, int nslots) {
+  size_t lists, counts, y, total;
+  Work(int P, int H, int nslots, int splits) {
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
     lists = 0;
     counts = up((size_t)nslots * P * 4);
     y = counts + up((size_t)nslots * 4);
+    total = y + up((size_t)splits * P * H * 4);
   }
 };
 
@@ -667,7 +712,9 @@ struct Work {
 
 size_t mxfp4_work_bytes(int T, int K, int H, int I, int nslots) {
   if (T < 1 || K < 1 || H < 1 || I < 1 || nslots < 1) return 0;
-  return mxfp4_few(T, K, H, I) ? mxfp4_few_bytes(T * K, I) : mfma_work_bytes(T, K, H, nslots);
+  return mxfp4_few(T, K, H, I, nslots)
+             ? mxfp4_few_bytes(T * K, I)
+             : Work(T * K, H, nslots, w2_splits(T, K, H, I, nslots)).total;
 }
 
 // Why the MXFP4 kernels do not cover a call, or null.
@@ -699,25 +746,31 @@ int experts_mxfp4(const void* x, int T, int H, int I, int K, const float* topk_w
   if (T == 0) return WISP_OK;
   const int rc = check_work(T, K, H, I, nslots, work, work_bytes);
   if (rc != WISP_OK) return rc;
-  if (mxfp4_few(T, K, H, I))
+  if (mxfp4_few(T, K, H, I, nslots))
     return mxfp4_few_layer(x, nullptr, 0, 0, nullptr, T, H, I, K, const_cast<float*>(topk_w),
                            const_cast<int32_t*>(slots), nslots, w13, w13_stride, s13, s13_stride,
                            w2, w2_stride, s2, s2_stride, work, out, st, ev);
   const int P = T * K;
-  const Work wk(P, nslots);
+  const int splits = w2_splits(T, K, H, I, nslots);
+  const Work wk(P, H, nslots, splits);
   int32_t* lists = (int32_t*)((char*)work + wk.lists);
   int32_t* counts = (int32_t*)((char*)work + wk.counts);
   launch_gather(slots, P, nslots, lists, counts, st);
   const GroupedArgs a13{(const uint16_t*)x, H, I, K, P, lists, counts, (const uint8_t*)w13,
-                        w13_stride, (const uint8_t*)s13, s13_stride, act};
+                        w13_stride, (const uint8_t*)s13, s13_stride, act, 1};
   const GroupedArgs a2{(const uint16_t*)act, H, I, K, P, lists, counts, (const uint8_t*)w2,
-                       w2_stride, (const uint8_t*)s2, s2_stride, (char*)work + wk.y};
+                       w2_stride, (const uint8_t*)s2, s2_stride, (char*)work + wk.y, splits};
   WISP_HIP_TRY((launch_product<true>(a13, nslots, st, ev ? ev->ev[0] : nullptr,
                                      ev ? ev->ev[1] : nullptr)));
   WISP_HIP_TRY((launch_product<false>(a2, nslots, st, ev ? ev->ev[2] : nullptr,
                                       ev ? ev->ev[3] : nullptr)));
   WISP_HIP_TRY(hipGetLastError());
-  return experts_mfma_combine(T, H, K, topk_w, slots, nslots, work, out, st);
+  if (splits == 1) return experts_mfma_combine(T, H, K, topk_w, slots, nslots, work, out, st);
+  hipLaunchKernelGGL(mx_combine_kernel, dim3((H + 1023) / 1024, T), dim3(256), 0, st,
+                     (const float*)((char*)work + wk.y), splits, P, H, K, nslots, topk_w, slots,
+                     (uint16_t*)out);
+  WISP_HIP_TRY(hipGetLastError());
+  return WISP_OK;
 }
 
 }  // namespace wisp
@@ -793,7 +846,7 @@ extern "C" int wisp_moe_layer_mxfp4(const void* x, const void* logits, int logit
                       s2_stride, act, out, where);
   if (rc != WISP_OK) return rc;
   if (T > 0 && E <= kMaxExperts && K <= E && logits && topk_w && topk_ids &&
-      (logits_dtype == WISP_F32 || logits_dtype == WISP_BF16) && mxfp4_few(T, K, H, I)) {
+      (logits_dtype == WISP_F32 || logits_dtype == WISP_BF16) && mxfp4_few(T, K, H, I, E)) {
     rc = check_work(T, K, H, I, E, work, work_bytes);
     if (rc != WISP_OK) return rc;
     return mxfp4_few_layer(x, logits, logits_dtype, renormalize, nullptr, T, H, I, K, topk_w,

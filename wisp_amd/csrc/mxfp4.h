@@ -10,6 +10,8 @@
 // bits, and no exponent below bf16's subnormals.
 #pragma once
 
+#include <math.h>
+
 #include "common.h"
 
 namespace wisp {
@@ -24,6 +26,12 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBlock = 32;        // values of one scale
 constexpr int kBlockBytes = 16;   // their codes
+
+// The number of experts that the pairs of T tokens spread over, on average.
+inline double distinct(int T, int K, int nslots) {
+  const double e = nslots > K ? nslots : K;
+  return e * (1.0 - pow(1.0 - K / e, T));
+}
 
 // The bits of the conversions' scale operand for byte `q` (0..3) of a word of
 // scale bytes.
