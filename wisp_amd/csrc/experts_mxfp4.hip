@@ -606,8 +606,11 @@ hipError_t launch_grouped(const GroupedArgs& a, dim3 grid, hipStream_t st, hipEv
   return hipSuccess;
 }
 
-// Calls of at least this many pairs a slot take the block tiles.
-constexpr int kTilePairs = 64;
+// Calls of at least this many pairs a slot take the block tiles: from here the
+// blocks above pass over a slot's weights twice.  Measured, the blocks above
+// against tiles (us a call): Qwen3 199 / 202 at 64 pairs a slot, 231 / 206 at
+// 80, 314 / 298 at 128; Mixtral 341 / 403 at 64, 429 / 417 at 80.
+constexpr int kTilePairs = 72;
 
 // How long a call's tiles of this shape take, in token tiles of a wave (a
 // chunk costs a wave about half a token tile besides its products): the
@@ -687,12 +690,15 @@ __global__ __launch_bounds__(256) void mx_combine_kernel(const float* __restrict
 }
 
 // Splits of w2's k range: a call whose panels are too few to fill the GPU (16
-// of 256 rows at H 4096) splits it, into parts of at least four stages.  It
-// goes by the whole call alone, for the bytes depend on it.  Measured, 1 / 4
-// splits, Mixtral, 6 tokens: w2 100 / 49 us.
+// of 256 rows at H 4096), and whose block tiles would be, splits it into parts
+// of at least four stages.  It goes by the whole call alone, for the bytes
+// depend on it.  Measured, 1 / 4 splits, Mixtral, 6 tokens: w2 100 / 49 us.
 int w2_splits(int T, int K, int H, int I, int nslots) {
-  if ((int64_t)T * K >= (int64_t)kTilePairs * nslots) return 1;
-  const double blocks = mx::distinct(T, K, nslots) * ((H + 255) / 256);
+  const int panels = (H + 255) / 256;
+  const double mean = (double)T * K / nslots;
+  if (mean >= kTilePairs && ceil(mean / BigShape<6>::kToks) * nslots * panels >= tile::kBlocks)
+    return 1;
+  const double blocks = mx::distinct(T, K, nslots) * panels;
   return std::max(1, std::min((int)ceil(512 / blocks), I / (4 * kStageK)));
 }
 
