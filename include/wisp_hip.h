@@ -42,6 +42,8 @@ typedef struct ihipStream_t* wisp_stream_t; /* == hipStream_t */
 #define WISP_BF16 1
 #define WISP_FP8_E4M3 2 /* layer dtype: expert weights float8_e4m3fn (OCP) with
                            float32 block scales; x, act and out bfloat16 */
+#define WISP_MXFP4 3    /* layer dtype: expert weights MXFP4 (below), x, act and
+                           out bfloat16 */
 
 /* layer modes (WISP_MODE, fused_moe.py:76-79) */
 #define WISP_MODE_PAGED 0
@@ -307,7 +309,9 @@ typedef struct wisp_layer_desc {
   int pagein_engine;             /* WISP_PAGEIN_*; KERNEL falls back to
                                     MEMCPY when the masters are not pinned,
                                     device-mapped and 16-byte aligned     */
-  size_t w13_elems, w2_elems;    /* elements of one expert's w13 / w2    */
+  size_t w13_elems, w2_elems;    /* elements of one expert's w13 / w2
+                                    (MXFP4: bytes of codes, I*H and H*I/2;
+                                    strides in bytes too)                 */
   void* scratch_w13;             /* device, slot s at +s*stride [2I, H]  */
   size_t scratch_w13_stride;     /* elements                             */
   void* scratch_w2;              /* device, slot s at +s*stride [H, I]   */
@@ -323,7 +327,9 @@ typedef struct wisp_layer_desc {
   /* block-FP8 experts (dtype WISP_FP8_E4M3; zero / NULL otherwise).  The
      weights above are then float8_e4m3fn (strides in bytes) and each expert
      carries float32 block scales: s13 [2*ceil(I/bn), ceil(H/bk)],
-     s2 [ceil(H/bn), ceil(I/bk)] (fused_moe_fp8.py:188-202). */
+     s2 [ceil(H/bn), ceil(I/bk)] (fused_moe_fp8.py:188-202).  With dtype
+     WISP_MXFP4 the scale buffers hold bytes ([2I, H/32] and [H, I/32]), and
+     their elems and strides count bytes; block_n and block_k are not used. */
   int block_n, block_k;          /* weight block [rows, cols]            */
   size_t s13_elems, s2_elems;    /* scale elements of one expert         */
   float* scratch_s13;            /* device, slot s at +s*stride          */
@@ -399,7 +405,9 @@ int wisp_layer_create(const wisp_layer_desc* desc, void** handle);
 int wisp_layer_destroy(void* handle);
 /* Re-point the context at a new scratch / cap (after a resize).  Layers of
  * dtype WISP_FP8_E4M3 have no resize (the reference's FP8 state has none):
- * WISP_ERR_UNSUPPORTED. */
+ * WISP_ERR_UNSUPPORTED.  An MXFP4 layer's scales move with its w13: a slot's
+ * scales must lie in the slot's slab, and do in the new scratch at the same
+ * distance. */
 int wisp_layer_set_scratch(void* handle, void* scratch_w13, void* scratch_w2, int cap,
                            int32_t* slot_to_expert, int64_t* lru_tick);
 

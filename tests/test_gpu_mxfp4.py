@@ -2,6 +2,8 @@
 back bit for bit, the experts and the whole layer within the bound that float32
 sums and two bf16 roundings allow (derived in ``oracle.mxfp4.experts``), at
 sizes, masks and values where they can go wrong."""
+import functools
+
 import numpy as np
 import pytest
 import torch
@@ -135,6 +137,7 @@ def test_quantize_refusals():
 # ---------------------------------------------------------------------------
 
 
+@functools.lru_cache(maxsize=None)
 def _weights(E, H, I, seed, std=0.05):
     rng = np.random.default_rng(seed)
     out = []
@@ -142,7 +145,7 @@ def _weights(E, H, I, seed, std=0.05):
         w = rng.standard_normal(shape).astype(np.float32) * std
         w *= 2.0 ** rng.integers(-3, 4, (*shape[:2], 1)).astype(np.float32)
         out += O.quantize(w)
-    return out  # w13, s13, w2, s2
+    return tuple(out)  # w13, s13, w2, s2
 
 
 def _routing(T, E, K, seed):

@@ -77,6 +77,45 @@ def test_layer_arguments(hiplib, kw):
         n // 16, P, n // 2, P, n // 32, P, P, P, 1 << 20, None) == INVALID
 
 
+def _desc(**kw):
+    H, I, E = 64, 32, 4
+    n = H * I
+    d = _lib.LayerDesc()
+    d.struct_bytes = C.sizeof(_lib.LayerDesc)
+    d.num_experts, d.cap, d.hidden, d.inter = E, 2, H, I
+    d.dtype, d.mode = _lib.WISP_MXFP4, _lib.WISP_MODE_PAGED
+    d.w13_elems, d.w2_elems, d.s13_elems, d.s2_elems = n, n // 2, n // 16, n // 32
+    for part in ("w13", "w2", "s13", "s2"):
+        for side in ("scratch_", "master_"):
+            setattr(d, side + part, P)
+            setattr(d, side + part + "_stride", 4096)
+    d.expert_map = d.slot_to_expert = d.lru_tick = d.counters = P
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("kw", [
+    dict(w13_elems=2 * 64 * 32), dict(w2_elems=64 * 32), dict(s13_elems=64), dict(s2_elems=32),
+    dict(hidden=48), dict(inter=16), dict(hidden=0), dict(scratch_s13=None), dict(master_s2=None),
+    dict(scratch_s13_stride=64), dict(master_w13_stride=1024), dict(packed_master=P), dict(dtype=4),
+])
+def test_layer_descriptor(hiplib, kw):
+    h = C.c_void_p()
+    assert hiplib.wisp_layer_create(C.byref(_desc(**kw)), C.byref(h)) == INVALID
+    assert not h.value
+
+
+def test_work_bytes(hiplib):
+    w = hiplib.wisp_moe_mxfp4_work_bytes
+    assert w(0, 2, 64, 32, 4) == w(1, 0, 64, 32, 4) == w(1, 2, 64, 32, 0) == 0
+    assert w(1, 2, 64, 32, 4) >= 2 * 32 * 4              # act in float32
+    assert w(100, 2, 64, 32, 4) >= 200 * 64 * 4          # y
+    # a group of a call fits the call's buffer
+    for T in range(13, 64):
+        assert w(T, 2, 64, 32, 4) <= w(T + 1, 2, 64, 32, 4)
+
+
 def test_host_tensors_are_refused():
     u8 = torch.zeros((2, 64, 32), dtype=torch.uint8)
     for call in (lambda: mx.quantize_mxfp4(torch.zeros((2, 64))),

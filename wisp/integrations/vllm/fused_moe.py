@@ -129,6 +129,18 @@ def _resolve_packed_masters() -> bool:
         "0", "false", "no", "off")
 
 
+def _resolve_expert_format() -> str:
+    """``WISP_EXPERT_FORMAT``: ``native`` (default) holds the experts as the
+    checkpoint has them; ``mxfp4`` quantises a bf16 layer's experts to 4-bit
+    microscaled floating point when its weights are loaded
+    (``wisp.integrations.vllm.fused_moe_mxfp4``)."""
+    raw = os.environ.get("WISP_EXPERT_FORMAT", "native").strip().lower()
+    if raw not in ("native", "mxfp4"):
+        logger.warning("WISP_EXPERT_FORMAT=%r is not 'native' or 'mxfp4'; using native", raw)
+        raw = "native"
+    return raw
+
+
 class _PackedRef:
     """A weak reference to a (packed tensor, stride) pair."""
 
@@ -169,9 +181,10 @@ class _Workspace:
     """Per-layer device workspaces and the pinned decision record, grown on demand."""
 
     def __init__(self, device: torch.device, hidden: int, inter: int,
-                 dtype: torch.dtype, fp8: bool = False) -> None:
+                 dtype: torch.dtype, fp8: bool = False, mxfp4_experts: int = 0) -> None:
         self.device, self.hidden, self.inter, self.dtype = device, hidden, inter, dtype
         self.fp8 = fp8
+        self.mxfp4_experts = mxfp4_experts  # of an MXFP4 layer
         self.pairs = 0
         self.record_words = 0
         self.work_bytes = 0
@@ -196,7 +209,11 @@ class _Workspace:
         pairs = max(1, T * K)
         words = lib().wisp_record_words(T, K)
         need = 0
-        if self.fp8 and self.hidden > 0:
+        if self.mxfp4_experts:
+            # (a call is planned by the layer's experts, not by its slots)
+            need = lib().wisp_moe_mxfp4_work_bytes(max(1, T), K, self.hidden, self.inter,
+                                                   self.mxfp4_experts)
+        elif self.fp8 and self.hidden > 0:
             need = lib().wisp_moe_fp8_work_bytes(max(1, T), K, self.hidden, self.inter, nslots)
         elif self.dtype == torch.bfloat16 and self.hidden > 0:
             need = lib().wisp_moe_work_bytes(max(1, T), K, self.hidden, nslots)
@@ -341,6 +358,12 @@ class WispMoEState:
         if self._packed is not None:
             return self._packed_stride
         return (self._w13_elems + self._w2_elems) * self.cpu_w13.element_size()
+
+    @property
+    def slot_bytes(self) -> int:
+        """HBM bytes of the weights in one scratch slot."""
+        return (self.scratch_w13[0].numel() * self.scratch_w13.element_size()
+                + self.scratch_w2[0].numel() * self.scratch_w2.element_size())
 
     def _make_desc(self) -> "_lib.LayerDesc":
         d = _lib.LayerDesc()
@@ -615,11 +638,7 @@ def expert_bytes_per_cap() -> int:
     """HBM bytes one scratch slot holds (its w13 and w2), summed over the
     registered layers: what changing the per-layer cap by one slot frees or
     claims (reference 571-582)."""
-    total = 0
-    for st in _LAYER_STATES:
-        total += st.scratch_w13[0].numel() * st.scratch_w13.element_size()
-        total += st.scratch_w2[0].numel() * st.scratch_w2.element_size()
-    return total
+    return sum(st.slot_bytes for st in _LAYER_STATES)
 
 
 def snapshot_expert_stats(reset: bool = True) -> dict:
@@ -688,6 +707,9 @@ def _patched_process_weights_after_loading(self, layer: torch.nn.Module) -> None
     if getattr(layer, "w13_weight", None) is None or getattr(layer, "w2_weight", None) is None:
         return
     device = torch.device("cuda", torch.cuda.current_device())
+    if _resolve_expert_format() == "mxfp4":
+        _mxfp4_layer(layer, device)
+        return
     slab = getattr(layer, "_wisp_cpu_slab", None)
     if slab is not None:
         pinned = slab if slab.is_pinned() else slab.pin_memory()
@@ -709,22 +731,52 @@ def _patched_process_weights_after_loading(self, layer: torch.nn.Module) -> None
         _placeholders(layer, cpu_w13.dtype, device)
         return
     E = int(cpu_w13.shape[0])
-    override = _WISP_RUNTIME_CONFIG["cap_experts_override"]
-    if mode == _Mode.RESIDENT:
-        cap = E
-    else:
-        cap = override if override is not None else _resolve_cap_experts(E)
+    cap = _layer_cap(mode, E)
     state = WispMoEState(cpu_w13, cpu_w2, cap, mode, device, len(_LAYER_STATES))
-    _LAYER_STATES.append(state)
-    _LAYER_BY_ID[id(layer)] = state
-    if mode == _Mode.RESIDENT:
-        state.prime_identity()
-    layer._wisp_state = state
+    _register(layer, state)
     _placeholders(layer, cpu_w13.dtype, device)
     logger.info("wisp[%s]: layer %d: num_experts=%d cap_experts=%d pinned=%.2f GiB "
                 "scratch=%.2f GiB", mode, state.layer_idx, E, cap,
                 E * state._slab_elems * cpu_w13.element_size() / 2**30,
                 cap * state._slab_elems * cpu_w13.element_size() / 2**30)
+
+
+def _layer_cap(mode: str, experts: int) -> int:
+    """Scratch slots of a layer of ``experts`` experts in ``mode``."""
+    if mode == _Mode.RESIDENT:
+        return experts
+    override = _WISP_RUNTIME_CONFIG["cap_experts_override"]
+    return override if override is not None else _resolve_cap_experts(experts)
+
+
+def _register(layer: torch.nn.Module, state: WispMoEState) -> None:
+    _LAYER_STATES.append(state)
+    _LAYER_BY_ID[id(layer)] = state
+    if state.mode == _Mode.RESIDENT:
+        state.prime_identity()
+    layer._wisp_state = state
+
+
+def _mxfp4_layer(layer: torch.nn.Module, device: torch.device) -> None:
+    """Quantise a loaded layer's experts to MXFP4 and build its state over
+    them; the checkpoint's weights are let go."""
+    from .fused_moe_mxfp4 import WispMoEStateMxfp4, quantize_masters_mxfp4
+    mode: str = _WISP_RUNTIME_CONFIG["mode"]
+    if mode == _Mode.COPY:
+        raise NotImplementedError("wisp: WISP_EXPERT_FORMAT=mxfp4 needs mode paged or resident")
+    w13, w2 = layer.w13_weight.data, layer.w2_weight.data
+    if w13.dtype != torch.bfloat16:
+        raise NotImplementedError(f"wisp: WISP_EXPERT_FORMAT=mxfp4 takes bfloat16 experts, not "
+                                  f"{w13.dtype}")
+    masters = quantize_masters_mxfp4(w13, w2, device)
+    E = int(w13.shape[0])
+    state = WispMoEStateMxfp4(*masters, _layer_cap(mode, E), mode, device, len(_LAYER_STATES))
+    layer._wisp_cpu_slab = layer._wisp_cpu_pin_w13 = layer._wisp_cpu_pin_w2 = None
+    _register(layer, state)
+    _placeholders(layer, torch.bfloat16, device)
+    logger.info("wisp[%s]: layer %d: num_experts=%d cap_experts=%d, experts in MXFP4, "
+                "pinned=%.2f GiB scratch=%.2f GiB", mode, state.layer_idx, E, state.cap_experts,
+                E * state.slot_bytes / 2**30, state.cap_experts * state.slot_bytes / 2**30)
 
 
 def _placeholders(layer: torch.nn.Module, dtype: torch.dtype, device: torch.device) -> None:

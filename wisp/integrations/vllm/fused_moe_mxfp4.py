@@ -13,16 +13,24 @@ a value is ``E2M1(code) * 2**(s - 127)``, ``s == 255`` is NaN.  Weights are
 ``s13 [E, 2I, H/32]``, ``s2 [E, H, I/32]``.  Activations are bfloat16; products
 are summed in float32; the SwiGLU result and the output are rounded to bfloat16
 once each.
+
+``WispMoEStateMxfp4`` is the paging state over such experts: masters in pinned
+host memory, one ``[w13 | w2 | s13 | s2]`` slab per expert, the same pager,
+page-in, prefetch and resize as the bf16 state's.  ``WISP_EXPERT_FORMAT=mxfp4``
+makes ``install_wisp_moe`` quantise a bf16 layer's experts when its weights are
+loaded and run the layer on such a state.
 """
 from __future__ import annotations
 
+import ctypes as C
 import functools
 
 import torch
 
 from wisp_amd import _lib
 from wisp_amd._lib import check, lib
-from .fused_moe import _check_out, _require_device
+from .fused_moe import (WispMoEState, _check_out, _Mode, _require_device, _resolve_pagein_engine,
+                        _resolve_pagein_streams, _Workspace)
 
 BLOCK = 32
 _DTYPES = {torch.float32: _lib.WISP_F32, torch.bfloat16: _lib.WISP_BF16}
@@ -197,4 +205,152 @@ def route_and_experts_mxfp4(x: torch.Tensor, router_logits: torch.Tensor, top_k:
     return out
 
 
-__all__ = ["quantize_mxfp4", "dequantize_mxfp4", "experts_mxfp4", "route_and_experts_mxfp4"]
+# ---------------------------------------------------------------------------
+# The paging state
+# ---------------------------------------------------------------------------
+
+
+class Mxfp4SlabLayout:
+    """Byte layout of one expert's ``[w13 | w2 | s13 | s2]`` slab."""
+
+    def __init__(self, hidden: int, inter: int) -> None:
+        H, I = int(hidden), int(inter)
+        if H < BLOCK or I < BLOCK or H % BLOCK or I % BLOCK:
+            raise ValueError(f"wisp.mxfp4: hidden={H} and inter={I} must be multiples of {BLOCK}")
+        self.hidden, self.inter = H, I
+        self.parts = ((2 * I, H // 2), (H, I // 2), (2 * I, H // BLOCK), (H, I // BLOCK))
+        self.offsets, end = [], 0
+        for rows, cols in self.parts:
+            self.offsets.append(end)
+            end += rows * cols
+        self.used = end
+        self.slab = -(-end // 256) * 256
+
+    def views(self, buf: torch.Tensor):
+        """``buf [N, slab] uint8`` -> ``(w13, w2, s13, s2)`` views of N experts."""
+        base = buf.storage_offset()
+        return tuple(torch.as_strided(buf, (buf.shape[0], rows, cols), (self.slab, cols, 1),
+                                      base + off)
+                     for (rows, cols), off in zip(self.parts, self.offsets))
+
+
+def mxfp4_slab_masters(num_experts: int, hidden: int, inter: int, pin: bool = True):
+    """Host masters as one slab per expert: ``(buf, w13, w2, s13, s2)``, zero
+    codes with scale 1."""
+    lay = Mxfp4SlabLayout(hidden, inter)
+    buf = torch.zeros((num_experts, lay.slab), dtype=torch.uint8, pin_memory=pin)
+    w13, w2, s13, s2 = lay.views(buf)
+    s13.fill_(127)
+    s2.fill_(127)
+    return buf, w13, w2, s13, s2
+
+
+def quantize_masters_mxfp4(w13: torch.Tensor, w2: torch.Tensor, device) -> tuple:
+    """``w13 [E, 2I, H]`` and ``w2 [E, H, I]`` (bfloat16 or float32, host or
+    device memory) -> pinned host masters ``(w13, w2, s13, s2)`` in MXFP4, one
+    slab per expert, quantised on ``device`` an expert at a time."""
+    if w13.dim() != 3 or w2.dim() != 3 or w13.shape[0] != w2.shape[0] or \
+            w13.shape[1] != 2 * w2.shape[2] or w13.shape[2] != w2.shape[1]:
+        raise ValueError("wisp.mxfp4: experts are w13 [E, 2I, H] and w2 [E, H, I]")
+    E, H, I = w13.shape[0], w13.shape[2], w2.shape[2]
+    _, *views = mxfp4_slab_masters(E, H, I)
+    for e in range(E):
+        (q13, s13), (q2, s2) = (quantize_mxfp4(w[e].to(device)) for w in (w13, w2))
+        for dst, src in zip(views, (q13, q2, s13, s2)):
+            dst[e].copy_(src)
+    return tuple(views)
+
+
+class WispMoEStateMxfp4(WispMoEState):
+    """Per-layer paging state over MXFP4 experts.
+
+    ``cpu_w13 [E, 2I, H/2]``, ``cpu_w2 [E, H, I/2]`` codes and ``cpu_s13``,
+    ``cpu_s2`` scales, ``uint8`` host tensors; pinned ones (views of one slab
+    per expert, as :func:`quantize_masters_mxfp4` makes them) page in by the copy
+    kernel, an expert a copy.  Routing, the pager, prefetch and resize are the
+    unquantised state's; activations and outputs are bfloat16.
+    """
+
+    def __init__(self, cpu_w13: torch.Tensor, cpu_w2: torch.Tensor, cpu_s13: torch.Tensor,
+                 cpu_s2: torch.Tensor, cap_experts: int, mode: str, device,
+                 layer_idx: int) -> None:
+        if cpu_w13.dim() != 3 or cpu_w2.dim() != 3:
+            raise ValueError("wisp.mxfp4: cpu_w13 is [E, 2I, H/2], cpu_w2 [E, H, I/2]")
+        E, H, I = cpu_w13.shape[0], 2 * cpu_w13.shape[2], 2 * cpu_w2.shape[2]
+        lay = Mxfp4SlabLayout(H, I)
+        masters = (cpu_w13, cpu_w2, cpu_s13, cpu_s2)
+        for t, name, part in zip(masters, ("cpu_w13", "cpu_w2", "cpu_s13", "cpu_s2"), lay.parts):
+            if t.device.type != "cpu":
+                raise ValueError(f"wisp.mxfp4: {name} must live in host memory")
+            if t.dtype != torch.uint8 or t.shape != (E, *part):
+                raise ValueError(f"wisp.mxfp4: {name} must be a uint8 {(E, *part)} tensor")
+            if t.stride(2) != 1 or t.stride(1) != part[1]:
+                raise ValueError(f"wisp.mxfp4: each expert of {name} must be contiguous")
+        if not 1 <= cap_experts <= E:
+            raise ValueError(f"cap_experts={cap_experts} outside [1, {E}]")
+        self._layout = lay
+        self.layer_idx = int(layer_idx)
+        self.num_experts, self.cap_experts = int(E), int(cap_experts)
+        self.mode = mode
+        self.hidden, self.inter = lay.hidden, lay.inter
+        self.dtype = torch.bfloat16  # activations
+        self.cpu_w13, self.cpu_w2, self.cpu_s13, self.cpu_s2 = masters
+        self.device = torch.device(device)
+        self._alloc_scratch(self.cap_experts)
+        dev = self.device
+        self.expert_map_device = torch.full((E,), -1, dtype=torch.int32, device=dev)
+        self._counters = torch.zeros(8, dtype=torch.int64, device=dev)
+        self.stats_pred_hits = 0
+        self._pf_record = None
+        self._pf_words = 0
+        self._pf_n = 0
+        self._ws = _Workspace(dev, self.hidden, self.inter, torch.bfloat16, mxfp4_experts=int(E))
+        self._last_pairs = 0
+        self._handle = C.c_void_p()
+        self._desc = self._make_desc()
+        check(lib().wisp_layer_create(C.byref(self._desc), C.byref(self._handle)),
+              "wisp_layer_create")
+
+    @property
+    def slot_bytes(self) -> int:
+        return self._layout.used
+
+    @property
+    def packed_bytes_per_expert(self) -> int:
+        return self._layout.used
+
+    def _alloc_scratch(self, cap: int) -> None:
+        lay = self._layout
+        self._scratch = torch.empty((cap, lay.slab), dtype=torch.uint8, device=self.device)
+        self.scratch_w13, self.scratch_w2, self.scratch_s13, self.scratch_s2 = \
+            lay.views(self._scratch)
+        self._slot_to_expert = torch.full((cap,), -1, dtype=torch.int32, device=self.device)
+        self._lru_tick = torch.zeros(cap, dtype=torch.int64, device=self.device)
+
+    def _make_desc(self) -> "_lib.LayerDesc":
+        lay = self._layout
+        d = _lib.LayerDesc()
+        d.struct_bytes = C.sizeof(_lib.LayerDesc)
+        d.num_experts, d.cap = self.num_experts, self.cap_experts
+        d.hidden, d.inter = self.hidden, self.inter
+        d.dtype = _lib.WISP_MXFP4
+        d.mode = _lib.WISP_MODE_RESIDENT if self.mode == _Mode.RESIDENT else _lib.WISP_MODE_PAGED
+        d.pagein_streams = _resolve_pagein_streams()
+        d.pagein_engine = _resolve_pagein_engine()
+        sizes = [rows * cols for rows, cols in lay.parts]
+        d.w13_elems, d.w2_elems, d.s13_elems, d.s2_elems = sizes
+        for part in ("w13", "w2", "s13", "s2"):
+            scratch, master = getattr(self, "scratch_" + part), getattr(self, "cpu_" + part)
+            setattr(d, "scratch_" + part, scratch.data_ptr())
+            setattr(d, f"scratch_{part}_stride", lay.slab)
+            setattr(d, "master_" + part, master.data_ptr())
+            setattr(d, f"master_{part}_stride", master.stride(0))
+        d.expert_map = self.expert_map_device.data_ptr()
+        d.slot_to_expert = self._slot_to_expert.data_ptr()
+        d.lru_tick = self._lru_tick.data_ptr()
+        d.counters = self._counters.data_ptr()
+        return d
+
+
+__all__ = ["quantize_mxfp4", "dequantize_mxfp4", "experts_mxfp4", "route_and_experts_mxfp4",
+           "Mxfp4SlabLayout", "mxfp4_slab_masters", "quantize_masters_mxfp4", "WispMoEStateMxfp4"]

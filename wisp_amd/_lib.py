@@ -20,6 +20,7 @@ WISP_ERR_UNSUPPORTED = 4
 WISP_F32 = 0
 WISP_BF16 = 1
 WISP_FP8_E4M3 = 2
+WISP_MXFP4 = 3
 
 WISP_MODE_PAGED = 0
 WISP_MODE_RESIDENT = 1

@@ -12,6 +12,7 @@
 #include <type_traits>
 
 #include "dma_pipeline.h"
+#include "experts_mxfp4.h"
 #include "mxfp4.h"
 #include "tile_pipeline.h"
 
@@ -19,13 +20,6 @@ namespace wisp {
 
 int experts_mfma_combine(int T, int H, int K, const float* topk_w, const int32_t* slots,
                          int nslots, const void* work, void* out, hipStream_t st);
-bool mxfp4_few(int T, int K, int H, int I, int nslots);
-size_t mxfp4_few_bytes(int P, int I);
-int mxfp4_few_layer(const void* x, const void* logits, int logits_dtype, int renorm,
-                    int64_t* forward, int T, int H, int I, int K, float* topk_w, int32_t* slots,
-                    int nslots, const void* w13, size_t w13_stride, const void* s13,
-                    size_t s13_stride, const void* w2, size_t w2_stride, const void* s2,
-                    size_t s2_stride, void* act, void* out, hipStream_t st, const StageEvents* ev);
 
 namespace {
 
@@ -716,11 +710,18 @@ struct Work {
 
 }  // namespace
 
-size_t mxfp4_work_bytes(int T, int K, int H, int I, int nslots) {
+// How a call is computed, by what it is as a whole: its tokens, shape and number
+// of experts, never by the groups or slots it is paged in, so that paged and
+// resident runs of one batch give the same bytes.
+Mxfp4Plan mxfp4_plan(int T, int K, int H, int I, int experts) {
+  if (mxfp4_few(T, K, H, I, experts)) return {true, 1};
+  return {false, w2_splits(std::max(T, 1), K, H, I, experts)};
+}
+
+// Work buffer of (part of) a call of T tokens over nslots slots.
+size_t mxfp4_work_bytes(const Mxfp4Plan& plan, int T, int K, int H, int I, int nslots) {
   if (T < 1 || K < 1 || H < 1 || I < 1 || nslots < 1) return 0;
-  return mxfp4_few(T, K, H, I, nslots)
-             ? mxfp4_few_bytes(T * K, I)
-             : Work(T * K, H, nslots, w2_splits(T, K, H, I, nslots)).total;
+  return plan.few ? mxfp4_few_bytes(T * K, I) : Work(T * K, H, nslots, plan.splits).total;
 }
 
 // Why the MXFP4 kernels do not cover a call, or null.
@@ -734,8 +735,9 @@ const char* mxfp4_unsupported(int H, int I, int K) {
 
 namespace {
 
-int check_work(int T, int K, int H, int I, int nslots, const void* work, size_t work_bytes) {
-  if (nslots <= 65535 && work && work_bytes >= mxfp4_work_bytes(T, K, H, I, nslots) &&
+int check_work(const Mxfp4Plan& plan, int T, int K, int H, int I, int nslots, const void* work,
+               size_t work_bytes) {
+  if (nslots <= 65535 && work && work_bytes >= mxfp4_work_bytes(plan, T, K, H, I, nslots) &&
       (uintptr_t)work % 256 == 0)
     return WISP_OK;
   wisp_set_last_error("work buffer missing, misaligned or too small", "MXFP4 experts");
@@ -744,20 +746,20 @@ int check_work(int T, int K, int H, int I, int nslots, const void* work, size_t 
 
 }  // namespace
 
-int experts_mxfp4(const void* x, int T, int H, int I, int K, const float* topk_w,
-                  const int32_t* slots, int nslots, const void* w13, size_t w13_stride,
-                  const void* s13, size_t s13_stride, const void* w2, size_t w2_stride,
-                  const void* s2, size_t s2_stride, void* act, void* out, void* work,
-                  size_t work_bytes, hipStream_t st, const StageEvents* ev) {
+int experts_mxfp4(const Mxfp4Plan& plan, const void* x, int T, int H, int I, int K,
+                  const float* topk_w, const int32_t* slots, int nslots, const void* w13,
+                  size_t w13_stride, const void* s13, size_t s13_stride, const void* w2,
+                  size_t w2_stride, const void* s2, size_t s2_stride, void* act, void* out,
+                  void* work, size_t work_bytes, hipStream_t st, const StageEvents* ev) {
   if (T == 0) return WISP_OK;
-  const int rc = check_work(T, K, H, I, nslots, work, work_bytes);
+  const int rc = check_work(plan, T, K, H, I, nslots, work, work_bytes);
   if (rc != WISP_OK) return rc;
-  if (mxfp4_few(T, K, H, I, nslots))
+  if (plan.few)
     return mxfp4_few_layer(x, nullptr, 0, 0, nullptr, T, H, I, K, const_cast<float*>(topk_w),
                            const_cast<int32_t*>(slots), nslots, w13, w13_stride, s13, s13_stride,
                            w2, w2_stride, s2, s2_stride, work, out, st, ev);
   const int P = T * K;
-  const int splits = w2_splits(T, K, H, I, nslots);
+  const int splits = plan.splits;
   const Work wk(P, H, nslots, splits);
   int32_t* lists = (int32_t*)((char*)work + wk.lists);
   int32_t* counts = (int32_t*)((char*)work + wk.counts);
@@ -777,6 +779,28 @@ int experts_mxfp4(const void* x, int T, int H, int I, int K, const float* topk_w
                      (uint16_t*)out);
   WISP_HIP_TRY(hipGetLastError());
   return WISP_OK;
+}
+
+// Routing (logits [T][experts]) and the experts, expert e in slot e.  `forward`:
+// the layer-call counter or null.
+int layer_mxfp4(const Mxfp4Plan& plan, const void* x, const void* logits, int logits_dtype,
+                int renorm, int64_t* forward, int T, int H, int I, int K, float* topk_w,
+                int32_t* ids, int experts, const void* w13, size_t w13_stride, const void* s13,
+                size_t s13_stride, const void* w2, size_t w2_stride, const void* s2,
+                size_t s2_stride, void* act, void* out, void* work, size_t work_bytes,
+                hipStream_t st, const StageEvents* ev) {
+  if (T > 0 && plan.few) {
+    const int rc = check_work(plan, T, K, H, I, experts, work, work_bytes);
+    if (rc != WISP_OK) return rc;
+    return mxfp4_few_layer(x, logits, logits_dtype, renorm, forward, T, H, I, K, topk_w, ids,
+                           experts, w13, w13_stride, s13, s13_stride, w2, w2_stride, s2, s2_stride,
+                           work, out, st, ev);
+  }
+  const int rc = wisp_route_topk_softmax(logits, logits_dtype, T, experts, K, renorm, topk_w, ids,
+                                         forward, (wisp_stream_t)st);
+  if (rc != WISP_OK) return rc;
+  return experts_mxfp4(plan, x, T, H, I, K, topk_w, ids, experts, w13, w13_stride, s13, s13_stride,
+                       w2, w2_stride, s2, s2_stride, act, out, work, work_bytes, st, ev);
 }
 
 }  // namespace wisp
@@ -816,7 +840,8 @@ int check_call(const void* x, int T, int H, int I, int K, int nslots, const void
 }  // namespace
 
 extern "C" size_t wisp_moe_mxfp4_work_bytes(int T, int K, int H, int I, int nslots) {
-  return wisp::mxfp4_work_bytes(T, K, H, I, nslots);
+  if (T < 1 || K < 1 || H < 1 || I < 1 || nslots < 1) return 0;
+  return wisp::mxfp4_work_bytes(wisp::mxfp4_plan(T, K, H, I, nslots), T, K, H, I, nslots);
 }
 
 extern "C" int wisp_moe_experts_mxfp4(const void* x, int T, int H, int I, int K,
@@ -834,9 +859,9 @@ extern "C" int wisp_moe_experts_mxfp4(const void* x, int T, int H, int I, int K,
     wisp_set_last_error("missing routing", where);
     return WISP_ERR_INVALID;
   }
-  return experts_mxfp4(x, T, H, I, K, topk_w, slots, nslots, w13, w13_stride, s13, s13_stride, w2,
-                       w2_stride, s2, s2_stride, act, out, work, work_bytes, (hipStream_t)stream,
-                       nullptr);
+  return experts_mxfp4(mxfp4_plan(T, K, H, I, nslots), x, T, H, I, K, topk_w, slots, nslots, w13,
+                       w13_stride, s13, s13_stride, w2, w2_stride, s2, s2_stride, act, out, work,
+                       work_bytes, (hipStream_t)stream, nullptr);
 }
 
 extern "C" int wisp_moe_layer_mxfp4(const void* x, const void* logits, int logits_dtype, int T,
@@ -851,18 +876,13 @@ extern "C" int wisp_moe_layer_mxfp4(const void* x, const void* logits, int logit
   int rc = check_call(x, T, H, I, K, E, w13, w13_stride, s13, s13_stride, w2, w2_stride, s2,
                       s2_stride, act, out, where);
   if (rc != WISP_OK) return rc;
-  if (T > 0 && E <= kMaxExperts && K <= E && logits && topk_w && topk_ids &&
-      (logits_dtype == WISP_F32 || logits_dtype == WISP_BF16) && mxfp4_few(T, K, H, I, E)) {
-    rc = check_work(T, K, H, I, E, work, work_bytes);
-    if (rc != WISP_OK) return rc;
-    return mxfp4_few_layer(x, logits, logits_dtype, renormalize, nullptr, T, H, I, K, topk_w,
-                           topk_ids, E, w13, w13_stride, s13, s13_stride, w2, w2_stride, s2,
-                           s2_stride, work, out, (hipStream_t)stream, nullptr);
+  if (E > kMaxExperts || K > E || (T > 0 && (!logits || !topk_w || !topk_ids)) ||
+      (logits_dtype != WISP_F32 && logits_dtype != WISP_BF16)) {
+    wisp_set_last_error("invalid routing arguments", where);
+    return WISP_ERR_INVALID;
   }
-  rc = wisp_route_topk_softmax(logits, logits_dtype, T, E, K, renormalize, topk_w, topk_ids,
-                               nullptr, stream);
-  if (rc != WISP_OK) return rc;
-  return experts_mxfp4(x, T, H, I, K, topk_w, topk_ids, E, w13, w13_stride, s13, s13_stride, w2,
-                       w2_stride, s2, s2_stride, act, out, work, work_bytes, (hipStream_t)stream,
-                       nullptr);
+  const Mxfp4Plan plan = mxfp4_plan(T, K, H, I, E);
+  return layer_mxfp4(plan, x, logits, logits_dtype, renormalize, nullptr, T, H, I, K, topk_w,
+                     topk_ids, E, w13, w13_stride, s13, s13_stride, w2, w2_stride, s2, s2_stride,
+                     act, out, work, work_bytes, (hipStream_t)stream, nullptr);
 }

@@ -9,6 +9,7 @@
 // between the launches.
 #include <algorithm>
 
+#include "experts_mxfp4.h"
 #include "mxfp4.h"
 #include "route_core.h"
 
@@ -281,7 +282,6 @@ bool mxfp4_few(int T, int K, int H, int I, int nslots) {
 // Bytes of act between the two launches.
 size_t mxfp4_few_bytes(int P, int I) { return (size_t)P * I * sizeof(float); }
 
-// One of route (logits given: writes topk_w and ids) or slots (the caller's).
 int mxfp4_few_layer(const void* x, const void* logits, int logits_dtype, int renorm,
                     int64_t* forward, int T, int H, int I, int K, float* topk_w, int32_t* slots,
                     int nslots, const void* w13, size_t w13_stride, const void* s13,

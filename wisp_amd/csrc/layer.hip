@@ -50,6 +50,7 @@
 #include <vector>
 
 #include "common.h"
+#include "experts_mxfp4.h"
 #include "pagein.h"
 #include "pager_core.h"
 #include "phase_plan.h"
@@ -169,8 +170,11 @@ constexpr int kCopyStreams = 2;
 constexpr int kProfRing = 512;
 constexpr int kPinRing = 64;
 
-// Bytes of one weight element, and of one activation element (x, act, out).
-size_t elem_size(int dtype) { return dtype == WISP_F32 ? 4 : dtype == WISP_FP8_E4M3 ? 1 : 2; }
+// Bytes of one weight element, and of one activation element (x, act, out)
+// (MXFP4: a byte of codes).
+size_t elem_size(int dtype) {
+  return dtype == WISP_F32 ? 4 : dtype == WISP_FP8_E4M3 || dtype == WISP_MXFP4 ? 1 : 2;
+}
 size_t act_size(int dtype) { return dtype == WISP_F32 ? 4 : 2; }
 
 // One tensor of an expert as the page-in moves it (see PageInPlane): host
@@ -210,6 +214,8 @@ struct PinLaunch {
 struct Layer {
   wisp_layer_desc d;
   bool fp8 = false;
+  bool mx = false;
+  Mxfp4Plan plan{};  // an MXFP4 layer's, of the call under way
   // the tensors one page-in moves per expert, merged where they are adjacent
   int nplanes = 0;
   Plane planes[kMaxPlanes];
@@ -335,7 +341,7 @@ int issue_copies(Layer& L, const int32_t* pairs, int n, double* bytes, hipStream
   return WISP_OK;
 }
 
-// The layer's tensors as page-in planes: w13, w2 and (block-FP8) the two
+// The layer's tensors as page-in planes: w13, w2 and (block-FP8, MXFP4) the two
 // scale tensors, merged when one starts where the previous ends in both the
 // master and the scratch with equal strides, so a [w13 | w2 | s13 | s2] slab
 // per expert moves as one copy.  A single merged plane is padded to 16 bytes
@@ -349,11 +355,12 @@ void build_planes(Layer& L) {
               (char*)d.scratch_w13, d.scratch_w13_stride * wb, d.w13_elems * wb};
   raw[n++] = {(const char*)d.master_w2, nullptr, d.master_w2_stride * wb, (char*)d.scratch_w2,
               d.scratch_w2_stride * wb, d.w2_elems * wb};
-  if (L.fp8) {
-    raw[n++] = {(const char*)d.master_s13, nullptr, d.master_s13_stride * 4,
-                (char*)d.scratch_s13, d.scratch_s13_stride * 4, d.s13_elems * 4};
-    raw[n++] = {(const char*)d.master_s2, nullptr, d.master_s2_stride * 4, (char*)d.scratch_s2,
-                d.scratch_s2_stride * 4, d.s2_elems * 4};
+  if (L.fp8 || L.mx) {
+    const size_t sb = L.fp8 ? 4 : 1;
+    raw[n++] = {(const char*)d.master_s13, nullptr, d.master_s13_stride * sb,
+                (char*)d.scratch_s13, d.scratch_s13_stride * sb, d.s13_elems * sb};
+    raw[n++] = {(const char*)d.master_s2, nullptr, d.master_s2_stride * sb, (char*)d.scratch_s2,
+                d.scratch_s2_stride * sb, d.s2_elems * sb};
   }
   L.expert_bytes = 0;
   for (int i = 0; i < n; ++i) L.expert_bytes += raw[i].bytes;
@@ -493,7 +500,7 @@ void set_fused_ok(Layer& L) {
   const wisp_layer_desc& d = L.d;
   const Plane& p0 = L.planes[0];
   const size_t w13_bytes = d.w13_elems * L.es;
-  L.fused_ok = L.kpin && L.nplanes >= 1 && p0.host == (const char*)d.master_w13 &&
+  L.fused_ok = L.kpin && !L.mx && L.nplanes >= 1 && p0.host == (const char*)d.master_w13 &&
                p0.d == (char*)d.scratch_w13 && p0.bytes >= w13_bytes &&
                p0.m_stride == d.master_w13_stride * L.es &&
                p0.d_stride == d.scratch_w13_stride * L.es;
@@ -629,6 +636,20 @@ int w2(Layer& L, const void* act, int T, int K, const float* w, const int32_t* s
 int experts(Layer& L, const void* x, int T, int K, const float* w, const int32_t* slots,
             void* act, void* out, int algo, const wisp_workspace* ws, hipStream_t st) {
   const wisp_layer_desc& d = L.d;
+  if (L.mx) {
+    ProfLaunch* p13 = prof_begin(L, 0);
+    ProfLaunch* p2 = prof_begin(L, 1);
+    if (p13 && p2) L.prof_w13_calls += 1;
+    const StageEvents ev = {{p13 ? p13->start : nullptr, p13 ? p13->stop : nullptr,
+                             p2 ? p2->start : nullptr, p2 ? p2->stop : nullptr}};
+    const int rc = experts_mxfp4(L.plan, x, T, d.hidden, d.inter, K, w, slots, d.cap, d.scratch_w13,
+                                 d.scratch_w13_stride, d.scratch_s13, d.scratch_s13_stride,
+                                 d.scratch_w2, d.scratch_w2_stride, d.scratch_s2,
+                                 d.scratch_s2_stride, act, out, ws->work, ws->work_bytes, st,
+                                 (p13 && p2) ? &ev : nullptr);
+    if (rc == WISP_OK && p13 && p2) p13->pending = p2->pending = true;
+    return rc;
+  }
   if (L.fp8) {
     ProfLaunch* p13 = prof_begin(L, 0);
     ProfLaunch* p2 = prof_begin(L, 1);
@@ -671,6 +692,10 @@ int experts(Layer& L, const void* x, int T, int K, const float* w, const int32_t
 // without touching the pager state.
 int choose_algo(const Layer& L, int algo, int T, int K) {
   const wisp_layer_desc& d = L.d;
+  if (d.dtype == WISP_MXFP4)  // (a request for one of its two ways is not taken)
+    return algo != WISP_ALGO_AUTO ? -1
+           : mxfp4_plan(T, K, d.hidden, d.inter, d.num_experts).few ? WISP_ALGO_GEMV
+                                                                    : WISP_ALGO_MFMA;
   if (algo == WISP_ALGO_AUTO) return auto_algo(d.dtype, d.hidden, d.inter, T, K);
   if (algo == WISP_ALGO_MFMA && d.dtype == WISP_F32) return -1;
   if (algo == WISP_ALGO_MFMA && d.dtype == WISP_BF16 && !mfma_supported(d.hidden, d.inter))
@@ -782,6 +807,9 @@ bool work_ok(const Layer& L, int a, int T, int K, const wisp_workspace* ws) {
     need = mfma_work_bytes(T, K, d.hidden, d.cap);
   else if (a == WISP_ALGO_MFMA && d.dtype == WISP_FP8_E4M3)
     need = fp8_work_bytes(T, K, d.hidden, d.inter, d.cap);
+  else if (d.dtype == WISP_MXFP4)
+    need = mxfp4_work_bytes(mxfp4_plan(T, K, d.hidden, d.inter, d.num_experts), T, K, d.hidden,
+                            d.inter, d.cap);
   if (need == 0 || T == 0) return true;
   return ws->work && ws->work_bytes >= need && ((uintptr_t)ws->work) % 256 == 0;
 }
@@ -826,7 +854,7 @@ namespace wisp {
 // layer is in flight.
 static int alloc_decode(Layer& L, int cap) {
   const wisp_layer_desc& d = L.d;
-  if (L.fp8 || d.hidden < 1 || d.mode != WISP_MODE_PAGED || cap <= L.spec_cap) return WISP_OK;
+  if (L.fp8 || L.mx || d.hidden < 1 || d.mode != WISP_MODE_PAGED || cap <= L.spec_cap) return WISP_OK;
   if (L.act_spec) WISP_HIP_TRY(hipFree(L.act_spec));
   L.act_spec = nullptr;
   L.spec_cap = 0;
@@ -853,6 +881,16 @@ static bool fp8_desc_ok(const wisp_layer_desc& d) {
   return d.s13_elems == 2 * ((I + bn - 1) / bn) * ((H + bk - 1) / bk) &&
          d.s2_elems == ((H + bn - 1) / bn) * ((I + bk - 1) / bk);
 }
+
+// MXFP4 fields of a descriptor: an expert MLP of whole blocks with its scales.
+static bool mxfp4_desc_ok(const wisp_layer_desc& d) {
+  if (d.hidden < 1 || mxfp4_unsupported(d.hidden, d.inter, 1)) return false;
+  const size_t n = (size_t)d.hidden * d.inter;
+  return d.w13_elems == n && d.w2_elems == n / 2 && d.s13_elems == n / 16 &&
+         d.s2_elems == n / 32 && d.scratch_s13 && d.scratch_s2 && d.master_s13 && d.master_s2 &&
+         d.scratch_s13_stride >= d.s13_elems && d.scratch_s2_stride >= d.s2_elems &&
+         d.master_s13_stride >= d.s13_elems && d.master_s2_stride >= d.s2_elems;
+}
 }  // namespace wisp
 
 extern "C" int wisp_layer_create(const wisp_layer_desc* desc, void** handle) {
@@ -866,10 +904,13 @@ extern "C" int wisp_layer_create(const wisp_layer_desc* desc, void** handle) {
   const wisp_layer_desc& d = *desc;
   if (d.num_experts < 1 || d.num_experts > kMaxExperts || d.cap < 1 || d.cap > kMaxExperts ||
       d.hidden < 0 || d.inter < 0 || d.w13_elems < 1 || d.w2_elems < 1 ||
-      (d.hidden > 0 && (d.w13_elems != (size_t)2 * d.inter * d.hidden ||
-                        d.w2_elems != (size_t)d.hidden * d.inter)) ||
-      (d.dtype != WISP_F32 && d.dtype != WISP_BF16 && d.dtype != WISP_FP8_E4M3) ||
+      (d.hidden > 0 && d.dtype != WISP_MXFP4 &&
+       (d.w13_elems != (size_t)2 * d.inter * d.hidden ||
+        d.w2_elems != (size_t)d.hidden * d.inter)) ||
+      (d.dtype != WISP_F32 && d.dtype != WISP_BF16 && d.dtype != WISP_FP8_E4M3 &&
+       d.dtype != WISP_MXFP4) ||
       (d.dtype == WISP_FP8_E4M3 && !fp8_desc_ok(d)) ||
+      (d.dtype == WISP_MXFP4 && !mxfp4_desc_ok(d)) ||
       (d.mode != WISP_MODE_PAGED && d.mode != WISP_MODE_RESIDENT) || !d.scratch_w13 ||
       !d.scratch_w2 || !d.master_w13 || !d.master_w2 || !d.expert_map || !d.slot_to_expert ||
       !d.lru_tick || !d.counters || d.scratch_w13_stride < d.w13_elems ||
@@ -893,6 +934,7 @@ extern "C" int wisp_layer_create(const wisp_layer_desc* desc, void** handle) {
   Layer* L = new Layer();
   L->d = d;
   L->fp8 = d.dtype == WISP_FP8_E4M3;
+  L->mx = d.dtype == WISP_MXFP4;
   L->es = elem_size(d.dtype);
   L->nstreams = d.pagein_streams;
   build_planes(*L);
@@ -967,9 +1009,25 @@ extern "C" int wisp_layer_set_scratch(void* handle, void* scratch_w13, void* scr
     wisp_set_last_error("block-FP8 layers are not resized", "wisp_layer_set_scratch");
     return WISP_ERR_UNSUPPORTED;
   }
+  const ptrdiff_t o13 = (const char*)L->d.scratch_s13 - (const char*)L->d.scratch_w13;
+  const ptrdiff_t o2 = (const char*)L->d.scratch_s2 - (const char*)L->d.scratch_w13;
+  if (L->mx) {
+    const ptrdiff_t slab = (ptrdiff_t)L->d.scratch_w13_stride;
+    if (o13 < 0 || o2 < 0 || o13 + (ptrdiff_t)L->d.s13_elems > slab ||
+        o2 + (ptrdiff_t)L->d.s2_elems > slab ||
+        L->d.scratch_s13_stride != L->d.scratch_w13_stride ||
+        L->d.scratch_s2_stride != L->d.scratch_w13_stride) {
+      wisp_set_last_error("the MXFP4 scales are not in the slots' slabs", "wisp_layer_set_scratch");
+      return WISP_ERR_UNSUPPORTED;
+    }
+  }
   for (int c = 0; c < kCopyStreams; ++c) (void)hipStreamSynchronize(L->copy[c]);
   harvest_pagein_timing(*L);
   for (int i = 0; i < kPinRing; ++i) harvest_pin(*L, i);
+  if (L->mx) {
+    L->d.scratch_s13 = (float*)((char*)scratch_w13 + o13);
+    L->d.scratch_s2 = (float*)((char*)scratch_w13 + o2);
+  }
   L->d.scratch_w13 = scratch_w13;
   L->d.scratch_w2 = scratch_w2;
   // the masters (and their device mappings) are unchanged; only the scratch
@@ -1019,6 +1077,16 @@ extern "C" int wisp_layer_forward(void* handle, const void* x, const void* logit
                         "wisp_layer_forward");
     return WISP_ERR_UNSUPPORTED;
   }
+  if (L->mx) {
+    const char* why = mxfp4_unsupported(d.hidden, d.inter, K);
+    if (!why && ((uintptr_t)d.scratch_s13 % 4 || (uintptr_t)d.scratch_s2 % 4 ||
+                 d.scratch_s13_stride % 4 || d.scratch_s2_stride % 4))
+      why = "scale scratch and its strides must be 4-byte aligned";
+    if (why) {
+      wisp_set_last_error(why, "wisp_layer_forward");
+      return WISP_ERR_UNSUPPORTED;
+    }
+  }
   if (L->fp8) {
     const char* why = fp8_unsupported(d.hidden, d.inter, K, d.block_n, d.block_k);
     if (!why && (((uintptr_t)d.scratch_s13) % 16 || ((uintptr_t)d.scratch_s2) % 16))
@@ -1040,10 +1108,26 @@ extern "C" int wisp_layer_forward(void* handle, const void* x, const void* logit
     return WISP_ERR_INVALID;
   }
   if (L->profile) L->prof_calls += 1;
+  if (L->mx) L->plan = mxfp4_plan(T, K, d.hidden, d.inter, d.num_experts);
 
   L->rec_on_device = false;
   if (d.mode == WISP_MODE_RESIDENT) {
-    if (a == WISP_ALGO_GEMV && !L->fp8 && logits &&
+    if (L->mx && L->plan.few && (logits_dtype == WISP_F32 || logits_dtype == WISP_BF16)) {
+      // [route + w13] [w2]
+      ProfLaunch* p13 = prof_begin(*L, 0);
+      ProfLaunch* p2 = prof_begin(*L, 1);
+      if (p13 && p2) L->prof_w13_calls += 1;
+      const StageEvents ev = {{p13 ? p13->start : nullptr, p13 ? p13->stop : nullptr,
+                               p2 ? p2->start : nullptr, p2 ? p2->stop : nullptr}};
+      rc = layer_mxfp4(L->plan, x, logits, logits_dtype, renormalize, d.counters + kForward, T,
+                       d.hidden, d.inter, K, ws->topk_w, ws->topk_ids, d.num_experts,
+                       d.scratch_w13, d.scratch_w13_stride, d.scratch_s13, d.scratch_s13_stride,
+                       d.scratch_w2, d.scratch_w2_stride, d.scratch_s2, d.scratch_s2_stride,
+                       ws->act, out, ws->work, ws->work_bytes, st, (p13 && p2) ? &ev : nullptr);
+      if (rc == WISP_OK && p13 && p2) p13->pending = p2->pending = true;
+      return rc;
+    }
+    if (a == WISP_ALGO_GEMV && !L->fp8 && !L->mx && logits &&
         (logits_dtype == WISP_F32 || logits_dtype == WISP_BF16) && ws->topk_w && ws->topk_ids &&
         route_w13_supported(d.dtype, T, d.hidden, d.inter, d.num_experts, K)) {
       // [route + w13] [w2]
@@ -1083,7 +1167,7 @@ extern "C" int wisp_layer_forward(void* handle, const void* x, const void* logit
   int32_t* rec_host = ws->record_dev && !rec_dev_only ? record_device_ptr(ws->record) : nullptr;
   L->rec_on_device = rec_dev_only;
   if (L->decode_fused && T == 1 && fuse_route && rec_dev_only && a == WISP_ALGO_GEMV &&
-      L->fused_ok && !L->fp8 && L->act_spec && L->spec_cap >= d.cap &&
+      L->fused_ok && !L->fp8 && !L->mx && L->act_spec && L->spec_cap >= d.cap &&
       (logits_dtype == WISP_F32 || logits_dtype == WISP_BF16) &&
       decode_w13_supported(d.dtype, d.hidden, d.num_experts, K, d.cap)) {
     // [route + pager + page-in + w13 per slot] [w2]: the launch's w13
@@ -1138,7 +1222,7 @@ extern "C" int wisp_layer_forward(void* handle, const void* x, const void* logit
   }
   WISP_HIP_TRY(hipEventRecord(L->ev_decided, st));
 
-  const bool speculate = a == WISP_ALGO_GEMV && one_group && !L->fp8;
+  const bool speculate = a == WISP_ALGO_GEMV && one_group && !L->fp8 && !L->mx;
   ProfLaunch* spec_w2 = nullptr;
   int spec_rc = WISP_OK;
   if (speculate) {
