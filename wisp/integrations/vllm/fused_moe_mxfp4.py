@@ -46,7 +46,7 @@ def _on_device(fn):
         t = args[0] if args else kwargs.get(first)
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise ValueError(f"wisp.mxfp4: {fn.__name__} takes device tensors")
-        if t.device.index == torch.cuda.current_device():
+        if t.get_device() == torch.cuda.current_device():
             return fn(*args, **kwargs)
         with torch.cuda.device(t.device):
             return fn(*args, **kwargs)
@@ -112,15 +112,19 @@ def _check_weights(x, w13, w2, s13, s2) -> tuple[int, int, int]:
         raise ValueError("wisp.mxfp4: x is [T, H], w13 [E, 2I, H/2], w2 [E, H, I/2]")
     H = x.shape[1]
     E, I = w13.shape[0], 2 * w2.shape[2]
-    dev = x.device
-    for t, name, rows, cols in ((w13, "w13", 2 * I, H // 2), (w2, "w2", H, I // 2),
-                                (s13, "s13", 2 * I, H // BLOCK), (s2, "s2", H, I // BLOCK)):
-        if t.dtype != torch.uint8 or t.shape != (E, rows, cols):
-            raise ValueError(f"wisp.mxfp4: {name} must be a uint8 {(E, rows, cols)} tensor")
-        if t.device != dev:
-            _require_device(t, dev, name)
-        if not t.is_contiguous() and (t.stride(2) != 1 or t.stride(1) != cols):
-            raise ValueError(f"wisp.mxfp4: each expert of {name} must be contiguous")
+    if w13.shape != (E, 2 * I, H // 2) or w2.shape != (E, H, I // 2) or \
+            s13.shape != (E, 2 * I, H // BLOCK) or s2.shape != (E, H, I // BLOCK):
+        raise ValueError(f"wisp.mxfp4: for x [T, {H}], E = {E} and I = {I}, w13 is "
+                         f"{(E, 2 * I, H // 2)}, w2 {(E, H, I // 2)}, s13 "
+                         f"{(E, 2 * I, H // BLOCK)} and s2 {(E, H, I // BLOCK)}")
+    dev = x.get_device()
+    for t in (w13, w2, s13, s2):
+        if t.dtype != torch.uint8:
+            raise ValueError("wisp.mxfp4: codes and scales are uint8 tensors")
+        if t.get_device() != dev:
+            _require_device(t, x.device, "an expert tensor")
+        if not t.is_contiguous() and (t.stride(2) != 1 or t.stride(1) != t.shape[2]):
+            raise ValueError("wisp.mxfp4: each expert of w13, w2, s13 and s2 must be contiguous")
     return E, H, I
 
 
