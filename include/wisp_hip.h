@@ -231,8 +231,7 @@ int wisp_dequant_mxfp4(const uint8_t* codes, const uint8_t* scales, int64_t rows
  * w13 + s*w13_stride ([2I, H/2]), scales at s13 + s*s13_stride ([2I, H/32]);
  * W2 [H, I/2] and s2 [H, I/32] likewise; strides in bytes.  H and I must be
  * multiples of 32, H*I below 2^31, weights and their strides 16-byte aligned,
- * scales and their strides 4-byte aligned (the aligned words that hold an
- * expert's scale bytes are read whole).
+ * scales and their strides 4-byte aligned.
  * A slot outside [0, nslots) contributes zero.  act: T*K*I elements; work:
  * device, 256-byte aligned, wisp_moe_mxfp4_work_bytes(T, K, H, I, nslots)
  * bytes. */
@@ -253,7 +252,8 @@ int wisp_moe_layer_mxfp4(const void* x, const void* logits, int logits_dtype, in
                          wisp_stream_t stream);
 
 /* Bytes of the work buffer of the MXFP4 experts (pair lists and fp32 per-pair
- * outputs; for a few tokens act in float32).  Not monotone in T. */
+ * outputs; for a few tokens act in float32); 0 for bad counts.  Not monotone
+ * in T. */
 size_t wisp_moe_mxfp4_work_bytes(int T, int K, int H, int I, int nslots);
 
 /* Bytes of the device array wisp_moe_experts_noalloc works in, per GPU, in

@@ -179,7 +179,8 @@ SHAPES = [  # T, H, I, E, K
     (3, 1056, 352, 24, 3), (5, 64, 96, 70, 20), (8, 2048, 768, 16, 8), (16, 512, 256, 16, 8),
     (17, 256, 64, 5, 5), (33, 160, 128, 4, 1), (70, 160, 96, 4, 2), (77, 1056, 352, 24, 3),
     (200, 128, 192, 3, 1), (300, 512, 256, 16, 2), (600, 256, 416, 2, 2), (1100, 384, 288, 3, 2),
-    (12, 64, 4160, 6, 4), (20, 96, 3104, 4, 4), (40, 128, 9216, 3, 2), (130, 128, 128, 2, 1), (200, 256, 640, 3, 2), (401, 512, 128, 2, 2), (1300, 256, 384, 5, 1),
+    (12, 64, 4160, 6, 4), (20, 96, 3104, 4, 4), (40, 128, 9216, 3, 2), (130, 128, 128, 2, 1),
+    (200, 256, 640, 3, 2), (401, 512, 128, 2, 2), (1300, 256, 384, 5, 1),
 ]
 
 
@@ -189,6 +190,33 @@ def test_experts_match_the_oracle(T, H, I, E, K):
     ids, w = _routing(T, E, K, T + 1)
     x = _x(T, H, T + 2)
     _close(_run(x, w, ids, weights), x, w, ids, weights)
+
+
+@pytest.mark.parametrize("T,H,I,E,K", [(13, 64, 6400, 4, 2), (20, 96, 6208, 3, 1),
+                                       (30, 32, 8448, 2, 2), (13, 64, 14336, 4, 2)])
+def test_experts_of_a_long_inner_range(T, H, I, E, K):
+    """w2's k range does not split evenly; a call of NaNs before leaves NaNs
+    wherever a kernel keeps its operands."""
+    weights = _weights(E, H, I, T)
+    dev = _dev(weights)
+    ids, w = _routing(T, E, K, T + 1)
+    x = _x(T, H, T + 2)
+    assert torch.isnan(_run(torch.full_like(x, float("nan")), w, ids, dev)).all()
+    _close(_run(x, w, ids, dev), x, w, ids, weights)
+
+
+@pytest.mark.parametrize("H,I", [(32, 64), (128, 128)])
+def test_experts_of_many_tokens(H, I):
+    """More tokens than 16 bits count: the last rows are those of a small call."""
+    T, E, K = 70001, 3, 2
+    weights = _weights(E, H, I, 8)
+    dev = _dev(weights)
+    ids, w = _routing(T, E, K, 9)
+    x = _x(T, H, 10)
+    got = _run(x, w, ids, dev)
+    for part in (slice(0, 20), slice(65530, 65550), slice(T - 20, T)):
+        assert torch.equal(got[part], _run(x[part], w[part], ids[part], dev))
+        _close(got[part], x[part], w[part], ids[part], weights)
 
 
 @pytest.mark.parametrize("T,H,I,E,K", [s for s in SHAPES if s[0] in (1, 3, 17, 77, 300)])

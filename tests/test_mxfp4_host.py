@@ -109,6 +109,7 @@ def test_layer_descriptor(hiplib, kw):
 def test_work_bytes(hiplib):
     w = hiplib.wisp_moe_mxfp4_work_bytes
     assert w(0, 2, 64, 32, 4) == w(1, 0, 64, 32, 4) == w(1, 2, 64, 32, 0) == 0
+    assert w(1 << 26, 64, 64, 32, 4) == 0                # more pairs than 31 bits count
     assert w(1, 2, 64, 32, 4) >= 2 * 32 * 4              # act in float32
     assert w(100, 2, 64, 32, 4) >= 200 * 64 * 4          # y
     # a group of a call fits the call's buffer

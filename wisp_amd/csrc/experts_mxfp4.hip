@@ -273,8 +273,9 @@ struct Tile {
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[g][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     };
-    clear();  // (the last split may be empty)
-    // The first turn loads; what it computes is dropped.
+    clear();
+    // The first turn loads; what it computes is dropped.  (No range is empty:
+    // the grid's splits are w2_splits' or one.)
 #pragma unroll 1
     for (int c = from - kSub; c < to; c += kSub) {
       if (c == from) clear();
@@ -324,7 +325,7 @@ mx_grouped_kernel(GroupedArgs a) {
   t.n0 = (blockIdx.x * Sh::WR + t.wave) * t.per * 16;
   const uint32_t blocks = (uint32_t)(kW13 ? 2 * a.I : a.H) * (uint32_t)t.nblk;
   t.W = mx::buffer(a.W + (size_t)s * a.w_stride, blocks * mx::kBlockBytes);
-  t.S = mx::buffer(a.S + (size_t)s * a.s_stride, (blocks + 3) & ~3u);
+  t.S = mx::buffer(a.S + (size_t)s * a.s_stride, blocks);  // a multiple of four
 #pragma unroll
   for (int g = 0; g < Sh::NG; ++g)  // (tiles past the end repeat the last)
     t.tile0[g] = (g < t.per ? 0 : a.I) + min(t.n0 + g % t.per * 16, t.N - 16);
@@ -646,9 +647,9 @@ hipError_t launch_product(const GroupedArgs& a, int nslots, hipStream_t st, hipE
   };
   // (the tiles' token offsets are 32 bits wide)
   const uint64_t bytes = (uint64_t)(kW13 ? a.P / a.K : a.P) * (kW13 ? a.H : a.I) * 2;
-  if (a.splits == 1 && a.P >= kTilePairs * spread && (kW13 ? a.H : a.I) % kChunk == 0 && nslots <= kMaxExperts &&
-      bytes < 1ull << 32) {
-    const int panels = (int)(((kW13 ? a.I : a.H) + (kW13 ? 127 : 255)) / (kW13 ? 128 : 256));
+  if (a.splits == 1 && a.P >= kTilePairs * spread && (kW13 ? a.H : a.I) % kChunk == 0 &&
+      nslots <= kMaxExperts && bytes < 1ull << 32) {
+    const int panels = kW13 ? (a.I + 127) / 128 : (a.H + 255) / 256;
     return tile_cost<BigShape<4>>(a.P, spread, panels) < tile_cost<BigShape<6>>(a.P, spread, panels)
                ? launch_tiles<BigShape<4>, kW13>(a, nslots, st, e0, e1)
                : launch_tiles<BigShape<6>, kW13>(a, nslots, st, e0, e1);
@@ -685,15 +686,18 @@ __global__ __launch_bounds__(256) void mx_combine_kernel(const float* __restrict
 
 // Splits of w2's k range: a call whose panels are too few to fill the GPU (16
 // of 256 rows at H 4096), and whose block tiles would be, splits it into parts
-// of at least four stages.  It goes by the whole call alone, for the bytes
-// depend on it.  Measured, 1 / 4 splits, Mixtral, 6 tokens: w2 100 / 49 us.
+// of at least four stages, none of them empty (25 stages in six parts of five
+// would leave one).  It goes by the whole call alone, for the bytes depend on
+// it.  Measured, 1 / 4 splits, Mixtral, 6 tokens: w2 100 / 49 us.
 int w2_splits(int T, int K, int H, int I, int nslots) {
   const int panels = (H + 255) / 256;
   const double mean = (double)T * K / nslots;
   if (mean >= kTilePairs && ceil(mean / BigShape<6>::kToks) * nslots * panels >= tile::kBlocks)
     return 1;
   const double blocks = mx::distinct(T, K, nslots) * panels;
-  return std::max(1, std::min((int)ceil(512 / blocks), I / (4 * kStageK)));
+  const int splits = std::max(1, std::min((int)ceil(512 / blocks), I / (4 * kStageK)));
+  const int stages = (I + kStageK - 1) / kStageK, span = (stages + splits - 1) / splits;
+  return (stages + span - 1) / span;
 }
 
 // Work buffer (pair lists, counts, y).
@@ -840,7 +844,7 @@ int check_call(const void* x, int T, int H, int I, int K, int nslots, const void
 }  // namespace
 
 extern "C" size_t wisp_moe_mxfp4_work_bytes(int T, int K, int H, int I, int nslots) {
-  if (T < 1 || K < 1 || H < 1 || I < 1 || nslots < 1) return 0;
+  if (T < 1 || K < 1 || H < 1 || I < 1 || nslots < 1 || (int64_t)T * K > 0x7fffffff) return 0;
   return wisp::mxfp4_work_bytes(wisp::mxfp4_plan(T, K, H, I, nslots), T, K, H, I, nslots);
 }
 

@@ -108,9 +108,9 @@ __global__ __launch_bounds__(256) void mx_few_w13_kernel(FewW13 a, Src src) {
     s = __builtin_amdgcn_readfirstlane(chosen);
   }
   const int i = (blockIdx.x * 4 + wave) * 4 + (lane >> 4);  // I is a multiple of 32
-  const uint32_t blocks = 2u * a.I * nblk;
+  const uint32_t blocks = 2u * a.I * nblk;  // a multiple of four
   const mx::Buffer W = mx::buffer(a.W + (size_t)s * a.w_stride, blocks * mx::kBlockBytes);
-  const mx::Buffer S = mx::buffer(a.S + (size_t)s * a.s_stride, (blocks + 3) & ~3u);
+  const mx::Buffer S = mx::buffer(a.S + (size_t)s * a.s_stride, blocks);
   const uint32_t row[2] = {(uint32_t)i * nblk, (uint32_t)(a.I + i) * nblk};
   float sum[2] = {0.f, 0.f};
   for (int b0 = 0; b0 < nblk; b0 += 16 * kTurn) {
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(64 * kW2Waves) void mx_few_w2_kernel(FewW2 a) {
     float sum = 0.f;
     if (s >= 0 && s < a.nslots) {
       const mx::Buffer W = mx::buffer(a.W + (size_t)s * a.w_stride, blocks * mx::kBlockBytes);
-      const mx::Buffer S = mx::buffer(a.S + (size_t)s * a.s_stride, (blocks + 3) & ~3u);
+      const mx::Buffer S = mx::buffer(a.S + (size_t)s * a.s_stride, blocks);
       const u32x4* ap = reinterpret_cast<const u32x4*>(a.act + (size_t)p * a.I);
       for (int b0 = from; b0 < to; b0 += kWindow) {
         u32x4 w[kW2Turn], v[kW2Turn];
