@@ -45,6 +45,21 @@ struct Shape {
   static constexpr int kWaveW = NG * 16 * 128;            // a wave's codes of a stage
 };
 
+// Where the 16-byte pieces of row r stand: piece b at b ^ swizzle(r), in
+// 256-byte token rows and in the block tiles' 64-byte code rows.  Lane l reads
+// row l % 16 at a piece that depends on l / 16, and one cycle of a 16-byte LDS
+// read serves groups of four lanes of different l / 16 together, so pieces
+// that differ by l / 16 must not meet between such groups.  The row's own
+// number as the swizzle does: 17 to 41 % of the LDS cycles were bank
+// conflicts, now none in the grouped kernel and 9 % in the tiles.  Measured
+// (us a call): Qwen3, 512 tokens 111.7 -> 108.7, Mixtral, 1000 873 -> 855.
+__device__ __attribute__((always_inline)) inline int token_swizzle(int r) {
+  return (r & 3) << 2 | (r >> 2 & 3);
+}
+__device__ __attribute__((always_inline)) inline int code_swizzle(int r) {
+  return (r >> 2 & 1) * 3 ^ (r >> 3 & 1);
+}
+
 struct GroupedArgs {
   const uint16_t* A;  // token matrix: x (w13) or act (w2)
   int H, I, K, P;
@@ -92,7 +107,7 @@ __device__ inline void store_act4(uint16_t* p, const f32x4& g, const f32x4& u) {
 // k = 32 (l / 16) + 8 j .. + 7.  Lane l loads the scales of the wave's row l.
 //
 // Token rows are copied to LDS asynchronously one chunk ahead, 256 bytes of
-// each, 16-byte piece b of row r at position b ^ (r % 16).
+// each, its pieces swizzled (token_swizzle).
 //
 // kOdd: rows that are not whole stages.  Blocks past a row's end read as
 // zeros, and each lane loads its own blocks' scales.
@@ -207,7 +222,7 @@ struct Tile {
     const bool none = kOdd && (c + h) * 4 + q >= nblk;
     auto token = [&](int i, int j) {
       const u32x4 v = *reinterpret_cast<const u32x4*>(rds + (i * 16 + (lane & 15)) * kTokBytes +
-                                                      (((q * 4 + j) ^ (lane & 15)) << 4));
+                                                      (((q * 4 + j) ^ token_swizzle(lane)) << 4));
       return none ? u32x4{} : v;
     };
 #pragma unroll
@@ -262,7 +277,7 @@ struct Tile {
     for (int i = 0; i < NC; ++i) {
       const int r = (i * Sh::WR + wave) * kTokPerCopy + (lane >> 4);
       const int p = list[m0 + min(r, mrows - 1)];
-      tok.piece[i] = (lane & 15) ^ (r & 15);
+      tok.piece[i] = (lane & 15) ^ token_swizzle(r);
       tok.src[i] = reinterpret_cast<const unsigned char*>(
           a.A + (size_t)(kW13 ? p / a.K : p) * Kdim + tok.piece[i] * 8);
     }
@@ -397,7 +412,7 @@ struct BigTile {
       const int r = (i * Big::kWaves + wave) * kTokPerCopy + q;
       const int p = __shfl(pr, i * kTokPerCopy + q);
       s.src[i] = (uint32_t)(kW13 ? p / a.K : p) * (uint32_t)(Kdim * 2) +
-                 (((lane & 15) ^ (r & 15)) << 4);
+                 (((lane & 15) ^ token_swizzle(r)) << 4);
     }
     const uint32_t blocks = (uint32_t)(kW13 ? 2 * a.I : a.H) * (uint32_t)nblk;
     s.W = mx::buffer(a.W + (size_t)w.slot * a.w_stride, blocks * mx::kBlockBytes);
@@ -434,20 +449,19 @@ struct BigTile {
     u32x4 codes[NG], v0[NG];
     float scale[NG];
   };
-  // Through the wave's own LDS: 16-byte block b of row r at position
-  // b ^ (r / 4 % 4).
+  // Through the wave's own LDS (code_swizzle).
   __device__ __attribute__((always_inline)) void put(const Weights& w) const {
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const int r = g * 16 + (lane >> 2);
-      *reinterpret_cast<u32x4*>(wlds + r * 64 + (((lane & 3) ^ (r >> 2 & 3)) << 4)) = w.w[g];
+      *reinterpret_cast<u32x4*>(wlds + r * 64 + (((lane & 3) ^ code_swizzle(r)) << 4)) = w.w[g];
     }
   }
   __device__ __attribute__((always_inline)) void get(uint32_t s, Operands& o) const {
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const int r = g * 16 + (lane & 15);
-      o.codes[g] = *reinterpret_cast<const u32x4*>(wlds + r * 64 + ((q ^ (r >> 2 & 3)) << 4));
+      o.codes[g] = *reinterpret_cast<const u32x4*>(wlds + r * 64 + ((q ^ code_swizzle(r)) << 4));
       o.scale[g] = __uint_as_float(mx::scale_of(__shfl((int)s, r), q));
     }
   }
@@ -470,7 +484,7 @@ struct BigTile {
     auto token = [&](int i, int j) {
       return *reinterpret_cast<const u32x4*>(
           rds + ((i * Big::WT + wt) * 16 + (lane & 15)) * kTokBytes +
-          (((q * 4 + j) ^ (lane & 15)) << 4));
+          (((q * 4 + j) ^ token_swizzle(lane)) << 4));
     };
 #pragma unroll
     for (int i = 0; i < NT; ++i) t[i] = token(i, 0);
