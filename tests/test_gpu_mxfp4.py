@@ -181,6 +181,7 @@ SHAPES = [  # T, H, I, E, K
     (200, 128, 192, 3, 1), (300, 512, 256, 16, 2), (600, 256, 416, 2, 2), (1100, 384, 288, 3, 2),
     (12, 64, 4160, 6, 4), (20, 96, 3104, 4, 4), (40, 128, 9216, 3, 2), (130, 128, 128, 2, 1),
     (200, 256, 640, 3, 2), (401, 512, 128, 2, 2), (1300, 256, 384, 5, 1),
+    (250, 256, 512, 4, 1), (250, 160, 96, 4, 1), (330, 256, 512, 4, 1), (330, 160, 96, 4, 1),
 ]
 
 

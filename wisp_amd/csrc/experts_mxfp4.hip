@@ -157,21 +157,22 @@ struct Tile {
     }
   }
 
-  // Token copies of a pass: this lane's source pieces of chunk 0.
+  // Token copies of a pass: their rows, and this lane's piece of each in chunk 0.
   struct Tokens {
-    const unsigned char* src[NC];
-    int piece[NC];  // with kOdd
+    uint32_t row[NC];
+    int piece;
   };
   __device__ __attribute__((always_inline)) void copy(int c, const Tokens& t,
                                                       unsigned char* stage) const {
+    // (before the first chunk the first, past a row's end its last piece once
+    // more: no product uses it)
+    const int b = kOdd ? min(max(c, 0) * 16 + t.piece, Kdim / 8 - 1)
+                       : max(min(c, chunks - 1), 0) * 16 + t.piece;
+    const unsigned char* src = reinterpret_cast<const unsigned char*>(a.A) + b * 16;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      // (before the first chunk the first, past a row's end its last piece
-      // once more: no product uses it)
-      const int b = kOdd ? min(max(c, 0) * 16 + t.piece[i], Kdim / 8 - 1) - t.piece[i]
-                         : max(min(c, chunks - 1), 0) * 16;
-      dma::dma16(t.src[i] + (ptrdiff_t)b * 16, stage + (i * Sh::WR + wave) * 1024);
-    }
+    for (int i = 0; i < NC; ++i)
+      dma::dma16(src + (uint64_t)t.row[i] * (uint32_t)(Kdim * 2),
+                 stage + (i * Sh::WR + wave) * 1024);
   }
 
   // A wave's codes of a chunk in operand order, their scales, and the operands
@@ -217,6 +218,9 @@ struct Tile {
     // this chunk's tokens have landed: all loads but the youngest, the weights
     dma::wait_vm<h == 0 ? 0 : kLoads>();
     dma::lds_barrier();
+    // (six token tiles leave no registers for a second set of operands: with one,
+    // made behind the last tile, 6 to 14 us of 160 to 310 a call less in spills)
+    constexpr bool kOne = NT > 5;
     u32x4 t[NT], v1[NG];
     // (what stands past a row's end may be an infinity)
     const bool none = kOdd && (c + h) * 4 + q >= nblk;
@@ -231,8 +235,8 @@ struct Tile {
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      u32x4(&v)[NG] = j & 1 ? v1 : o.v0;
-      u32x4(&vn)[NG] = j & 1 ? o.v0 : v1;
+      u32x4(&v)[NG] = kOne || j % 2 == 0 ? o.v0 : v1;
+      u32x4(&vn)[NG] = kOne || j % 2 == 1 ? o.v0 : v1;
       if (j == 3) {
         if constexpr (h == 1) {
           put(w);
@@ -249,13 +253,12 @@ struct Tile {
 #pragma unroll
         for (int g = 0; g < NG; ++g) acc[g][i] = mx::mfma(v[g], t[i], acc[g][i]);
         if (j < 3) t[i] = token(i, j + 1);
+        // the operands made behind tile i
+        const bool late = kOne || j == 3;
+        const int g0 = late ? (i == NT - 1 ? 0 : NG) : i * NG / NT;
+        const int g1 = late ? NG : (i + 1) * NG / NT;
 #pragma unroll
-        for (int g = i * NG / NT; g < (i + 1) * NG / NT; ++g)
-          if (j < 3 || i == NT - 1) vn[g] = mx::bf16_of(o.codes[g][(j + 1) & 3], o.scale[g]);
-        if (j == 3 && i == NT - 1) {
-#pragma unroll
-          for (int g = 0; g < i * NG / NT; ++g) vn[g] = mx::bf16_of(o.codes[g][0], o.scale[g]);
-        }
+        for (int g = g0; g < g1; ++g) vn[g] = mx::bf16_of(o.codes[g][(j + 1) & 3], o.scale[g]);
         // (all loads at once would fill the address unit's queue)
         if (h == 0 && j < 2) {
 #pragma unroll
@@ -273,13 +276,12 @@ struct Tile {
     Operands o = {};
     uint32_t s[NS] = {};
     Tokens tok;
+    static_assert(Sh::WR * kTokPerCopy % 16 == 0, "a lane's rows have one swizzle");
+    tok.piece = (lane & 15) ^ token_swizzle(wave * kTokPerCopy + (lane >> 4));
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int r = (i * Sh::WR + wave) * kTokPerCopy + (lane >> 4);
-      const int p = list[m0 + min(r, mrows - 1)];
-      tok.piece[i] = (lane & 15) ^ token_swizzle(r);
-      tok.src[i] = reinterpret_cast<const unsigned char*>(
-          a.A + (size_t)(kW13 ? p / a.K : p) * Kdim + tok.piece[i] * 8);
+      const int p = list[m0 + min((i * Sh::WR + wave) * kTokPerCopy + (lane >> 4), mrows - 1)];
+      tok.row[i] = kW13 ? p / a.K : p;
     }
     f32x4 acc[NG][NT];
     auto clear = [&] {
@@ -616,10 +618,10 @@ hipError_t launch_grouped(const GroupedArgs& a, dim3 grid, hipStream_t st, hipEv
 }
 
 // Calls of at least this many pairs a slot take the block tiles: from here the
-// blocks above pass over a slot's weights twice.  Measured, the blocks above
-// against tiles (us a call): Qwen3 199 / 202 at 64 pairs a slot, 231 / 206 at
-// 80, 314 / 298 at 128; Mixtral 341 / 403 at 64, 429 / 417 at 80.
-constexpr int kTilePairs = 72;
+// blocks above pass over most slots' weights twice.  Measured, the blocks above
+// against tiles (us a call): Qwen3 177 / 212 at 72 pairs a slot, 211 / 213 at
+// 80; Mixtral 325 / 449 at 80, 408 / 452 at 90, 508 / 457 at 100.
+constexpr int kTilePairs = 84;
 
 // How long a call's tiles of this shape take, in token tiles of a wave (a
 // chunk costs a wave about half a token tile besides its products): the
@@ -648,6 +650,35 @@ hipError_t launch_tiles(const GroupedArgs& a, int nslots, hipStream_t st, hipEve
   return hipSuccess;
 }
 
+// The token tiles (of 16) of a pass of the grouped kernel: those by which the
+// slots' passes take the least.  A pass with more tiles takes longer (kPass, the
+// times of calls of one pass over many experts), one with fewer leaves more
+// slots a second pass over their weights.  The slots' pairs lie around their
+// mean by the spread of a random router's; where the blocks do not fill the GPU
+// the fullest slot alone counts.  Measured, NT / NT + 1 (us a call; M: Mixtral,
+// else Qwen3): 8 pairs a slot 81 / 81, 9: 89 / 81; 20: 97 / 98, 22: 105 / 99;
+// 34: 113 / 115, 40: 144 / 117; 44: 121 / 129, 56: 169 / 139, M 50: 224 / 244,
+// M 54: 273 / 247; 64: 163 / 169, 72: 207 / 177, M 64: 262 / 302, M 72:
+// 331 / 302.  The fullest slot: 24 experts of 1056 x 352 at 87 pairs a slot,
+// 4 / 6 tiles 73 / 98.
+int token_tiles(int P, int spread, int K, int64_t blocks) {
+  constexpr double kPass[] = {1, 1.08, 1.25, 1.45, 1.7, 2};
+  const double mean = (double)P / spread;
+  const double dev = sqrt(mean * (1 - std::min(1.0, (double)K / spread)));
+  const double fullest = 0.93 + 0.22 * log2((double)spread);  // in devs, of so many slots
+  int best = 1;
+  double least = 0;
+  for (int nt = 1; nt <= 6; ++nt) {
+    double passes = 0;
+    for (double z : {-1.3, -0.5, 0.5, 1.3})
+      passes += ceil(std::max(1.0, mean + (blocks < 512 ? fullest : z) * dev) / (16 * nt));
+    passes += ceil((mean + fullest * dev) / (16 * nt));
+    const double cost = passes * kPass[nt - 1];
+    if (nt == 1 || cost < least) best = nt, least = cost;
+  }
+  return best;
+}
+
 template <bool kW13>
 hipError_t launch_product(const GroupedArgs& a, int nslots, hipStream_t st, hipEvent_t e0,
                           hipEvent_t e1) {
@@ -661,17 +692,21 @@ hipError_t launch_product(const GroupedArgs& a, int nslots, hipStream_t st, hipE
   };
   // (the tiles' token offsets are 32 bits wide)
   const uint64_t bytes = (uint64_t)(kW13 ? a.P / a.K : a.P) * (kW13 ? a.H : a.I) * 2;
+  const int panels = kW13 ? (a.I + 127) / 128 : (a.H + 255) / 256;
   if (a.splits == 1 && a.P >= kTilePairs * spread && (kW13 ? a.H : a.I) % kChunk == 0 &&
       nslots <= kMaxExperts && bytes < 1ull << 32) {
-    const int panels = kW13 ? (a.I + 127) / 128 : (a.H + 255) / 256;
     return tile_cost<BigShape<4>>(a.P, spread, panels) < tile_cost<BigShape<6>>(a.P, spread, panels)
                ? launch_tiles<BigShape<4>, kW13>(a, nslots, st, e0, e1)
                : launch_tiles<BigShape<6>, kW13>(a, nslots, st, e0, e1);
   }
-  if (a.P <= 8 * spread) return go(Shape<4, 4, 1>{});
-  if (a.P <= 20 * spread) return go(Shape<4, 4, 2>{});
-  if (a.P <= 34 * spread) return go(Shape<4, 4, 3>{});
-  return go(Shape<4, 4, 4>{});
+  switch (token_tiles(a.P, spread, a.K, (int64_t)panels * spread * a.splits)) {
+    case 1: return go(Shape<4, 4, 1>{});
+    case 2: return go(Shape<4, 4, 2>{});
+    case 3: return go(Shape<4, 4, 3>{});
+    case 4: return go(Shape<4, 4, 4>{});
+    case 5: return go(Shape<4, 4, 5>{});
+    default: return go(Shape<4, 4, 6>{});
+  }
 }
 
 // out[t, h] = bf16(sum_k w[t,k] * sum_z y[z, (t,k), h]), k and z ascending;
