@@ -206,6 +206,18 @@ def test_experts_of_a_long_inner_range(T, H, I, E, K):
     _close(_run(x, w, ids, dev), x, w, ids, weights)
 
 
+@pytest.mark.parametrize("T", [1, 20, 400])
+def test_experts_of_large_gates(T):
+    """Gates from -1500 to 1500: the exponential of their negative overflows."""
+    E, H, I, K = 2, 256, 128, 1
+    weights = _weights(E, H, I, 21, std=10.0)
+    ids, w = _routing(T, E, K, 22)
+    x = _x(T, H, 23)
+    g = x[:1].double().numpy() @ O.dequantize(weights[0][ids[0, 0]], weights[1][ids[0, 0]])[:I].T
+    assert (g < -95).any() and (g > 95).any()
+    _close(_run(x, w, ids, weights), x, w, ids, weights)
+
+
 @pytest.mark.parametrize("H,I", [(32, 64), (128, 128)])
 def test_experts_of_many_tokens(H, I):
     """More tokens than 16 bits count: the last rows are those of a small call."""

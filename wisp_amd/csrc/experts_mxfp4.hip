@@ -75,14 +75,14 @@ struct GroupedArgs {
 
 // g / (1 + e^-g), its last few float32 bits apart: act is rounded to bf16.
 // (The exponential's argument is clamped where e^-g is 0 or infinite anyway,
-// so that an infinite g gives what the formula does.)
+// so that an infinite g gives what the formula does; what t's rounding left
+// enters as a factor near 1, which leaves an infinite power one.)
 __device__ inline float silu_fast(float g) {
   constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596299e-8f, kLn2 = 0.693147182f;
   const float n = __builtin_amdgcn_fmed3f(-g, -104.f, 89.f);
   const float t = n * kLog2e;
-  const float low = fmaf(n, kLog2e, -t) + n * kLog2eLow;  // what t's rounding left
-  float e = __builtin_amdgcn_exp2f(t);
-  e = fmaf(e * kLn2, low, e);
+  const float low = fmaf(n, kLog2e, -t) + n * kLog2eLow;
+  const float e = __builtin_amdgcn_exp2f(t) * fmaf(kLn2, low, 1.f);
   return g * __builtin_amdgcn_rcpf(1.f + e);
 }
 
