@@ -182,6 +182,8 @@ SHAPES = [  # T, H, I, E, K
     (12, 64, 4160, 6, 4), (20, 96, 3104, 4, 4), (40, 128, 9216, 3, 2), (130, 128, 128, 2, 1),
     (200, 256, 640, 3, 2), (401, 512, 128, 2, 2), (1300, 256, 384, 5, 1),
     (250, 256, 512, 4, 1), (250, 160, 96, 4, 1), (330, 256, 512, 4, 1), (330, 160, 96, 4, 1),
+    (280, 128, 12800, 2, 1), (350, 128, 12800, 2, 1), (280, 25600, 128, 2, 1),
+    (350, 25600, 128, 2, 1),
 ]
 
 

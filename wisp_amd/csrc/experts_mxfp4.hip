@@ -356,7 +356,7 @@ mx_grouped_kernel(GroupedArgs a) {
 
 // ---------------------------------------------------------------------------
 // Large calls: the same products in tiles of 256 weight rows (w13: 128 gate
-// and 128 up rows) by up to 128 or 192 tokens of a slot, eight waves in persistent
+// and 128 up rows) by up to 128, 160 or 192 tokens of a slot, eight waves in persistent
 // blocks, one per CU: wave (wr, wt) holds 64 rows against the token tiles wt,
 // wt + 2, ... of 16.  Stages are single chunks; the last chunk of a tile
 // already loads the first of the next.  The matrix instructions and the k
@@ -623,19 +623,31 @@ hipError_t launch_grouped(const GroupedArgs& a, dim3 grid, hipStream_t st, hipEv
 // 80; Mixtral 325 / 449 at 80, 408 / 452 at 90, 508 / 457 at 100.
 constexpr int kTilePairs = 84;
 
+// The pairs of a call's slots: their mean, the deviation that a random router
+// gives them, and how many deviations the fullest of so many slots has more.
+struct Spread {
+  double mean, dev, fullest;
+  Spread(int P, int slots, int K)
+      : mean((double)P / slots),
+        dev(sqrt(mean * (1 - std::min(1.0, (double)K / slots)))),
+        fullest(0.93 + 0.22 * log2((double)slots)) {}
+};
+
 // How long a call's tiles of this shape take, in token tiles of a wave (a
-// chunk costs a wave about half a token tile besides its products): the
-// rounds of 256 blocks, for slots of the average length, give or take the
-// square root that a random router's have.  Measured, shapes of 128 / 192
-// tokens (us): w13 and w2 of the Qwen3 8192-token chunk (512 a slot) 491 /
-// 448 and 322 / 299, of the Mixtral 1000-token chunk (250 a slot) 541 / 626 and
-// 449 / 316 (w2's few panels: 298 tiles are two rounds, 256 one).
+// chunk costs a wave about two token tiles besides its products): halfway
+// between their rounds of 256 blocks and their share of a round, since not every
+// block of the last round has a tile.  Measured, 128 / 160 / 192 tokens (us a
+// call): Qwen3 217 / 225 / 246 at 96 pairs a slot, 256 / 232 / 253 at 112, 355 /
+// 295 / 268 at 144, 372 / 407 / 387 at 187, 488 / 441 / 482 at 256, 884 / 857 /
+// 785 at 512; Mixtral 545 / 488 / 517 at 128, 690 / 751 / 582 at 175, 728 / 806
+// / 893 at 212, 1038 / 812 / 901 at 250.
 template <typename Big>
-double tile_cost(int P, int spread, int panels) {
-  const double mean = (double)P / spread, dev = sqrt(mean);
-  double tiles = 0;
-  for (double m : {mean - dev, mean, mean + dev}) tiles += ceil(m / Big::kToks) / 3 * spread;
-  return ceil(tiles * panels / tile::kBlocks) * (Big::NT + 0.6);
+double tile_cost(const Spread& s, int slots, int panels) {
+  auto of = [](double m) { return ceil(std::max(m, 1.0) / Big::kToks); };
+  const double tiles = (of(s.mean - s.dev) + of(s.mean) + of(s.mean + s.dev) +
+                        0.5 * of(s.mean + s.fullest * s.dev)) / 3.5 * slots;
+  const double rounds = tiles * panels / tile::kBlocks;
+  return 0.5 * (ceil(rounds) + std::max(rounds, 1.0)) * (Big::NT + 2);
 }
 
 template <typename Big, bool kW13>
@@ -653,26 +665,22 @@ hipError_t launch_tiles(const GroupedArgs& a, int nslots, hipStream_t st, hipEve
 // The token tiles (of 16) of a pass of the grouped kernel: those by which the
 // slots' passes take the least.  A pass with more tiles takes longer (kPass, the
 // times of calls of one pass over many experts), one with fewer leaves more
-// slots a second pass over their weights.  The slots' pairs lie around their
-// mean by the spread of a random router's; where the blocks do not fill the GPU
+// slots a second pass over their weights.  Where the blocks do not fill the GPU
 // the fullest slot alone counts.  Measured, NT / NT + 1 (us a call; M: Mixtral,
 // else Qwen3): 8 pairs a slot 81 / 81, 9: 89 / 81; 20: 97 / 98, 22: 105 / 99;
 // 34: 113 / 115, 40: 144 / 117; 44: 121 / 129, 56: 169 / 139, M 50: 224 / 244,
 // M 54: 273 / 247; 64: 163 / 169, 72: 207 / 177, M 64: 262 / 302, M 72:
 // 331 / 302.  The fullest slot: 24 experts of 1056 x 352 at 87 pairs a slot,
 // 4 / 6 tiles 73 / 98.
-int token_tiles(int P, int spread, int K, int64_t blocks) {
+int token_tiles(const Spread& s, int64_t blocks) {
   constexpr double kPass[] = {1, 1.08, 1.25, 1.45, 1.7, 2};
-  const double mean = (double)P / spread;
-  const double dev = sqrt(mean * (1 - std::min(1.0, (double)K / spread)));
-  const double fullest = 0.93 + 0.22 * log2((double)spread);  // in devs, of so many slots
   int best = 1;
   double least = 0;
   for (int nt = 1; nt <= 6; ++nt) {
     double passes = 0;
     for (double z : {-1.3, -0.5, 0.5, 1.3})
-      passes += ceil(std::max(1.0, mean + (blocks < 512 ? fullest : z) * dev) / (16 * nt));
-    passes += ceil((mean + fullest * dev) / (16 * nt));
+      passes += ceil(std::max(1.0, s.mean + (blocks < 512 ? s.fullest : z) * s.dev) / (16 * nt));
+    passes += ceil((s.mean + s.fullest * s.dev) / (16 * nt));
     const double cost = passes * kPass[nt - 1];
     if (nt == 1 || cost < least) best = nt, least = cost;
   }
@@ -683,6 +691,7 @@ template <bool kW13>
 hipError_t launch_product(const GroupedArgs& a, int nslots, hipStream_t st, hipEvent_t e0,
                           hipEvent_t e1) {
   const int spread = std::min(a.P, nslots);
+  const Spread pairs(a.P, spread, a.K);
   auto go = [&](auto shape) {
     using Sh = decltype(shape);
     constexpr int per = Sh::kRows / (kW13 ? 2 : 1);
@@ -695,11 +704,14 @@ hipError_t launch_product(const GroupedArgs& a, int nslots, hipStream_t st, hipE
   const int panels = kW13 ? (a.I + 127) / 128 : (a.H + 255) / 256;
   if (a.splits == 1 && a.P >= kTilePairs * spread && (kW13 ? a.H : a.I) % kChunk == 0 &&
       nslots <= kMaxExperts && bytes < 1ull << 32) {
-    return tile_cost<BigShape<4>>(a.P, spread, panels) < tile_cost<BigShape<6>>(a.P, spread, panels)
-               ? launch_tiles<BigShape<4>, kW13>(a, nslots, st, e0, e1)
-               : launch_tiles<BigShape<6>, kW13>(a, nslots, st, e0, e1);
+    const double c4 = tile_cost<BigShape<4>>(pairs, spread, panels),
+                 c5 = tile_cost<BigShape<5>>(pairs, spread, panels),
+                 c6 = tile_cost<BigShape<6>>(pairs, spread, panels);
+    return c4 < std::min(c5, c6) ? launch_tiles<BigShape<4>, kW13>(a, nslots, st, e0, e1)
+           : c5 < c6             ? launch_tiles<BigShape<5>, kW13>(a, nslots, st, e0, e1)
+                                 : launch_tiles<BigShape<6>, kW13>(a, nslots, st, e0, e1);
   }
-  switch (token_tiles(a.P, spread, a.K, (int64_t)panels * spread * a.splits)) {
+  switch (token_tiles(pairs, (int64_t)panels * spread * a.splits)) {
     case 1: return go(Shape<4, 4, 1>{});
     case 2: return go(Shape<4, 4, 2>{});
     case 3: return go(Shape<4, 4, 3>{});
