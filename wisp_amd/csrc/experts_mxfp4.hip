@@ -6,6 +6,14 @@
 // becomes its bf16 value, which is exact, in registers on its way into the
 // instruction: one conversion instruction gives two values with their scale
 // applied.
+//
+// Small and middle calls (mx_grouped_kernel) are bound by the stream of weights,
+// large ones (mx_tile_kernel) by the matrix instructions and what feeds them.
+// Measured (us, w13 + w2): Qwen3, 32 tokens 37 + 24 (5.0 and 3.9 TB/s of
+// weights; w2's rows are three stages, behind one that only loads), 512 tokens
+// 56 + 39; Mixtral, 6 tokens 75 + 50 (5.5 and 4.1); Qwen3, 8192 tokens 440 + 282
+// (940 and 730 TFLOP/s; w2 also writes 537 MB of y), Mixtral, 1000 tokens 565 +
+// 281 (830 and 840).
 #include <math.h>
 
 #include <algorithm>

@@ -6,7 +6,9 @@
 // each, so every pair has blocks of its own (an expert of two tokens is read
 // twice, the second time from cache), the sums are vector dot products (no
 // trip through LDS into a matrix operand's order), and act stays in float32
-// between the launches.
+// between the launches.  Measured (us, w13 + w2; a whole call in a graph):
+// Qwen3, one token 7.5 + 6.2; 12.5 (20 MB of weights, 4 us at the rate of a large
+// copy), 512 x 256 with 16 experts 3.9 + 4.0; 7.3.
 #include <algorithm>
 
 #include "experts_mxfp4.h"

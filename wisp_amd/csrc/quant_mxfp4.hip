@@ -10,7 +10,10 @@
 //
 // Both are streams: a lane holds eight values, one word of codes, and four
 // lanes hold a block, so that every load and store of a wave is one
-// contiguous run (16 bytes of bf16 or two times 16 of float32 a lane).
+// contiguous run (16 bytes of bf16 or two times 16 of float32 a lane); a thread
+// has four words' loads in flight.  Bound by memory.  Measured, bf16: 24576 x
+// 2048 values quantised in 24.3 us (5.2 TB/s of values, codes and scales) and
+// read back in 19.7 us (6.5 TB/s), 28672 x 4096 read back in 48 us (6.2 TB/s).
 #include "mxfp4.h"
 
 namespace wisp {
