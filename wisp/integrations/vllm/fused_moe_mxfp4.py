@@ -46,11 +46,15 @@ def _on_device(fn):
         t = args[0] if args else kwargs.get(first)
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise ValueError(f"wisp.mxfp4: {fn.__name__} takes device tensors")
-        if t.get_device() == torch.cuda.current_device():
+        if t.get_device() == torch._C._cuda_getDevice():  # (current_device() without its checks)
             return fn(*args, **kwargs)
         with torch.cuda.device(t.device):
             return fn(*args, **kwargs)
     return call
+
+
+def _stream(t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 @_on_device
@@ -72,7 +76,7 @@ def quantize_mxfp4(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     scales = torch.empty((*w.shape[:-1], C // BLOCK), dtype=torch.uint8, device=w.device)
     if w.numel():
         check(lib().wisp_quant_mxfp4(w.data_ptr(), _DTYPES[w.dtype], w.numel() // C, C,
-                                     codes.data_ptr(), scales.data_ptr(), _lib.stream_handle()),
+                                     codes.data_ptr(), scales.data_ptr(), _stream(w)),
               "quantize_mxfp4")
     return codes, scales
 
@@ -91,7 +95,8 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor,
             codes.shape[-1] % 16:
         raise ValueError(f"wisp.mxfp4: codes {tuple(codes.shape)} and scales "
                          f"{tuple(scales.shape)} disagree (16 bytes of codes a scale)")
-    _require_device(scales, codes.device, "scales")
+    if scales.get_device() != codes.get_device():
+        _require_device(scales, codes.device, "scales")
     codes, scales = codes.contiguous(), scales.contiguous()
     if codes.data_ptr() % 4:
         codes = codes.clone()
@@ -99,7 +104,7 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor,
     out = torch.empty((*codes.shape[:-1], C), dtype=dtype, device=codes.device)
     if out.numel():
         check(lib().wisp_dequant_mxfp4(codes.data_ptr(), scales.data_ptr(), out.numel() // C, C,
-                                       out.data_ptr(), _DTYPES[dtype], _lib.stream_handle()),
+                                       out.data_ptr(), _DTYPES[dtype], _stream(codes)),
               "dequantize_mxfp4")
     return out
 
@@ -157,8 +162,9 @@ def experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, slots: torch.Tensor, w1
     if slots.dim() != 2 or slots.shape[0] != T or topk_w.shape != slots.shape or \
             slots.dtype != torch.int32 or topk_w.dtype != torch.float32:
         raise ValueError(f"wisp.mxfp4: topk_w float32 and slots int32 must be [{T}, K]")
-    _require_device(slots, x.device, "slots")
-    _require_device(topk_w, x.device, "topk_w")
+    for t in (slots, topk_w):
+        if t.get_device() != x.get_device():
+            _require_device(t, x.device, "the routing")
     K = slots.shape[1]
     x, slots, topk_w = x.contiguous(), slots.contiguous(), topk_w.contiguous()
     out = _output(x, out)
@@ -172,7 +178,7 @@ def experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, slots: torch.Tensor, w1
     check(lib().wisp_moe_experts_mxfp4(
         x.data_ptr(), T, H, I, K, topk_w.data_ptr(), slots.data_ptr(), E, w13.data_ptr(),
         w13.stride(0), s13.data_ptr(), s13.stride(0), w2.data_ptr(), w2.stride(0), s2.data_ptr(),
-        s2.stride(0), p, out.data_ptr(), p + work, nbytes, _lib.stream_handle()), "experts_mxfp4")
+        s2.stride(0), p, out.data_ptr(), p + work, nbytes, _stream(x)), "experts_mxfp4")
     return out
 
 
@@ -190,7 +196,8 @@ def route_and_experts_mxfp4(x: torch.Tensor, router_logits: torch.Tensor, top_k:
         raise ValueError(f"wisp.mxfp4: router_logits must be [{T}, {E}]")
     if not 1 <= K <= E:
         raise ValueError(f"wisp.mxfp4: top_k={top_k} outside [1, {E}]")
-    _require_device(router_logits, x.device, "router_logits")
+    if router_logits.get_device() != x.get_device():
+        _require_device(router_logits, x.device, "router_logits")
     if router_logits.dtype not in _DTYPES:
         router_logits = router_logits.float()
     x, router_logits = x.contiguous(), router_logits.contiguous()
@@ -204,7 +211,7 @@ def route_and_experts_mxfp4(x: torch.Tensor, router_logits: torch.Tensor, top_k:
         x.data_ptr(), router_logits.data_ptr(), _DTYPES[router_logits.dtype], T, H, I, E, K,
         int(bool(renormalize)), p + routing, p + routing + 4 * T * K,
         w13.data_ptr(), w13.stride(0), s13.data_ptr(), s13.stride(0), w2.data_ptr(), w2.stride(0),
-        s2.data_ptr(), s2.stride(0), p, out.data_ptr(), p + work, nbytes, _lib.stream_handle()),
+        s2.data_ptr(), s2.stride(0), p, out.data_ptr(), p + work, nbytes, _stream(x)),
         "route_and_experts_mxfp4")
     return out
 
