@@ -387,6 +387,26 @@ def test_experts_other_stream_and_graph():
             assert torch.equal(r, b)
 
 
+@pytest.mark.parametrize("T,H,I,E,K", [(700, 256, 256, 6, 1), (30, 128, 2304, 4, 2)])
+def test_layer_in_a_graph(T, H, I, E, K):
+    """The block tiles, and w2's k range in parts, captured and replayed with
+    eager calls between."""
+    w13, s13, w2, s2 = _dev(_weights(E, H, I, 31))
+    x, lg = _x(T, H, 32).to(DEV), torch.randn((T, E), device=DEV)
+    call = lambda: mx.route_and_experts_mxfp4(x, lg, K, True, w13, w2, s13, s2)  # noqa: E731
+    call()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = call()
+    for _ in range(3):
+        x.mul_(-0.5)
+        lg.copy_(lg.flip(1))
+        want = call()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_experts_refusals():
     E, H, I, K, T = 4, 64, 32, 2, 3
     w13, s13, w2, s2 = _dev(_weights(E, H, I, 6))

@@ -80,6 +80,26 @@ def test_paged_trace(masters, monkeypatch, engine, logits):
     assert res.stats_forward == len(tokens)
 
 
+@pytest.mark.parametrize("H,I,tokens", [(256, 256, [1, 400, 30, 700]), (128, 2304, [5, 20, 60, 1]),
+                                        (128, 12800, [40, 350])])
+def test_paged_equals_resident(H, I, tokens):
+    """Where a resident call runs in block tiles or w2's k range in parts."""
+    E, K, g = 6, 2, torch.Generator().manual_seed(11)
+    w13 = (torch.randn((E, 2 * I, H), generator=g) * 0.05).to(torch.bfloat16)
+    w2 = (torch.randn((E, H, I), generator=g) * 0.05).to(torch.bfloat16)
+    m = mx.quantize_masters_mxfp4(w13, w2, DEV)
+    st = mx.WispMoEStateMxfp4(*m, 3, "paged", DEV, 0)
+    res = mx.WispMoEStateMxfp4(*m, E, "resident", DEV, 1)
+    res.prime_identity()
+    dev = [t.contiguous().to(DEV) for t in m]
+    for T in tokens:
+        x = torch.randn((T, H), generator=g).to(torch.bfloat16).to(DEV)
+        lg = torch.randn((T, E), generator=g).to(DEV)
+        got = st.forward(x, lg, K, True)
+        assert torch.equal(got, res.forward(x, lg, K, True)), T
+        assert torch.equal(got, mx.route_and_experts_mxfp4(x, lg, K, True, *dev)), T
+
+
 def test_slots_hold_the_masters_bytes(masters):
     st = mx.WispMoEStateMxfp4(*masters, 5, "paged", DEV, 0)
     for x, lg in _calls([1, 2, 9], 3):
