@@ -17,7 +17,6 @@
 #include <math.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "dma_pipeline.h"
 #include "experts_mxfp4.h"

@@ -10,6 +10,7 @@
 // Qwen3, one token 7.5 + 6.2; 12.5 (20 MB of weights, 4 us at the rate of a large
 // copy), 512 x 256 with 16 experts 3.9 + 4.0; 7.3.
 #include <algorithm>
+#include <type_traits>
 
 #include "experts_mxfp4.h"
 #include "mxfp4.h"
@@ -18,8 +19,6 @@
 namespace wisp {
 namespace {
 
-using mx::bf16x2;
-using mx::u32x2;
 using mx::u32x4;
 
 // Sum over each 8-lane half row, the same bits in every lane of it.
