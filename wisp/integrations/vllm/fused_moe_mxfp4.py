@@ -75,7 +75,8 @@ def quantize_mxfp4(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     codes = torch.empty((*w.shape[:-1], C // 2), dtype=torch.uint8, device=w.device)
     scales = torch.empty((*w.shape[:-1], C // BLOCK), dtype=torch.uint8, device=w.device)
     if w.numel():
-        check(lib().wisp_quant_mxfp4(w.data_ptr(), _DTYPES[w.dtype], w.numel() // C, C,
+        # (one run of blocks whatever the shape: a row's length may exceed the call's int)
+        check(lib().wisp_quant_mxfp4(w.data_ptr(), _DTYPES[w.dtype], w.numel() // BLOCK, BLOCK,
                                      codes.data_ptr(), scales.data_ptr(), _stream(w)),
               "quantize_mxfp4")
     return codes, scales
@@ -103,8 +104,9 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor,
     C = 2 * codes.shape[-1]
     out = torch.empty((*codes.shape[:-1], C), dtype=dtype, device=codes.device)
     if out.numel():
-        check(lib().wisp_dequant_mxfp4(codes.data_ptr(), scales.data_ptr(), out.numel() // C, C,
-                                       out.data_ptr(), _DTYPES[dtype], _stream(codes)),
+        check(lib().wisp_dequant_mxfp4(codes.data_ptr(), scales.data_ptr(),  # (as above)
+                                       out.numel() // BLOCK, BLOCK, out.data_ptr(),
+                                       _DTYPES[dtype], _stream(codes)),
               "dequantize_mxfp4")
     return out
 
