@@ -226,15 +226,19 @@ int wisp_quant_mxfp4(const void* x, int dtype, int64_t rows, int cols, uint8_t* 
 int wisp_dequant_mxfp4(const uint8_t* codes, const uint8_t* scales, int64_t rows, int cols,
                        void* out, int dtype, wisp_stream_t stream);
 
-/* wisp_moe_experts over MXFP4 weights: x, act and out are bfloat16; sums are
- * float32, act and out are rounded once.  W13 of slot s: codes at
+/* wisp_moe_experts over MXFP4 weights: x and out are bfloat16, sums are
+ * float32, out is rounded once.  Between the two products a pair's SwiGLU
+ * values are float32 in calls of few tokens (at most 12; which of them depends
+ * on T, K, H, I and nslots) and rounded to bfloat16 once in all others, so a
+ * token's bytes may differ between a small and a larger call.
+ * W13 of slot s: codes at
  * w13 + s*w13_stride ([2I, H/2]), scales at s13 + s*s13_stride ([2I, H/32]);
  * W2 [H, I/2] and s2 [H, I/32] likewise; strides in bytes.  H and I must be
  * multiples of 32, H*I below 2^31, weights and their strides 16-byte aligned,
  * scales and their strides 4-byte aligned.
- * A slot outside [0, nslots) contributes zero.  act: T*K*I elements; work:
- * device, 256-byte aligned, wisp_moe_mxfp4_work_bytes(T, K, H, I, nslots)
- * bytes. */
+ * A slot outside [0, nslots) contributes zero.  act: T*K*I bfloat16, scratch
+ * (a call of few tokens leaves it as it is); work: device, 256-byte aligned,
+ * wisp_moe_mxfp4_work_bytes(T, K, H, I, nslots) bytes. */
 int wisp_moe_experts_mxfp4(const void* x, int T, int H, int I, int K, const float* topk_w,
                            const int32_t* slots, int nslots, const void* w13, size_t w13_stride,
                            const void* s13, size_t s13_stride, const void* w2, size_t w2_stride,
@@ -372,7 +376,9 @@ typedef struct wisp_workspace {
                                     wisp_layer_sync_record)               */
   void* work;                    /* device, 256-byte aligned: MFMA path
                                     work buffer (wisp_moe_work_bytes with
-                                    nslots = cap)                         */
+                                    nslots = cap); MXFP4 layers, at every T:
+                                    wisp_moe_mxfp4_work_bytes with
+                                    nslots = num_experts                  */
   size_t work_bytes;
   size_t struct_bytes;           /* sizeof(wisp_workspace); another value
                                     is refused (WISP_ERR_INVALID)         */
@@ -413,7 +419,8 @@ int wisp_layer_set_scratch(void* handle, void* scratch_w13, void* scratch_w2, in
 
 /* One MoE layer call on `stream` for T tokens routed to top_k experts each:
  * route, page (paged mode) and compute.  Returns WISP_ERR_SUBBATCH when one
- * token alone needs more than cap experts.
+ * token alone needs more than cap experts.  MXFP4 layers take algo
+ * WISP_ALGO_AUTO only (else WISP_ERR_UNSUPPORTED).
  * Replaces: _patched_forward_cuda / _wisp_forward_cuda_paged
  *           (fused_moe.py:930-987, 990-1237). */
 int wisp_layer_forward(void* handle, const void* x, const void* logits, int logits_dtype,

@@ -1,6 +1,8 @@
 """MXFP4 operators at the ends of their ranges: rows and activations of more
 values than 32 bits count, the largest expert, many experts, and special
 values, missing slots and extreme scales in every kernel."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -9,6 +11,7 @@ from oracle import mxfp4 as O
 from oracle.moe import route
 from tests.test_gpu_mxfp4 import DEV, _close, _dev, _layer, _routing, _run, _weights, _x
 from wisp.integrations.vllm import fused_moe_mxfp4 as mx
+from wisp_amd import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -228,3 +231,61 @@ def test_largest_expert(T):
     assert np.abs(want[:, :4]).max() > 1
     err = np.abs(got[:, list(outs)].double().cpu().numpy() - want[:, :4])
     assert (err <= bound[:, :4]).all(), float((err / bound[:, :4]).max())
+
+
+# ---------------------------------------------------------------------------
+# Buffers as the C interface documents them
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("T,few", [(1, True), (12, True), (40, False)])
+def test_act_and_work_of_the_documented_sizes(T, few):
+    """Calls in buffers of exactly the documented bytes keep what stands behind
+    them, and act itself where act stays in float32."""
+    H, I, E, K = 96, 64, 5, 2
+    weights = _weights(E, H, I, 20)
+    dev = _dev(weights)
+    ids, w = _routing(T, E, K, 21)
+    x = _x(T, H, 22).to(DEV)
+    tw, ts = torch.from_numpy(w).to(DEV), torch.from_numpy(ids).to(DEV)
+    work_bytes = _lib.lib().wisp_moe_mxfp4_work_bytes(T, K, H, I, E)
+    act_bytes = T * K * I * 2
+    act = torch.full((act_bytes + 4096,), 7, dtype=torch.uint8, device=DEV)
+    work = torch.full((work_bytes + 4096,), 7, dtype=torch.uint8, device=DEV)
+    out = torch.full((T * H + 2048,), 7.0, dtype=torch.bfloat16, device=DEV)
+    w13, s13, w2, s2 = dev
+    _lib.check(_lib.lib().wisp_moe_experts_mxfp4(
+        x.data_ptr(), T, H, I, K, tw.data_ptr(), ts.data_ptr(), E, w13.data_ptr(), w13.stride(0),
+        s13.data_ptr(), s13.stride(0), w2.data_ptr(), w2.stride(0), s2.data_ptr(), s2.stride(0),
+        act.data_ptr(), out.data_ptr(), work.data_ptr(), work_bytes, _lib.stream_handle()), "call")
+    assert torch.equal(out[:T * H].view(T, H), _run(x, w, ids, dev))
+    assert (act[act_bytes:] == 7).all() and (work[work_bytes:] == 7).all()
+    assert (out[T * H:] == 7).all() and bool((act == 7).all()) == few
+
+
+@pytest.mark.parametrize("T", [1, 30])
+def test_a_layers_work_buffer_is_that_of_all_its_experts(T):
+    """wisp_layer_forward in a work buffer of wisp_moe_mxfp4_work_bytes with
+    nslots = num_experts; a call without one is refused before the pager's state
+    changes."""
+    H, I, E, K, cap = 128, 2304, 6, 2, 4
+    g = torch.Generator().manual_seed(23)
+    m = mx.quantize_masters_mxfp4((torch.randn((E, 2 * I, H), generator=g) * 0.05).bfloat16(),
+                                  (torch.randn((E, H, I), generator=g) * 0.05).bfloat16(), DEV)
+    st = mx.WispMoEStateMxfp4(*m, cap, "paged", DEV, 0)
+    x, lg = _x(T, H, 24).to(DEV), torch.randn((T, E), generator=g).to(DEV)
+    out = torch.empty_like(x)
+    ws = st._ws.ensure(T, K, cap)
+    need = _lib.lib().wisp_moe_mxfp4_work_bytes(T, K, H, I, E)
+    assert ws.work_bytes >= need
+
+    def call(nbytes):
+        ws.work_bytes = nbytes
+        return _lib.lib().wisp_layer_forward(st._handle, x.data_ptr(), lg.data_ptr(), _lib.WISP_F32,
+                                             T, K, 1, out.data_ptr(), C.byref(ws),
+                                             _lib.WISP_ALGO_AUTO, _lib.stream_handle())
+
+    assert call(0) == _lib.WISP_ERR_INVALID and st.expert_to_slot == {}
+    assert call(need) == _lib.WISP_OK
+    w13, w2, s13, s2 = (t.contiguous().to(DEV) for t in m)
+    assert torch.equal(out, mx.route_and_experts_mxfp4(x, lg, K, True, w13, w2, s13, s2))

@@ -10,9 +10,11 @@ Format.  A row's values in blocks of 32; each value a 4-bit E2M1 code (two to a
 byte, the earlier value in the low half), each block one E8M0 scale byte ``s``;
 a value is ``E2M1(code) * 2**(s - 127)``, ``s == 255`` is NaN.  Weights are
 ``uint8`` tensors: codes ``w13 [E, 2I, H/2]``, ``w2 [E, H, I/2]``, scales
-``s13 [E, 2I, H/32]``, ``s2 [E, H, I/32]``.  Activations are bfloat16; products
-are summed in float32; the SwiGLU result and the output are rounded to bfloat16
-once each.
+``s13 [E, 2I, H/32]``, ``s2 [E, H, I/32]``.  Activations are bfloat16, products
+are summed in float32 and the output is rounded to bfloat16 once.  The SwiGLU
+result stays in float32 in calls of few tokens (at most 12, by the whole call's
+tokens, shape and number of experts) and is rounded to bfloat16 once in all
+others, so a token's bytes may differ between a small and a larger call.
 
 ``WispMoEStateMxfp4`` is the paging state over such experts: masters in pinned
 host memory, one ``[w13 | w2 | s13 | s2]`` slab per expert, the same pager,
@@ -61,9 +63,9 @@ def _stream(t: torch.Tensor) -> int:
 def quantize_mxfp4(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``w [..., C]`` (float32 or bfloat16, C a multiple of 32) -> codes
     ``[..., C/2]`` and scales ``[..., C/32]``.  A block's scale is
-    ``2**(floor(log2(max|w|)) - 2)``; values are rounded to the nearest code
-    (ties to the even one) and saturate at 6 times the scale.  A block with an
-    infinity or a NaN reads back as NaNs."""
+    ``2**(floor(log2(max|w|)) - 2)``, no smaller than ``2**-127``; values are
+    rounded to the nearest code (ties to the even one) and saturate at 6 times
+    the scale.  A block with an infinity or a NaN reads back as NaNs."""
     if w.dtype not in _DTYPES:
         raise NotImplementedError(f"wisp.mxfp4: cannot quantise {w.dtype} (float32 and bfloat16)")
     if w.dim() < 1 or w.shape[-1] % BLOCK:
@@ -86,7 +88,8 @@ def quantize_mxfp4(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor,
                      dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of codes ``[..., C/2]`` and scales ``[..., C/32]`` as
-    ``[..., C]`` in ``dtype`` (bfloat16 or float32; both hold them exactly)."""
+    ``[..., C]`` in ``dtype`` (bfloat16 or float32; both hold them exactly, but
+    for magnitudes of ``2**128`` or more, which become infinities)."""
     if dtype not in _DTYPES:
         raise NotImplementedError(f"wisp.mxfp4: cannot read back as {dtype} "
                                   "(float32 and bfloat16)")

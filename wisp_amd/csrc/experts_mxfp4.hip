@@ -93,7 +93,11 @@ __device__ inline float silu_fast(float g) {
   return g * __builtin_amdgcn_rcpf(1.f + e);
 }
 
-// bf16(silu(g) * u) of four consecutive columns, one 8-byte store at p.
+// bf16(silu(g) * u) of four consecutive columns, one 8-byte store at p.  The
+// rounding is the matrix instruction's: its operands are bf16.  Against 64 bits
+// the output's error is 2.3e-3 of its norm with it and 1.7e-3 without (the
+// output's own rounding alone, as in the two launches for a few tokens, whose
+// act is float32).
 __device__ inline void store_act4(uint16_t* p, const f32x4& g, const f32x4& u) {
   uint32_t h[4];
 #pragma unroll
