@@ -9,11 +9,11 @@
 //
 // Small and middle calls (mx_grouped_kernel) are bound by the stream of weights,
 // large ones (mx_tile_kernel) by the matrix instructions and what feeds them.
-// Measured (us, w13 + w2): Qwen3, 32 tokens 37 + 24 (5.0 and 3.9 TB/s of
+// Measured (us, w13 + w2): Qwen3, 32 tokens 38 + 24 (4.9 and 3.9 TB/s of
 // weights; w2's rows are three stages, behind one that only loads), 512 tokens
-// 56 + 39; Mixtral, 6 tokens 75 + 50 (5.5 and 4.1); Qwen3, 8192 tokens 440 + 282
-// (940 and 730 TFLOP/s; w2 also writes 537 MB of y), Mixtral, 1000 tokens 565 +
-// 281 (830 and 840).
+// 57 + 40; Mixtral, 6 tokens 76 + 50 (5.4 and 4.1); Qwen3, 8192 tokens 452 + 284
+// (910 and 730 TFLOP/s; w2 also writes 537 MB of y), Mixtral, 1000 tokens 576 +
+// 285 (820 and 820).
 #include <math.h>
 
 #include <algorithm>
@@ -83,7 +83,9 @@ struct GroupedArgs {
 // g / (1 + e^-g), its last few float32 bits apart: act is rounded to bf16.
 // (The exponential's argument is clamped where e^-g is 0 or infinite anyway,
 // so that an infinite g gives what the formula does; what t's rounding left
-// enters as a factor near 1, which leaves an infinite power one.)
+// enters as a factor near 1, which leaves an infinite power one.)  Against
+// common.h's silu (us a call): Qwen3, 512 tokens 107 / 111, 8192 tokens 798 to
+// 804 / 810 to 825, Mixtral, 1000 tokens 824 to 828 / 834 to 839.
 __device__ inline float silu_fast(float g) {
   constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596299e-8f, kLn2 = 0.693147182f;
   const float n = __builtin_amdgcn_fmed3f(-g, -104.f, 89.f);
@@ -488,7 +490,9 @@ struct BigTile {
   // instead of computing (80 of 476 us at the Qwen3
   // 8192-token chunk's w13).
   // For the same reason nothing here is skipped for a tile that is not full:
-  // a branch's LDS reads are all waited for where it ends.
+  // a branch's LDS reads are all waited for where it ends.  (The compiler adds
+  // four small loops: it does not see that a code load's row offset, tile0 *
+  // rowb, is the wave's.)
   __device__ __attribute__((always_inline)) void step(unsigned char* __restrict__ wrs,
                                                       const unsigned char* __restrict__ rds, int c,
                                                       const Source& src, Weights& w, Operands& o,
@@ -631,7 +635,10 @@ hipError_t launch_grouped(const GroupedArgs& a, dim3 grid, hipStream_t st, hipEv
 // Calls of at least this many pairs a slot take the block tiles: from here the
 // blocks above pass over most slots' weights twice.  Measured, the blocks above
 // against tiles (us a call): Qwen3 177 / 212 at 72 pairs a slot, 211 / 213 at
-// 80; Mixtral 325 / 449 at 80, 408 / 452 at 90, 508 / 457 at 100.
+// 80; Mixtral 325 / 449 at 80, 508 / 457 at 100.  84 is where Qwen3's times meet;
+// Mixtral's meet at about 95, and below it takes longer than in the blocks: 317 /
+// 411 to 446 at 84, 361 / 444 at 87, 397 / 461 at 90, 438 / 445 at 93.  (Pairs
+// without a slot count: the slots are in device memory.)
 constexpr int kTilePairs = 84;
 
 // The pairs of a call's slots: their mean, the deviation that a random router
@@ -758,9 +765,11 @@ __global__ __launch_bounds__(256) void mx_combine_kernel(const float* __restrict
 
 // Splits of w2's k range: a call whose panels are too few to fill the GPU (16
 // of 256 rows at H 4096), and whose block tiles would be, splits it into parts
-// of at least four stages, none of them empty (25 stages in six parts of five
-// would leave one).  It goes by the whole call alone, for the bytes depend on
-// it.  Measured, 1 / 4 splits, Mixtral, 6 tokens: w2 100 / 49 us.
+// of at least four stages but for the last, which is not empty (25 stages in six
+// parts of five would leave one).  It goes by the whole call alone, for the
+// bytes depend on it.  Measured, 1 / 4 splits, Mixtral: w2 at 6 tokens 100 / 49
+// us; a call, where unsplit is block tiles, at 336 tokens 540 / 446, 400 544 /
+// 446, 512 559 / 503, 640 604 / 560, 700 615 / 584 to 615, 768 727 / 752.
 int w2_splits(int T, int K, int H, int I, int nslots) {
   const int panels = (H + 255) / 256;
   const double mean = (double)T * K / nslots;
