@@ -230,7 +230,8 @@ int wisp_dequant_mxfp4(const uint8_t* codes, const uint8_t* scales, int64_t rows
  * float32, out is rounded once.  Between the two products a pair's SwiGLU
  * values are float32 in calls of few tokens (at most 12; which of them depends
  * on T, K, H, I and nslots) and rounded to bfloat16 once in all others, so a
- * token's bytes may differ between a small and a larger call.
+ * token's bytes may differ between a small and a larger call.  Weights count as
+ * wisp_dequant_mxfp4 reads them back: 2^128 and more is infinite.
  * W13 of slot s: codes at
  * w13 + s*w13_stride ([2I, H/2]), scales at s13 + s*s13_stride ([2I, H/32]);
  * W2 [H, I/2] and s2 [H, I/32] likewise; strides in bytes.  H and I must be

@@ -289,3 +289,21 @@ def test_a_layers_work_buffer_is_that_of_all_its_experts(T):
     assert call(need) == _lib.WISP_OK
     w13, w2, s13, s2 = (t.contiguous().to(DEV) for t in m)
     assert torch.equal(out, mx.route_and_experts_mxfp4(x, lg, K, True, w13, w2, s13, s2))
+
+
+@pytest.mark.parametrize("T", [1, 40, 400])
+def test_weights_past_float32_are_infinite(T):
+    """Codes of the highest scales whose value is 2^128 or more, on one expert
+    and row: infinite there as they read back, whatever the activation."""
+    H, I, E = 128, 128, 2
+    dev = _dev(_weights(E, H, I, 25))
+    dev[0][1, 5, :16], dev[1][1, 5, 0] = 0x11, 254  # 2^126: finite
+    ids, w = _routing(T, E, 1, 26)
+    ids[0], x = 1, (_x(T, H, 27).double() * 2.0 ** -100).to(torch.bfloat16)
+    assert torch.isfinite(mx.dequantize_mxfp4(dev[0], dev[1], torch.float32)).all()
+    assert torch.isfinite(_run(x, w, ids, dev)).all()
+    dev[0][1, 5, 3] = 0x74  # 2 * 2^127 and 6 * 2^127
+    assert torch.isinf(mx.dequantize_mxfp4(dev[0], dev[1], torch.float32)).sum() == 2
+    got = _run(x, w, ids, dev)
+    hit = torch.from_numpy((ids == 1).any(axis=1)).to(DEV)
+    assert torch.isfinite(got[~hit]).all() and not torch.isfinite(got[hit]).all(dim=1).any()
