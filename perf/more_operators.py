@@ -56,13 +56,12 @@ def listed():
     return [
         # bs=1 generation: the norm in front of a bf16 layer.
         _norm("norm-decode-1", "norm", 1, 2048),
-        # An odd float32 one, the first norm of a model (no residual yet).
-        _norm("norm-odd-f32", "norm", 333, 1376, "f32", False),
-        # Batched generation in front of FP8 experts, and a large prompt chunk.
-        _norm("norm8-decode-32", "norm8", 32, 2048),
+        # In front of FP8 experts: odd sizes in float32, the first norm of a
+        # model (no residual yet); a large prompt chunk.
+        _norm("norm8-odd-f32", "norm8", 333, 1375, "f32", False),
         _norm("norm8-prompt-8192", "norm8", 8192, 4096),
-        # The SwiGLU between the products: batched generation, a large chunk.
-        _silu("silu8-qwen3-256", 256, 768),
+        # The SwiGLU between the products: odd sizes, a large chunk.
+        _silu("silu8-odd-231", 231, 352),
         _silu("silu8-qwen3-65536", 65536, 768),
         # bs=1 generation: eight experts of one row each.
         _grouped("mm-qwen3-w13-1", "mm", "qwen3", "w13", 1),
@@ -71,10 +70,13 @@ def listed():
         _grouped("mm-qwen3-w2-rank-777", "mm", "qwen3", "w2", 777, 8, 0.5),
         # A large prompt chunk in bfloat16.
         _grouped("mm-qwen3-w13-8192", "mm", "qwen3", "w13", 8192),
-        # In FP8: batched generation, odd sizes with a float32 output, a chunk
-        # through few large experts.
+        # Odd sizes with a float32 output, as a caller that sums many experts'
+        # outputs itself takes it.
+        _grouped("mm-odd-w2-77-f32", "mm", "odd", "w2", 77, 1, 0.5, "f32"),
+        # In FP8 (bf16 out): batched generation, odd sizes, a chunk through few
+        # large experts.
         _grouped("mm8-qwen3-w13-32", "mm8", "qwen3", "w13", 32),
-        _grouped("mm8-odd-w2-77-f32", "mm8", "odd", "w2", 77, 1, 0.5, "f32"),
+        _grouped("mm8-odd-w13-77", "mm8", "odd", "w13", 77, 1, 0.5),
         _grouped("mm8-mixtral-w13-2000", "mm8", "mixtral", "w13", 2000),
     ]
 
@@ -100,7 +102,7 @@ def draw(rng):
         ranks = rng.choice([1, 1, 2, 8]) if layer != "mixtral" else rng.choice([1, 2])
         c = _grouped("", op, layer, rng.choice(["w13", "w2"]), _log_int(rng, 1, most), ranks,
                      round(rng.choice([0.0, rng.uniform(0.0, 0.7)]), 2),
-                     rng.choice(["bf16", "bf16", "f32"]))
+                     rng.choice(["bf16", "bf16", "f32"]) if op == "mm" else "bf16")
     del c["name"]
     return c
 
@@ -256,7 +258,7 @@ def run(state):
             return rows.silu_mul_fp8(state["h"])
         if op == "mm":
             return gm.grouped_mm(*state["in"], state["ends"], dtype=state["dtype"])
-        return gm.grouped_mm_fp8(*state["in"], state["ends"], dtype=state["dtype"])
+        return gm.grouped_mm_fp8(*state["in"], state["ends"])
     if op in ("norm", "norm8"):
         y, r = _rms(state["x"], state["residual"], state["w"])
         return (y.to(state["x"].dtype), r) if op == "norm" else (*_quantize_rows(y), r)
