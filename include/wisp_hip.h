@@ -261,6 +261,60 @@ int wisp_moe_layer_mxfp4(const void* x, const void* logits, int logits_dtype, in
  * in T. */
 size_t wisp_moe_mxfp4_work_bytes(int T, int K, int H, int I, int nslots);
 
+/* Rows in 8 bits: float8_e4m3fn codes and one float32 scale per row and group
+ * of 128 columns ([rows, ceil(cols / 128)]; a row's last group may be
+ * shorter): s = max(max|y|, 1e-10) / 448, q = e4m3fn(y / s), nearest, from
+ * the float32 y.  A group that holds an infinity or a NaN gets NaN codes.
+ *
+ * RMS norm of rows x [rows, cols] (WISP_F32 or WISP_BF16) with the residual's
+ * addition: r = round(x + residual) to the residual's type, written to
+ * residual_out (residual NULL: r = x, nothing written);
+ * y = r * (mean(r^2) + eps)^(-1/2) * weight in float32; out (or NULL)
+ * [rows, cols] contiguous, y rounded to x's type; q [rows, cols] and scales
+ * (or NULL) y in 8 bits.  weight and residual are of x's type or WISP_F32;
+ * strides are the elements between rows, each row contiguous; cols up to
+ * 32768.  out and residual_out may each be x or residual itself (same rows),
+ * not each other.  No reference counterpart (vLLM's own norm precedes the MoE
+ * layer). */
+int wisp_add_rms_norm(const void* x, int dtype, int64_t rows, int cols, int64_t x_stride,
+                      const void* residual, int residual_dtype, int64_t residual_stride,
+                      void* residual_out, int64_t residual_out_stride, const void* weight,
+                      int weight_dtype, float eps, void* out, uint8_t* q, float* scales,
+                      wisp_stream_t stream);
+
+/* SwiGLU of rows h [rows, 2 * inter] (gate, then up; WISP_F32 or WISP_BF16,
+ * h_stride elements apart) in 8 bits, as above: q [rows, inter], scales
+ * [rows, ceil(inter / 128)] of silu(gate) * up, computed in float32.  No
+ * reference counterpart. */
+int wisp_silu_mul_fp8(const void* h, int dtype, int64_t rows, int inter, int64_t h_stride,
+                      uint8_t* q, float* scales, wisp_stream_t stream);
+
+/* Products grouped by expert over rows sorted by expert:
+ * out[i] = W[e] x[i] for the rows i in [ends[e - 1], ends[e]), group 0 from
+ * row 0.  ends: device int32 [E]; an end outside [0, M] counts as 0 or M, one
+ * below an earlier end as that one.  Rows behind the last group: left alone,
+ * or zeroed with zero_tail.  x [M, K] bfloat16, rows x_ld elements apart; W of
+ * expert e at w + e*w_stride, [N, K] bfloat16, rows w_ld elements apart; out
+ * [M, N] contiguous, WISP_BF16 or WISP_F32: float32 sums, rounded once.
+ * E <= 512, K a multiple of 8, x, w and their strides 16-byte aligned, an
+ * expert's weights below 2 GiB, rows of x less than 4 MiB apart.  No reference
+ * counterpart (its experts run over one GPU's pairs). */
+int wisp_grouped_mm(const void* x, int64_t x_ld, const void* w, int64_t w_stride, int64_t w_ld,
+                    const int32_t* ends, int E, int M, int N, int K, void* out, int out_dtype,
+                    int zero_tail, wisp_stream_t stream);
+
+/* The same over block FP8, out bfloat16: q [M, K] e4m3fn codes q_ld apart with
+ * scales s [M, ceil(K / 128)] s_ld apart; w e4m3fn codes (strides in elements)
+ * with block scales ws, expert e at + e*ws_stride, [ceil(N / 128),
+ * ceil(K / 128)] contiguous.  Per 128 columns
+ * acc += dot(q, w) * (s * ws) in float32; the dot is the fp8 matrix
+ * instruction's, off by up to some 2^-16 of the sum of its products' sizes on
+ * ordinary rows.  K a multiple of 16; otherwise as above. */
+int wisp_grouped_mm_fp8(const uint8_t* q, int64_t q_ld, const float* s, int64_t s_ld,
+                        const uint8_t* w, int64_t w_stride, int64_t w_ld, const float* ws,
+                        int64_t ws_stride, const int32_t* ends, int E, int M, int N, int K,
+                        void* out, int zero_tail, wisp_stream_t stream);
+
 /* Bytes of the device array wisp_moe_experts_noalloc works in, per GPU, in
  * a default build; building with WISP_NOALLOC_SCRATCH_MIB=n sets n MiB, and
  * wisp_noalloc_scratch_bytes() returns the size the library was built with.

@@ -1,0 +1,394 @@
+"""Grouped products on the GPU against the float64 oracle: within what a
+float32 sum and one rounding allow (derived in ``oracle.rows.grouped_mm``), at
+sizes, groups, strides and values where they can go wrong."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import rows as O
+from wisp.integrations.vllm import grouped_mm as G
+from wisp.integrations.vllm import rows_fp8 as R
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+BF, F32, FP8 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
+
+# The fp8 matrix instruction aligns the products of a block of 128 to its largest
+# one before it sums them and keeps at least 12 bits behind the point there:
+# measured, up to 1.7e-4 of the sum of the products' sizes on codes of the full
+# range, 1.3e-5 on quantised normal values.
+DOT8 = 2.0 ** -12
+
+
+def _f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def _bits(t):
+    return t.contiguous().view(torch.int16 if t.element_size() == 2 else torch.int32)
+
+
+def _randn(shape, seed, dtype=BF, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype).to(DEV)
+
+
+def _ends(counts):
+    return torch.tensor(np.cumsum(counts), dtype=torch.int32, device=DEV)
+
+
+def _near(got, want, bound, dtype):
+    half = O.BF16 if dtype == BF else O.STEP
+    bound = bound + half * (np.abs(want) + bound) + O.TINY
+    d = np.abs(_f64(got) - want)
+    assert got.dtype == dtype
+    assert np.all(d <= bound), float((d / bound).max())
+
+
+def _fp8(v):
+    """Codes of any values (to the nearest), by torch's cast."""
+    return v.clamp(-448, 448).to(FP8)
+
+
+def _case8(M, E, N, K, seed):
+    """Rows and weights in FP8 as they are made, scales of unequal size."""
+    q = _fp8(_randn((M, K), seed, F32, 100.0))
+    w = _fp8(_randn((E, N, K), seed + 1, F32, 100.0))
+    g, b = -(-K // 128), -(-N // 128)
+    s = torch.exp(_randn((M, g), seed + 2, F32)) * 0.01
+    ws = torch.exp(_randn((E, b, g), seed + 3, F32)) * 0.001
+    return q, s, w, ws
+
+
+def _values8(q, s, w, ws):
+    K, N = q.shape[1], w.shape[1]
+    x = _f64(q.float()) * np.repeat(_f64(s), 128, axis=1)[:, :K]
+    return x, _f64(w.float()) * O.spread(_f64(ws), N, K)
+
+
+def _check(M, E, N, K, counts, seed=0, dtype=BF):
+    x, w = _randn((M, K), seed), _randn((E, N, K), seed + 1, BF, 0.1)
+    ends = _ends(counts)
+    got = G.grouped_mm(x, w, ends, dtype=dtype)
+    _near(got, *O.grouped_mm(_f64(x), _f64(w), ends.tolist()), dtype)
+    return got
+
+
+def _check8(M, E, N, K, counts, seed=0):
+    case = _case8(M, E, N, K, seed)
+    ends = _ends(counts)
+    got = G.grouped_mm_fp8(*case, ends)
+    _near(got, *O.grouped_mm(*_values8(*case), ends.tolist(), DOT8), BF)
+    return got
+
+
+def _spread_counts(M, E, seed):
+    """Ragged counts with empty groups."""
+    r = np.random.RandomState(seed)
+    p = r.exponential(size=E) * (r.rand(E) < 0.7)
+    p = p if p.sum() else np.ones(E)
+    return r.multinomial(M, p / p.sum())
+
+
+# rows, experts, outputs, columns
+SIZES = [(1, 1, 1, 16), (1, 4, 8, 16), (5, 3, 17, 32), (16, 2, 64, 64), (17, 1, 100, 80),
+         (33, 5, 256, 128), (64, 1, 257, 144), (65, 2, 130, 272), (100, 7, 300, 352),
+         (231, 24, 704, 1056), (130, 1, 512, 256), (300, 2, 264, 512), (515, 3, 128, 176),
+         (1000, 4, 192, 1040), (600, 1, 320, 2048), (9, 130, 48, 64), (1100, 300, 40, 48)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("M,E,N,K", SIZES)
+def test_bf16_sizes(M, E, N, K, dtype):
+    _check(M, E, N, K, _spread_counts(M, E, M + N), M + K, dtype)
+
+
+@pytest.mark.parametrize("M,E,N,K", SIZES)
+def test_fp8_sizes(M, E, N, K):
+    _check8(M, E, N, K, _spread_counts(M, E, M + N), M + K)
+
+
+@pytest.mark.parametrize("K", [8, 24, 56, 72, 120, 136, 184, 200, 1000])
+def test_bf16_columns(K):
+    _check(40, 3, 70, K, [13, 0, 27], K)
+
+
+@pytest.mark.parametrize("K", [16, 48, 112, 128, 144, 240, 256, 272, 400, 1008])
+def test_fp8_columns(K):
+    _check8(40, 3, 150, K, [13, 0, 27], K)
+
+
+COUNTS = [[0, 0, 0], [0, 0, 1], [1, 0, 0], [64, 64, 64], [63, 65, 1], [128, 0, 129], [300, 1, 15],
+          [16, 17, 256], [257, 255, 3], [0, 700, 0], [1, 1, 1]]
+
+
+@pytest.mark.parametrize("counts", COUNTS)
+@pytest.mark.parametrize("tail", [0, 1, 37])
+def test_groups(counts, tail):
+    """Groups around the tiles' sizes, empty ones, and rows behind the last."""
+    M = sum(counts) + tail
+    if M:
+        _check(M, 3, 72, 96, counts, M)
+        _check8(M, 3, 72, 96, counts, M)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("rows", [1, 2, 8, 15, 16, 17, 40, 64, 70, 128, 140, 256, 300])
+def test_rows_do_not_depend_on_their_group_s_size(rows, fp8):
+    """A group's rows and the same rows one by one agree within the bound."""
+    if fp8:
+        _check8(rows, 1, 96, 256, [rows], rows)
+    else:
+        _check(rows, 1, 96, 256, [rows], rows)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_ends_that_descend_or_lie_outside(fp8):
+    M, E, N, K = 90, 6, 40, 64
+    for ends in ([10, 5, 30, 200, 100, 95], [-3, -1, 50, 20, 60, 60], [0, 0, 0, 0, 0, 0],
+                 [2 ** 31 - 1] * 6, [-2 ** 31] * 6, [90, 0, 0, 0, 0, 0]):
+        e = torch.tensor(ends, dtype=torch.int32, device=DEV)
+        if fp8:
+            case = _case8(M, E, N, K, 3)
+            _near(G.grouped_mm_fp8(*case, e), *O.grouped_mm(*_values8(*case), ends, DOT8), BF)
+        else:
+            x, w = _randn((M, K), 1), _randn((E, N, K), 2)
+            _near(G.grouped_mm(x, w, e), *O.grouped_mm(_f64(x), _f64(w), ends), BF)
+
+
+@pytest.mark.parametrize("N", [64, 41])
+def test_rows_behind_the_last_group(N):
+    """Left as they are in a given output, zero in a new one."""
+    x, w = _randn((200, 64), 4), _randn((3, N, 64), 5)
+    for counts in ([20, 0, 33], [0, 0, 0], [100, 50, 50], [100, 50, 49]):
+        n, ends = sum(counts), _ends(counts)
+        for dtype in (BF, F32):
+            new = G.grouped_mm(x, w, ends, dtype=dtype)
+            assert not new[n:].any() and not torch.isnan(new).any()
+            out = torch.full((200, N), float("nan"), dtype=dtype, device=DEV)
+            assert G.grouped_mm(x, w, ends, dtype=dtype, out=out) is out
+            assert torch.equal(out[:n], new[:n]) and out[n:].isnan().all()
+    case = _case8(200, 3, N, 64, 6)
+    out = torch.full((200, N), float("nan"), dtype=BF, device=DEV)
+    G.grouped_mm_fp8(*case, ends, out=out)
+    new = G.grouped_mm_fp8(*case, ends)
+    assert torch.equal(out[:199], new[:199]) and out[199].isnan().all() and not new[199].any()
+
+
+def test_values_stay_in_their_rows_and_columns():
+    """Infinities and NaNs in rows of another group, behind the last group, in
+    another expert's weights, in the columns behind a row's end and in rows
+    between the ones in use touch nothing else."""
+    M, E, N, K = 70, 3, 80, 72
+    big_x = torch.full((M, 128), float("nan"), dtype=BF, device=DEV)
+    big_w = torch.full((E, N + 5, 96), float("nan"), dtype=BF, device=DEV)
+    x, w = _randn((M, K), 7), _randn((E, N, K), 8)
+    big_x[:, :K], big_w[:, :N, :K] = x, w
+    ends = _ends([30, 0, 21])
+    want = G.grouped_mm(x, w, ends)
+    big_x[51:] = float("nan")
+    big_w[1] = float("inf")
+    assert torch.equal(G.grouped_mm(big_x[:, :K], big_w[:, :N, :K], ends), want)
+    big_x[33, 9], big_w[0, 4, 11] = float("inf"), float("nan")
+    got = G.grouped_mm(big_x[:, :K], big_w[:, :N, :K], ends)
+    bad = torch.zeros((M, N), dtype=torch.bool, device=DEV)
+    bad[33] = True
+    bad[:30, 4] = True
+    assert torch.equal(got[~bad], want[~bad]) and not torch.isfinite(got[bad]).any()
+
+
+def test_fp8_values_stay_in_their_rows_and_columns():
+    M, E, N, K = 70, 3, 150, 144
+    q, s, w, ws = _case8(M, E, N, K, 9)
+    big_q = torch.full((M, 256), 0x7f, dtype=torch.uint8, device=DEV).view(FP8)
+    big_w = torch.full((E, N + 3, 192), 0x7f, dtype=torch.uint8, device=DEV).view(FP8)
+    big_s = torch.full((M, 5), float("nan"), device=DEV)
+    big_q.view(torch.uint8)[:, :K], big_w.view(torch.uint8)[:, :N, :K] = \
+        q.view(torch.uint8), w.view(torch.uint8)
+    big_s[:, :2] = s
+    ends = _ends([30, 0, 21])
+    want = G.grouped_mm_fp8(q, s, w, ws, ends)
+    big_q.view(torch.uint8)[51:] = 0x7f
+    big_s[51:] = float("inf")
+    big_w.view(torch.uint8)[1] = 0x7f
+    ws = ws.clone()
+    ws[1] = float("nan")
+    got = G.grouped_mm_fp8(big_q[:, :K], big_s[:, :2], big_w[:, :N, :K], ws, ends)
+    assert torch.equal(got, want)
+    big_s[33, 1] = float("inf")
+    ws[0, 1, 0] = float("nan")
+    got = G.grouped_mm_fp8(big_q[:, :K], big_s[:, :2], big_w[:, :N, :K], ws, ends)
+    bad = torch.zeros((M, N), dtype=torch.bool, device=DEV)
+    bad[33] = True
+    bad[:30, 128:] = True
+    assert torch.equal(got[~bad], want[~bad]) and not torch.isfinite(got[bad]).any()
+
+
+@pytest.mark.parametrize("M", [30, 400])
+def test_strides(M):
+    """Rows and experts any distance apart, unaligned and transposed rows."""
+    E, N, K = 3, 56, 136
+    base, wide = _randn((M, 400), 10), _randn((E, N, 160), 11)
+    ends = _ends([M // 3, M // 3, M // 4])
+    w = wide[:, :, :K]
+    want = G.grouped_mm(base[:, 40:40 + K].contiguous(), w.contiguous(), ends)
+    assert torch.equal(G.grouped_mm(base[:, 40:40 + K], w, ends), want)
+    slab = torch.empty(E, N * K + 24, dtype=BF, device=DEV)
+    apart = slab[:, 8:8 + N * K].view(E, N, K)
+    apart.copy_(w)
+    assert torch.equal(G.grouped_mm(base[:, 40:40 + K], apart, ends), want)
+    off = G.grouped_mm(base[:, 41:41 + K], w, ends)   # unaligned rows are copied
+    assert torch.equal(off, G.grouped_mm(base[:, 41:41 + K].contiguous(), w, ends))
+    t = base[:, :K].t().contiguous().t()
+    assert torch.equal(G.grouped_mm(t, w, ends), G.grouped_mm(base[:, :K].contiguous(), w, ends))
+    one = G.grouped_mm(base[:, :K], w[:1].expand(E, N, K), ends)   # experts that share weights
+    assert torch.equal(one, G.grouped_mm(base[:, :K], w[:1].repeat(E, 1, 1), ends))
+    K = 144
+    q, s, w8, ws = _case8(M, E, N, K, 12)
+    want = G.grouped_mm_fp8(q, s, w8, ws, ends)
+    sw = torch.empty((M, 9), device=DEV)[:, 3:5].copy_(s)
+    slab = torch.zeros((E, 4 * N * K), dtype=torch.uint8, device=DEV)
+    apart = slab[:, 16:16 + N * K].view(E, N, K)
+    apart.copy_(w8.view(torch.uint8))
+    assert torch.equal(G.grouped_mm_fp8(q, sw, apart.view(FP8), ws, ends), want)
+    assert torch.equal(G.grouped_mm_fp8(q, s.t().contiguous().t(), w8, ws, ends), want)
+
+
+def test_expert_weights_beyond_32_bits():
+    """An expert's place past 2^32 bytes."""
+    E, N, K = 5, 16384, 32768
+    w = torch.zeros((E, N, K), dtype=BF, device=DEV)
+    w[4, -300:] = _randn((300, K), 13, BF, 0.05)
+    x = _randn((20, K), 14)
+    got = G.grouped_mm(x, w, _ends([3, 0, 2, 0, 15]), dtype=F32)
+    assert not got[:5].any() and not got[:, :-300].any()
+    want, bound = O.grouped_mm(_f64(x[5:]), _f64(w[4:, -300:]), [15])
+    _near(got[5:, -300:], want, bound, F32)
+
+
+def test_rows_beyond_32_bits():
+    """Rows and outputs past 2^32 bytes."""
+    M, N, K = 140000, 16384, 16384
+    x = torch.zeros((M, K), dtype=BF, device=DEV)
+    x[-70:] = _randn((70, K), 15)
+    w = _randn((2, 64, K), 16, BF, 0.05)
+    full = torch.zeros((2, N, K), dtype=BF, device=DEV)
+    full[:, -64:] = w
+    got = G.grouped_mm(x, full, _ends([M - 40, 40]))
+    want, bound = O.grouped_mm(_f64(x[-70:]), _f64(w), [30, 70])
+    _near(got[-70:, -64:], want, bound, BF)
+    assert not got[-70:, :-64].any() and not got[M - 2000:M - 70].any() and not got[:300].any()
+
+
+@pytest.mark.parametrize("M", [12, 200, 900])
+def test_runs_together(M):
+    """The operators as a rank uses them, against the oracle's own chain from
+    the codes each of them made."""
+    E, H, I = 4, 256, 160
+    x, res = _randn((M, H), 20), _randn((M, H), 21, BF, 3.0)
+    weight = (1 + 0.1 * _randn((H,), 22, F32)).to(BF)
+    w13, w2 = (torch.empty(s, dtype=FP8, device=DEV) for s in ((E, 2 * I, H), (E, H, I)))
+    s13 = torch.empty((E, 3, 2), device=DEV)
+    s2 = torch.empty((E, 2, 2), device=DEV)
+    for w, s, seed in ((w13, s13, 23), (w2, s2, 24)):
+        w.copy_(_fp8(_randn(w.shape, seed, F32, 100.0)))
+        s.copy_(torch.exp(0.3 * _randn(s.shape, seed + 5, F32)) * 2e-4)
+    ends = _ends(_spread_counts(M, E, M))
+    n = int(ends[-1])
+    q, s, r = R.add_rms_norm_fp8(x, weight, 1e-6, res)
+    h = G.grouped_mm_fp8(q, s, w13, s13, ends)
+    _near(h, *O.grouped_mm(*_values8(q, s, w13, s13), ends.tolist(), DOT8), BF)
+    a, sa = R.silu_mul_fp8(h)
+    y = G.grouped_mm_fp8(a, sa, w2, s2, ends)
+    _near(y, *O.grouped_mm(*_values8(a, sa, w2, s2), ends.tolist(), DOT8), BF)
+    # the whole chain without any rounding: three times eight bits
+    v = O.rms_norm(_f64((x.double() + res.double()).to(BF)), _f64(weight), 1e-6)
+    f13 = _f64(w13.float()) * O.spread(_f64(s13), 2 * I, H)
+    f2 = _f64(w2.float()) * O.spread(_f64(s2), H, I)
+    want, _ = O.grouped_mm(O.silu_mul(O.grouped_mm(v, f13, ends.tolist())[0])[0], f2,
+                           ends.tolist())
+    off = np.linalg.norm(_f64(y)[:n] - want[:n]) / np.linalg.norm(want[:n])
+    # a code is off by at most 2^-4 of its value, each product averages over its
+    # 160 or 256 columns: the rows' errors add as squares, 2^-4 per quantisation
+    # at the very most (relative to the norm), twice for gate and up
+    assert off <= 4 * 2.0 ** -4
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_in_a_graph_and_on_streams(fp8):
+    """Captured and replayed with other ends, rows and weights in the same
+    buffers, beside eager calls and a second graph; on a side stream."""
+    M, E, N, K = 300, 5, 200, 272
+    ins = _case8(M, E, N, K, 30) if fp8 else (_randn((M, K), 31), _randn((E, N, K), 32))
+    call = G.grouped_mm_fp8 if fp8 else G.grouped_mm
+    sets = [_ends(_spread_counts(M - k, E, k)) for k in range(4)]
+    ends = sets[0].clone()
+    call(*ins, ends)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(*ins, ends))
+        graphs.append(g)
+    for e in sets:
+        ends.copy_(e)
+        want = call(*ins, e)
+        for g, out in zip(graphs, outs):
+            out.fill_(7)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a = call(*ins, sets[1])
+    b = call(*ins, sets[2])
+    side.synchronize()
+    assert torch.equal(a, call(*ins, sets[1])) and torch.equal(b, call(*ins, sets[2]))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_the_same_bytes_again(fp8):
+    M, E, N, K = 700, 6, 320, 400
+    ins = _case8(M, E, N, K, 40) if fp8 else (_randn((M, K), 41), _randn((E, N, K), 42))
+    call = G.grouped_mm_fp8 if fp8 else G.grouped_mm
+    ends = _ends(_spread_counts(M, E, 43))
+    first = call(*ins, ends)
+    for _ in range(3):
+        assert torch.equal(_bits(call(*ins, ends)), _bits(first))
+
+
+def test_empty():
+    w = _randn((2, 16, 32), 50)
+    out = G.grouped_mm(torch.empty((0, 32), dtype=BF, device=DEV), w, _ends([0, 0]))
+    assert out.shape == (0, 16)
+    out = G.grouped_mm(_randn((4, 32), 51), w[:, :0], _ends([2, 2]))
+    assert out.shape == (4, 0)
+
+
+def test_refusals():
+    x, w, ends = _randn((6, 64), 60), _randn((2, 16, 64), 61), _ends([3, 3])
+    q, s, w8, ws = _case8(6, 2, 16, 64, 62)
+    for bad in (lambda: G.grouped_mm(x[0], w, ends), lambda: G.grouped_mm(x, w[0], ends),
+                lambda: G.grouped_mm(x, w, ends[:1]), lambda: G.grouped_mm(x, w, ends.long()),
+                lambda: G.grouped_mm(x[:, :32], w, ends), lambda: G.grouped_mm(x, w.cpu(), ends),
+                lambda: G.grouped_mm(x, w, ends.cpu()), lambda: G.grouped_mm(x, w[:0], ends[:0]),
+                lambda: G.grouped_mm(x, w.transpose(1, 2).contiguous().transpose(1, 2), ends),
+                lambda: G.grouped_mm(x, w, ends, out=torch.empty((6, 17), dtype=BF, device=DEV)),
+                lambda: G.grouped_mm(x, w, ends, dtype=F32, out=x[:, :16].contiguous()),
+                lambda: G.grouped_mm(x, w, ends, out=x.view(-1)[:96].view(6, 16)),
+                lambda: G.grouped_mm_fp8(q, s[:5], w8, ws, ends),
+                lambda: G.grouped_mm_fp8(q, s, w8, ws[:, :, :0], ends),
+                lambda: G.grouped_mm_fp8(q, s.double(), w8, ws, ends),
+                lambda: G.grouped_mm_fp8(q, s.cpu(), w8, ws, ends),
+                lambda: G.grouped_mm_fp8(q, s, w8, ws, ends, out=torch.empty((6, 16), device=DEV))):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: G.grouped_mm(x.float(), w, ends), lambda: G.grouped_mm(x, w.float(), ends),
+                lambda: G.grouped_mm(x, w, ends, dtype=torch.float16),
+                lambda: G.grouped_mm_fp8(x, s, w8, ws, ends),
+                lambda: G.grouped_mm_fp8(q[:, :24], s, w8[:, :, :24], ws, ends),
+                lambda: G.grouped_mm(x[:, :4], w[:, :, :4], ends)):
+        with pytest.raises(NotImplementedError):
+            bad()

@@ -1,0 +1,128 @@
+"""Matrix products grouped by expert, over rows that are sorted by expert.
+
+An expert-parallel rank gets its tokens' rows from an all-to-all in the order of
+its experts, as many of each as the routing made, in a buffer that may hold
+more.  The reference runs whole experts over (token, expert) pairs of one GPU
+only; these products are the parts of such a rank's experts::
+
+    q, s, residual = add_rms_norm_fp8(x, weight, eps, residual)
+    ...                                            # rows to the owners of their experts
+    h = grouped_mm_fp8(q, s, w13, s13, ends)       # [rows, 2 * I]
+    a, sa = silu_mul_fp8(h)
+    y = grouped_mm_fp8(a, sa, w2, s2, ends)        # [rows, H]
+
+``ends [E]`` (int32, on the device, never read by the host): group ``e`` is the
+rows ``[ends[e - 1], ends[e])``, from 0 for the first.  An end outside ``[0,
+rows]`` counts as 0 or ``rows``, one below an earlier end as that one, so groups
+never overlap.  Rows behind the last group are left as they are in a given
+``out`` and are zero in a new one.  Up to 512 experts; weights are ``[E, N, K]``
+(``w13``, ``w2`` as the MoE layers hold them), each row contiguous; an expert's
+are less than 2 GiB.
+"""
+from __future__ import annotations
+
+import torch
+
+from wisp_amd import _lib
+from wisp_amd._lib import check, lib
+from .fused_moe import _require_device
+from .rows_fp8 import FP8, GROUP, _DTYPES, _check_apart, _on_device, _stream
+
+
+def _sizes(x, w, ends) -> tuple[int, int, int, int]:
+    """``(M, E, N, K)`` of rows, weights and ends."""
+    if x.dim() != 2 or w.dim() != 3 or ends.dim() != 1 or w.shape[2] != x.shape[1] or \
+            ends.shape[0] != w.shape[0] or not w.shape[0]:
+        raise ValueError("wisp: grouped products take rows [M, K], weights [E, N, K] and ends "
+                         f"[E], got {tuple(x.shape)}, {tuple(w.shape)}, {tuple(ends.shape)}")
+    if ends.dtype != torch.int32:
+        raise ValueError("wisp: ends are int32")
+    dev = x.get_device()
+    for t, name in ((w, "w"), (ends, "ends")):
+        if t.get_device() != dev:
+            _require_device(t, x.device, name)
+    if w.stride(2) != 1 and w.shape[2] > 1:
+        raise ValueError("wisp: each row of w must be contiguous")
+    return x.shape[0], w.shape[0], w.shape[1], w.shape[2]
+
+
+def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x`` with contiguous rows that start 16-byte aligned."""
+    size = x.element_size()
+    if x.stride(1) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) * size % 16 == 0 and \
+            x.stride(0) >= x.shape[1]:
+        return x
+    x = x.contiguous()
+    return x.clone() if x.data_ptr() % 16 else x
+
+
+def _output(x, N, dtype, out, inputs) -> torch.Tensor:
+    if out is None:
+        return torch.empty((x.shape[0], N), dtype=dtype, device=x.device)
+    if out.shape != (x.shape[0], N) or out.dtype != dtype or not out.is_contiguous():
+        raise ValueError(f"wisp: out must be a contiguous {(x.shape[0], N)} {dtype} tensor")
+    if out.get_device() != x.get_device():
+        _require_device(out, x.device, "out")
+    _check_apart("out", out, [(t, False) for t in inputs])
+    return out
+
+
+@_on_device
+def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, *,
+               dtype: torch.dtype = torch.bfloat16,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[i] = w[e] @ x[i]`` for the rows ``i`` of group ``e``: bfloat16
+    ``x [M, K]`` and ``w [E, N, K]``, float32 sums, rounded once to ``dtype``
+    (bfloat16 or float32; a given ``out`` is of that type).  K is a multiple of
+    8; rows of ``x`` and experts of ``w`` may lie any distance apart."""
+    M, E, N, K = _sizes(x, w, ends)
+    if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
+        raise NotImplementedError("wisp: grouped_mm takes bfloat16 rows and weights")
+    if dtype not in _DTYPES:
+        raise NotImplementedError(f"wisp: grouped_mm cannot give {dtype} (float32 and bfloat16)")
+    x, ends = _aligned_rows(x), ends.contiguous()
+    given = out is not None
+    out = _output(x, N, dtype, out, (x, ends) if given else ())
+    if M and N:
+        check(lib().wisp_grouped_mm(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
+                                    w.stride(1), ends.data_ptr(), E, M, N, K, out.data_ptr(),
+                                    _DTYPES[dtype], int(not given), _stream(x)), "grouped_mm")
+    return out
+
+
+@_on_device
+def grouped_mm_fp8(q: torch.Tensor, s: torch.Tensor, w: torch.Tensor, ws: torch.Tensor,
+                   ends: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`grouped_mm` over block FP8, in bfloat16: codes ``q [M, K]`` with
+    scales ``s [M, ceil(K / 128)]`` (``add_rms_norm_fp8``, ``silu_mul_fp8``)
+    and codes ``w [E, N, K]`` with block scales ``ws [E, ceil(N / 128),
+    ceil(K / 128)]``, all codes ``float8_e4m3fn`` and scales float32.  K is a
+    multiple of 16.  The products of 128 columns are summed by the matrix
+    instruction, scaled and summed in float32 (to some 2^-16 of the sum of the
+    products' sizes: there is no float32 output), and rounded once."""
+    M, E, N, K = _sizes(q, w, ends)
+    if q.dtype != FP8 or w.dtype != FP8:
+        raise NotImplementedError("wisp: grouped_mm_fp8 takes float8_e4m3fn codes")
+    G, B = -(-K // GROUP), -(-N // GROUP)
+    if s.shape != (M, G) or ws.shape != (E, B, G) or s.dtype != torch.float32 or \
+            ws.dtype != torch.float32:
+        raise ValueError(f"wisp: scales are float32, s {(M, G)} and ws {(E, B, G)}")
+    for t, name in ((s, "s"), (ws, "ws")):
+        if t.get_device() != q.get_device():
+            _require_device(t, q.device, name)
+    if E and B and G and not ws[0].is_contiguous():
+        raise ValueError("wisp: each expert's block scales must be contiguous")
+    q, ends = _aligned_rows(q), ends.contiguous()
+    if (s.stride(1) != 1 and G > 1) or s.stride(0) < G:
+        s = s.contiguous()
+    given = out is not None
+    out = _output(q, N, torch.bfloat16, out, (q, s, ends) if given else ())
+    if M and N:
+        check(lib().wisp_grouped_mm_fp8(
+            q.data_ptr(), q.stride(0), s.data_ptr(), s.stride(0), w.data_ptr(), w.stride(0),
+            w.stride(1), ws.data_ptr(), ws.stride(0), ends.data_ptr(), E, M, N, K, out.data_ptr(),
+            int(not given), _stream(q)), "grouped_mm_fp8")
+    return out
+
+
+__all__ = ["grouped_mm", "grouped_mm_fp8"]

@@ -1,0 +1,192 @@
+"""Rows of activations before and between the experts' products: the RMS norm
+with the residual's addition, and the SwiGLU, with outputs in the rows' own
+type or in 8 bits with scales.
+
+The reference leaves both to vLLM; here they make the 8-bit rows that
+:func:`wisp.integrations.vllm.grouped_mm.grouped_mm_fp8` reads, so that a row is
+rounded once on its way into the product, and a program that sends rows to the
+owners of their experts moves half the bytes.
+
+8-bit rows: ``float8_e4m3fn`` codes ``[rows, cols]`` and one float32 scale per
+row and group of 128 columns, ``[rows, ceil(cols / 128)]`` (the format of
+``wisp_quant_fp8_groups``; here a row's last group may be shorter):
+``s = max(max|y|, 1e-10) / 448`` and ``q = y / s`` to the nearest code, from
+the float32 ``y``.  A group that holds an infinity or a NaN gets NaN codes.
+"""
+from __future__ import annotations
+
+import functools
+
+import torch
+
+from wisp_amd import _lib
+from wisp_amd._lib import check, lib
+from .fused_moe import _require_device
+
+FP8 = torch.float8_e4m3fn
+GROUP = 128
+_DTYPES = {torch.float32: _lib.WISP_F32, torch.bfloat16: _lib.WISP_BF16}
+
+
+def _on_device(fn):
+    """Runs ``fn`` with its first argument's GPU as the current device, on
+    that device's current stream."""
+    first = fn.__code__.co_varnames[0]
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        t = args[0] if args else kwargs.get(first)
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError(f"wisp: {fn.__name__} takes device tensors")
+        if t.get_device() == torch._C._cuda_getDevice():
+            return fn(*args, **kwargs)
+        with torch.cuda.device(t.device):
+            return fn(*args, **kwargs)
+    return call
+
+
+def _stream(t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with contiguous rows (any distance between them)."""
+    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+
+
+def _overlap(t: torch.Tensor, other: torch.Tensor) -> bool:
+    """Whether rows of ``t`` and ``other`` (2-D, contiguous rows) share bytes."""
+    def of(v):
+        size = v.element_size()
+        return v.data_ptr(), v.shape[1] * size, (v.stride(0) if v.shape[0] > 1 else 0) * size
+
+    (a, wide_a, step_a), (b, wide_b, step_b) = of(t), of(other)
+    if a >= b + (other.shape[0] - 1) * step_b + wide_b or \
+            b >= a + (t.shape[0] - 1) * step_a + wide_a:
+        return False
+    # columns of one buffer: rows interleave without meeting
+    return not (step_a == step_b and wide_a <= (b - a) % step_a <= step_a - wide_b) \
+        if step_a else True
+
+
+def _check_apart(name: str, t: torch.Tensor, others) -> None:
+    """``t`` is written row by row while the others are read and written: it
+    may be one of them, element by element, but not overlap one otherwise."""
+    for other, may_be in others:
+        if other is None or not t.numel() or not other.numel():
+            continue
+        other = other if other.dim() == 2 else other[None]
+        if may_be and t.data_ptr() == other.data_ptr() and t.dtype == other.dtype and \
+                (t.stride(0) == other.stride(0) or t.shape[0] == 1):
+            continue
+        if _overlap(t, other):
+            raise ValueError(f"wisp: {name} overlaps another tensor of the call")
+
+
+def _norm(x, weight, eps, residual, residual_out, out, want_out, want_fp8):
+    if x.dim() != 2 or weight.dim() != 1 or weight.shape[0] != x.shape[1]:
+        raise ValueError("wisp: x is [rows, cols] and weight [cols]")
+    if x.dtype not in _DTYPES:
+        raise NotImplementedError(f"wisp: rows of {x.dtype} (float32 and bfloat16)")
+    dev = x.get_device()
+    for t in (weight, residual):
+        if t is None:
+            continue
+        if t.dtype != x.dtype and t.dtype != torch.float32:
+            raise NotImplementedError("wisp: weight and residual are of x's type or float32")
+        if t.get_device() != dev:
+            _require_device(t, x.device, "weight" if t is weight else "residual")
+    rows, cols = x.shape
+    x, weight = _rows(x), weight.contiguous()
+    res = None
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f"wisp: residual must be {tuple(x.shape)}")
+        res = _rows(residual)
+        if residual_out is None:
+            residual_out = torch.empty_like(x, dtype=residual.dtype,
+                                            memory_format=torch.contiguous_format)
+        else:
+            if residual_out.shape != x.shape or residual_out.dtype != residual.dtype or \
+                    (cols > 1 and residual_out.stride(1) != 1) or \
+                    (rows > 1 and residual_out.stride(0) < cols):
+                raise ValueError(f"wisp: residual_out must be {tuple(x.shape)} {residual.dtype} "
+                                 "with contiguous rows")
+            if residual_out.get_device() != dev:
+                _require_device(residual_out, x.device, "residual_out")
+            _check_apart("residual_out", residual_out,
+                         ((x, True), (res, True), (weight, False)))
+    elif residual_out is not None:
+        raise ValueError("wisp: residual_out without a residual")
+    if out is not None:
+        if out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
+            raise ValueError(f"wisp: out must be a contiguous {tuple(x.shape)} {x.dtype} tensor")
+        if out.get_device() != dev:
+            _require_device(out, x.device, "out")
+        _check_apart("out", out, ((x, True), (res, True), (weight, False),
+                                  (residual_out, False)))
+    elif want_out:
+        out = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+    q = s = None
+    if want_fp8:
+        q = torch.empty((rows, cols), dtype=FP8, device=x.device)
+        s = torch.empty((rows, -(-cols // GROUP)), dtype=torch.float32, device=x.device)
+    if rows and cols:
+        check(lib().wisp_add_rms_norm(
+            x.data_ptr(), _DTYPES[x.dtype], rows, cols, x.stride(0),
+            None if res is None else res.data_ptr(),
+            0 if res is None else _DTYPES[res.dtype], 0 if res is None else res.stride(0),
+            None if res is None else residual_out.data_ptr(),
+            0 if res is None else residual_out.stride(0),
+            weight.data_ptr(), _DTYPES[weight.dtype], eps,
+            None if out is None else out.data_ptr(), None if q is None else q.data_ptr(),
+            None if s is None else s.data_ptr(), _stream(x)), "add_rms_norm")
+    return out, q, s, residual_out
+
+
+@_on_device
+def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                 residual: torch.Tensor | None = None, *, out: torch.Tensor | None = None,
+                 residual_out: torch.Tensor | None = None):
+    """``(out, residual_out)`` of rows ``x [rows, cols]`` (bfloat16 or
+    float32): ``r = x + residual`` rounded once to the residual's type (``x``
+    itself and ``None`` without a residual), ``out = r / sqrt(mean(r**2) +
+    eps) * weight`` in float32, rounded once to ``x``'s type.  The weight and
+    the residual are of ``x``'s type or float32.  Rows may lie any distance
+    apart; up to 32768 columns.  ``out`` may be ``x`` or ``residual``, and
+    ``residual_out`` may be ``residual`` or ``x``, but not one the other."""
+    out, _, _, residual_out = _norm(x, weight, eps, residual, residual_out, out, True, False)
+    return out, residual_out
+
+
+@_on_device
+def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                     residual: torch.Tensor | None = None, *, out: torch.Tensor | None = None,
+                     residual_out: torch.Tensor | None = None):
+    """:func:`add_rms_norm` in 8 bits: ``(codes, scales, residual_out)``.  With
+    ``out`` the normalised rows also go there in ``x``'s type (for a router
+    that reads them), from the same float32 values."""
+    _, q, s, residual_out = _norm(x, weight, eps, residual, residual_out, out, False, True)
+    return q, s, residual_out
+
+
+@_on_device
+def silu_mul_fp8(h: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """SwiGLU of a product's rows ``h [rows, 2 * I]`` (gate, then up; bfloat16
+    or float32, rows any distance apart) in 8 bits: codes ``[rows, I]`` and
+    scales ``[rows, ceil(I / 128)]`` of ``silu(h[:, :I]) * h[:, I:]``."""
+    if h.dim() != 2 or h.shape[1] % 2:
+        raise ValueError("wisp: h is [rows, 2 * I]")
+    if h.dtype not in _DTYPES:
+        raise NotImplementedError(f"wisp: rows of {h.dtype} (float32 and bfloat16)")
+    h = _rows(h)
+    rows, inter = h.shape[0], h.shape[1] // 2
+    q = torch.empty((rows, inter), dtype=FP8, device=h.device)
+    s = torch.empty((rows, -(-inter // GROUP)), dtype=torch.float32, device=h.device)
+    if rows and inter:
+        check(lib().wisp_silu_mul_fp8(h.data_ptr(), _DTYPES[h.dtype], rows, inter, h.stride(0),
+                                      q.data_ptr(), s.data_ptr(), _stream(h)), "silu_mul_fp8")
+    return q, s
+
+
+__all__ = ["add_rms_norm", "add_rms_norm_fp8", "silu_mul_fp8"]

@@ -112,6 +112,13 @@ SIGNATURES = {
                                     _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz,
                                     _vp]),
     "wisp_moe_mxfp4_work_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "wisp_add_rms_norm": (_i32, [_vp, _i32, _i64, _i32, _i64, _vp, _i32, _i64, _vp, _i64, _vp,
+                                 _i32, C.c_float, _vp, _vp, _vp, _vp]),
+    "wisp_grouped_mm": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _i32,
+                               _i32, _vp]),
+    "wisp_grouped_mm_fp8": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i32,
+                                   _i32, _i32, _i32, _vp, _i32, _vp]),
+    "wisp_silu_mul_fp8": (_i32, [_vp, _i32, _i64, _i32, _i64, _vp, _vp, _vp]),
     "wisp_layer_create": (_i32, [C.POINTER(LayerDesc), C.POINTER(_vp)]),
     "wisp_layer_destroy": (_i32, [_vp]),
     "wisp_layer_set_scratch": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp]),

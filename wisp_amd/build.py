@@ -28,6 +28,8 @@ SOURCES = [
     "experts_mxfp4.hip",
     "experts_mxfp4_few.hip",
     "quant_mxfp4.hip",
+    "rows_fp8.hip",
+    "grouped_mm.hip",
     "pagein.hip",
     "packed.hip",
     "prefetch.hip",
