@@ -12,7 +12,7 @@
 // v_mfma_f32_16x16x32_bf16; 128 columns in FP8, one v_mfma_f32_16x16x128_f8f6f4
 // and one block of the scales.  The weights are the A operand, so a lane holds
 // consecutive outputs of one row of x.
-#include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -65,6 +65,18 @@ __device__ __attribute__((always_inline)) inline u32x4 load16(Buffer b, int voff
 __device__ __attribute__((always_inline)) inline float load4(Buffer b, int voff, int soff) {
   return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(b, voff, soff, 0));
 }
+__device__ __attribute__((always_inline)) inline void store16b(u32x4 v, Buffer b, int voff,
+                                                                 int soff) {
+  __builtin_amdgcn_raw_buffer_store_b128(v, b, voff, soff, 0);
+}
+__device__ __attribute__((always_inline)) inline void store4b(uint32_t v, Buffer b, int voff,
+                                                                 int soff) {
+  __builtin_amdgcn_raw_buffer_store_b32(v, b, voff, soff, 0);
+}
+__device__ __attribute__((always_inline)) inline void store2b(uint16_t v, Buffer b, int voff,
+                                                                 int soff) {
+  __builtin_amdgcn_raw_buffer_store_b16(v, b, voff, soff, 0);
+}
 __device__ __attribute__((always_inline)) inline f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                  __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -84,6 +96,9 @@ typedef int Buffer;
 __device__ inline Buffer buffer(const void*, uint32_t) { return 0; }
 __device__ inline u32x4 load16(Buffer, int, int) { return u32x4{}; }
 __device__ inline float load4(Buffer, int, int) { return 0.f; }
+__device__ inline void store16b(u32x4, Buffer, int, int) {}
+__device__ inline void store4b(uint32_t, Buffer, int, int) {}
+__device__ inline void store2b(uint16_t, Buffer, int, int) {}
 __device__ inline f32x4 mfma_bf16(u32x4, u32x4, f32x4 c) { return c; }
 __device__ inline f32x4 mfma_fp8(u32x4, u32x4, u32x4, u32x4) { return f32x4{}; }
 #endif
@@ -197,35 +212,54 @@ __device__ inline void zero_rows(const Args& a, int last) {
 // over the banks.
 __device__ inline int at(int r, int cb) { return r * kChunk + ((cb ^ (r & 7)) << 4); }
 
-// 16 consecutive outputs (4 groups of 4) of one row of out.
-__device__ inline void store16(const Args& a, int64_t row, int n, const f32x4 (&v)[4], bool wide) {
-  if (a.out_f32) {
-    float* p = (float*)a.out + row * a.N + n;
-    if (wide && n + 16 <= a.N) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) reinterpret_cast<f32x4*>(p)[g] = v[g];
-    } else {
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + 4 * g + j < a.N) p[4 * g + j] = v[g][j];
-    }
-  } else {
-    uint16_t* p = (uint16_t*)a.out + row * a.N + n;
-    uint32_t u[8];
+// A tile's outputs, from row row0 of out on: rows behind the tile's are behind
+// the buffer's end, and so is where a column behind N is sent.
+struct Outputs {
+  Buffer b;
+  int N, wide;
+};
+__device__ __attribute__((always_inline)) inline Outputs outputs(const Args& a, int64_t row0,
+                                                                 int rows) {
+  const int wide = a.out_f32 ? 4 : 2;
+  return Outputs{buffer((uint8_t*)a.out + row0 * a.N * wide, (uint32_t)(rows * a.N * wide)), a.N,
+                 wide};
+}
+constexpr int kNowhere = INT32_MIN;  // an offset behind every end, with any tile's added
+
+// 16 consecutive outputs (4 groups of 4), columns [n, n + 16) of row
+// 16 * t + col.  (The tile's part of the offset is the wave's: per lane, the
+// compiler would hold every tile's in a register through the products.)
+template <bool F32, bool WHOLE>
+__device__ __attribute__((always_inline)) inline void store16(const Outputs& o, int t, int col,
+                                                              int n, const f32x4 (&v)[4]) {
+  const int at = (col * o.N + n) * o.wide, soff = 16 * t * o.N * o.wide;
+  if constexpr (F32) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      u[2 * g] = bf16_pair(v[g][0], v[g][1]);
-      u[2 * g + 1] = bf16_pair(v[g][2], v[g][3]);
-    }
-    if (wide && n + 16 <= a.N) {
-      reinterpret_cast<u32x4*>(p)[0] = u32x4{u[0], u[1], u[2], u[3]};
-      reinterpret_cast<u32x4*>(p)[1] = u32x4{u[4], u[5], u[6], u[7]};
-    } else {
+      if constexpr (WHOLE) {
+        store16b(__builtin_bit_cast(u32x4, v[g]), o.b, n + 4 * g < o.N ? at + 16 * g : kNowhere,
+                 soff);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (n + i < a.N) p[i] = (uint16_t)(u[i / 2] >> (16 * (i & 1)));
+        for (int j = 0; j < 4; ++j)
+          store4b(__float_as_uint(v[g][j]), o.b,
+                  n + 4 * g + j < o.N ? at + 16 * g + 4 * j : kNowhere, soff);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 x = v[2 * h], y = v[2 * h + 1];
+      const u32x4 u = {bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(y[0], y[1]),
+                       bf16_pair(y[2], y[3])};
+      if constexpr (WHOLE) {
+        store16b(u, o.b, n + 8 * h < o.N ? at + 16 * h : kNowhere, soff);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          store2b((uint16_t)(u[i / 2] >> (16 * (i & 1))), o.b,
+                  n + 8 * h + i < o.N ? at + 16 * h + 2 * i : kNowhere, soff);
+      }
     }
   }
 }
@@ -250,7 +284,11 @@ struct Shape {
   static constexpr int kLds = 4 * kTile + kScales + (int)sizeof(Table);
 };
 
-template <bool FP8, int NT>
+// What a kernel writes: 16-byte pieces of bfloat16 (N a multiple of 8) or of
+// float32 (of 4), or single values.
+enum Out { kBf16, kF32, kNarrow };
+
+template <bool FP8, int NT, Out OUT>
 __global__ __launch_bounds__(256, NT == 16 ? 1 : 2) void grouped_tile_kernel(const Args a) {
   using Sh = Shape<NT>;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -263,7 +301,6 @@ __global__ __launch_bounds__(256, NT == 16 ? 1 : 2) void grouped_tile_kernel(con
   __syncthreads();
   const int npanels = (a.N + kPanel - 1) / kPanel;
   const int chunks = (a.row_bytes + kChunk - 1) / kChunk, pairs = (chunks + 1) / 2;
-  const bool wide = a.N % 16 == 0 && (uintptr_t)a.out % 16 == 0;
 
   // lane offsets into the weights and the rows of x
   const int wvoff = (16 * (col >> 2) + (col & 3)) * (int)a.w_ld + 16 * quarter;
@@ -350,10 +387,52 @@ __global__ __launch_bounds__(256, NT == 16 ? 1 : 2) void grouped_tile_kernel(con
   };
 
   f32x4 acc[4][NT];
+
+  // A stage is multiplied in blocks of four 16-byte fragments a lane: bf16, one
+  // half chunk of four tiles of 16 rows; FP8, one chunk of two.  The fragments of
+  // a block are read while the one before it is multiplied; the last block of
+  // a stage is multiplied behind the barrier, over the first reads of the next.
+  constexpr int kSteps = FP8 ? 2 : 4;               // of a stage, along the columns
+  constexpr int kWide = FP8 ? 2 : 4;                // tiles of 16 rows of a block
+  constexpr int kBlocks = kSteps * (NT / kWide);
+  u32x4 f[2][4];
+  float fs[2][2];
+  auto read = [&](int i, int stage, int b) {
+    const int step = b / (NT / kWide), t0 = b % (NT / kWide) * kWide;
+    const uint8_t* tile = smem + (2 * stage + (FP8 ? step : step / 2)) * Sh::kTile;
 #pragma unroll
-  for (int g = 0; g < 4; ++g)
+    for (int k = 0; k < 4; ++k) {
+      const int t = t0 + (FP8 ? k / 2 : k), h = FP8 ? k & 1 : step & 1;
+      f[i][k] = *reinterpret_cast<const u32x4*>(tile + at(16 * t + col, 4 * h + quarter));
+    }
+    if constexpr (FP8)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) acc[g][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < 2; ++t)
+        fs[i][t] = scales[(2 * stage + step) * Sh::kToks + 16 * (t0 + t) + col];
+  };
+  auto multiply = [&](int i, int b, int nt) {
+    const int step = b / (NT / kWide), t0 = b % (NT / kWide) * kWide;
+    if (t0 >= nt) return;
+    if constexpr (!FP8) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          acc[g][t0 + t] = mfma_bf16(wf[step / 2][step & 1][g], f[i][t], acc[g][t0 + t]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const float sc = fs[i][t] * wscale[step];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 d = mfma_fp8(wf[step][0][g], wf[step][1][g], f[i][2 * t], f[i][2 * t + 1]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[g][t0 + t][j] = __builtin_fmaf(d[j], sc, acc[g][t0 + t][j]);
+        }
+      }
+    }
+  };
 
   Place cur = next(Place{Work{-1, 0, 0, 0}, 0});
   if (cur.work.expert >= 0) {
@@ -364,97 +443,75 @@ __global__ __launch_bounds__(256, NT == 16 ? 1 : 2) void grouped_tile_kernel(con
     Place wnext = next(cur);
     load_x(wnext);
     __syncthreads();
-    for (int stage = 0;; stage ^= 1) {
-      const Place xnext = next(wnext);
-      const int nt = (cur.work.rows + 15) / 16;
+    read(0, 0, 0);
+    int stage = 0;
+    do {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint8_t* tile = smem + (2 * stage + c) * Sh::kTile;
-        const int left = a.row_bytes - (2 * cur.pair + c) * kChunk;
-        if (left < kChunk) {
+      for (int g = 0; g < 4; ++g)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (64 * h + 16 * quarter >= left)
+        for (int t = 0; t < NT; ++t) acc[g][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const Work work = cur.work;
+      const int nt = (work.rows + 15) / 16;
+      for (int pair = 0; pair < pairs; ++pair) {
+        const Place xnext = next(wnext);
 #pragma unroll
-              for (int g = 0; g < 4; ++g) wf[c][h][g] = u32x4{0, 0, 0, 0};
-        }
-        if constexpr (!FP8) {
+        for (int c = 0; c < 2; ++c) {
+          const int left = a.row_bytes - (2 * pair + c) * kChunk;
+          if (left < kChunk) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h)
+              if (64 * h + 16 * quarter >= left)
 #pragma unroll
-            for (int t0 = 0; t0 < NT; t0 += 4) {
-              if (t0 >= nt) break;
-              u32x4 f[4];
-#pragma unroll
-              for (int t = 0; t < 4; ++t)
-                f[t] = *reinterpret_cast<const u32x4*>(
-                    tile + at(16 * (t0 + t) + col, 4 * h + quarter));
-#pragma unroll
-              for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                  acc[g][t0 + t] = mfma_bf16(wf[c][h][g], f[t], acc[g][t0 + t]);
-            }
-        } else {
-#pragma unroll
-          for (int t0 = 0; t0 < NT; t0 += 2) {
-            if (t0 >= nt) break;
-            u32x4 f[2][2];
-            float sc[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                f[t][h] = *reinterpret_cast<const u32x4*>(
-                    tile + at(16 * (t0 + t) + col, 4 * h + quarter));
-              sc[t] = scales[(2 * stage + c) * Sh::kToks + 16 * (t0 + t) + col] * wscale[c];
-            }
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                const f32x4 d = mfma_fp8(wf[c][0][g], wf[c][1][g], f[t][0], f[t][1]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  acc[g][t0 + t][j] = __builtin_fmaf(d[j], sc[t], acc[g][t0 + t][j]);
-              }
+                for (int g = 0; g < 4; ++g) wf[c][h][g] = u32x4{0, 0, 0, 0};
           }
         }
-        if (c == 0) {
-          store_x(wnext, stage ^ 1);
-          load_x(xnext);
-        }
-        load_w(wnext, c);
-      }
-      if (cur.pair + 1 == pairs) {
-        const int n = cur.work.panel * kPanel + wave * kWaveRows + 16 * quarter;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int r = 16 * t + col;
-          if (r < cur.work.rows && n < a.N) {
-            const f32x4 v[4] = {acc[0][t], acc[1][t], acc[2][t], acc[3][t]};
-            store16(a, cur.work.row0 + r, n, v, wide);
+        for (int b = 0; b < kBlocks; ++b) {
+          if (b + 1 < kBlocks) {
+            read((b + 1) & 1, stage, b + 1);
+          } else {
+            block_lds_sync();
+            read((b + 1) & 1, stage ^ 1, 0);
           }
-#pragma unroll
-          for (int g = 0; g < 4; ++g) acc[g][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+          __builtin_amdgcn_sched_barrier(0);
+          multiply(b & 1, b, nt);
+          __builtin_amdgcn_sched_barrier(0);
+          if (b == kBlocks / 4) {
+            store_x(wnext, stage ^ 1);
+            load_x(xnext);
+          }
+          if (b + 1 == kBlocks / 2) load_w(wnext, 0);
+          if (b + 1 == kBlocks) load_w(wnext, 1);
+          __builtin_amdgcn_sched_barrier(0);
         }
+        stage ^= 1;
+        cur = wnext;
+        wnext = xnext;
       }
-      cur = wnext;
-      wnext = xnext;
-      if (cur.work.expert < 0) break;
-      block_lds_sync();
-    }
+      const Outputs o = outputs(a, work.row0, work.rows);
+      const int n = work.panel * kPanel + wave * kWaveRows + 16 * quarter;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const f32x4 v[4] = {acc[0][t], acc[1][t], acc[2][t], acc[3][t]};
+        if constexpr (OUT != kNarrow)
+          store16<OUT == kF32, true>(o, t, col, n, v);
+        else if (a.out_f32)
+          store16<true, false>(o, t, col, n, v);
+        else
+          store16<false, false>(o, t, col, n, v);
+      }
+    } while (cur.work.expert >= 0);
   }
   if (a.zero_tail) zero_rows(a, tab->last);
 }
 
-template <bool FP8, int NT>
+template <bool FP8, int NT, Out OUT>
 hipError_t launch_tile(const Args& a, hipStream_t st) {
   static std::atomic<uint64_t> done{0};
-  const hipError_t e = allow_lds(&grouped_tile_kernel<FP8, NT>, Shape<NT>::kLds, Shape<NT>::kLds,
-                                 &done);
+  const hipError_t e = allow_lds(&grouped_tile_kernel<FP8, NT, OUT>, Shape<NT>::kLds,
+                                 Shape<NT>::kLds, &done);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((grouped_tile_kernel<FP8, NT>), dim3(NT == 16 ? 256 : 512), dim3(256),
+  hipLaunchKernelGGL((grouped_tile_kernel<FP8, NT, OUT>), dim3(NT == 16 ? 256 : 512), dim3(256),
                      Shape<NT>::kLds, st, a);
   return hipGetLastError();
 }
@@ -464,15 +521,25 @@ int refuse(int rc, const char* why, const char* where) {
   return rc;
 }
 
-template <bool FP8>
-int grouped(const Args& a, hipStream_t st) {
+template <bool FP8, Out OUT>
+hipError_t launch_of(const Args& a, hipStream_t st) {
   // rows an expert has if the rows are spread evenly
   const int per = a.M / a.E;
+  if constexpr (!FP8) {
+    if (per > 128) return launch_tile<false, 16, OUT>(a, st);
+  }
+  return launch_tile<FP8, 4, OUT>(a, st);
+}
+
+template <bool FP8>
+int grouped(const Args& a, hipStream_t st) {
   hipError_t e;
-  if (per > 64 && !FP8)
-    e = launch_tile<false, 8>(a, st);
+  if (a.N % (a.out_f32 ? 4 : 8))
+    e = launch_tile<FP8, 4, kNarrow>(a, st);
+  else if (a.out_f32)
+    e = launch_of<false, kF32>(a, st);
   else
-    e = launch_tile<FP8, 4>(a, st);
+    e = launch_of<FP8, kBf16>(a, st);
   WISP_HIP_TRY(e);
   return WISP_OK;
 }
@@ -485,8 +552,8 @@ const char* unsupported(int64_t x_ld, int64_t w_ld, int64_t w_stride, int64_t N,
       (uintptr_t)w % 16)
     return "x, w and their strides must be 16-byte aligned";
   // (32-bit offsets inside a tile of x and inside an expert's weights)
-  if (N * w_ld * elem >= (int64_t)1 << 31 || x_ld * elem >= (int64_t)1 << 22)
-    return "an expert's weights of 2 GiB or rows of x 4 MiB apart";
+  if (N * w_ld * elem >= (int64_t)1 << 31 || x_ld * elem >= (int64_t)1 << 22 || N >= 1 << 21)
+    return "an expert's weights of 2 GiB, rows of x 4 MiB apart or 2^21 outputs";
   return nullptr;
 }
 
