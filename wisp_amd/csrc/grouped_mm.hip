@@ -12,7 +12,7 @@
 // v_mfma_f32_16x16x32_bf16; 128 columns in FP8, one v_mfma_f32_16x16x128_f8f6f4
 // and one block of the scales.  The weights are the A operand, so a lane holds
 // consecutive outputs of one row of x.
-#include <type_traits>
+#include <algorithm>
 
 #include "common.h"
 
@@ -20,7 +20,9 @@ namespace wisp {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -29,8 +31,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 constexpr int kChunk = 128;   // bytes of a row per chunk
 constexpr int kBlock = 128;   // rows and columns of a block of FP8 weights
 constexpr int kWaves = 4;     // of a block
-constexpr int kWaveRows = 64;  // weight rows of a wave
-constexpr int kPanel = kWaves * kWaveRows;
+constexpr int kPanel = 256;   // weight rows of the large tiles
 
 struct Args {
   const uint8_t* x;
@@ -59,6 +60,21 @@ __device__ __attribute__((always_inline)) inline Buffer buffer(const void* p, ui
   return __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), 0,
                                            __builtin_amdgcn_readfirstlane((int)bytes), 0x00027000);
 }
+// 16 bytes at p, the same for the whole wave, plus a lane's offset.
+__device__ __attribute__((always_inline)) inline u32x4 load_global(const uint8_t* p, uint32_t off) {
+  typedef const __attribute__((address_space(1))) uint8_t* Bytes;
+  return *(const __attribute__((address_space(1))) u32x4*)((Bytes)p + off);
+}
+__device__ __attribute__((always_inline)) inline float load_global4(const uint8_t* p, uint32_t off) {
+  typedef const __attribute__((address_space(1))) uint8_t* Bytes;
+  return *(const __attribute__((address_space(1))) float*)((Bytes)p + off);
+}
+__device__ __attribute__((always_inline)) inline const uint8_t* uniform(const uint8_t* p) {
+  const uint64_t a = (uint64_t)p;
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32));
+  return (const uint8_t*)(((uint64_t)hi << 32) | lo);
+}
 __device__ __attribute__((always_inline)) inline u32x4 load16(Buffer b, int voff, int soff) {
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, voff, soff, 0));
 }
@@ -68,6 +84,10 @@ __device__ __attribute__((always_inline)) inline float load4(Buffer b, int voff,
 __device__ __attribute__((always_inline)) inline void store16b(u32x4 v, Buffer b, int voff,
                                                                  int soff) {
   __builtin_amdgcn_raw_buffer_store_b128(v, b, voff, soff, 0);
+}
+__device__ __attribute__((always_inline)) inline void store8b(u32x2 v, Buffer b, int voff,
+                                                                 int soff) {
+  __builtin_amdgcn_raw_buffer_store_b64(v, b, voff, soff, 0);
 }
 __device__ __attribute__((always_inline)) inline void store4b(uint32_t v, Buffer b, int voff,
                                                                  int soff) {
@@ -79,6 +99,10 @@ __device__ __attribute__((always_inline)) inline void store2b(uint16_t v, Buffer
 }
 __device__ __attribute__((always_inline)) inline f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __attribute__((always_inline)) inline f32x16 mfma_bf16(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                  __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 __device__ __attribute__((always_inline)) inline f32x4 mfma_fp8(u32x4 a0, u32x4 a1, u32x4 b0,
@@ -94,12 +118,17 @@ __device__ __attribute__((always_inline)) inline f32x4 mfma_fp8(u32x4 a0, u32x4 
 #else  // the host pass does not know these builtins
 typedef int Buffer;
 __device__ inline Buffer buffer(const void*, uint32_t) { return 0; }
+__device__ inline u32x4 load_global(const uint8_t*, uint32_t) { return u32x4{}; }
+__device__ inline float load_global4(const uint8_t*, uint32_t) { return 0.f; }
+__device__ inline const uint8_t* uniform(const uint8_t* p) { return p; }
 __device__ inline u32x4 load16(Buffer, int, int) { return u32x4{}; }
 __device__ inline float load4(Buffer, int, int) { return 0.f; }
 __device__ inline void store16b(u32x4, Buffer, int, int) {}
+__device__ inline void store8b(u32x2, Buffer, int, int) {}
 __device__ inline void store4b(uint32_t, Buffer, int, int) {}
 __device__ inline void store2b(uint16_t, Buffer, int, int) {}
 __device__ inline f32x4 mfma_bf16(u32x4, u32x4, f32x4 c) { return c; }
+__device__ inline f32x16 mfma_bf16(u32x4, u32x4, f32x16 c) { return c; }
 __device__ inline f32x4 mfma_fp8(u32x4, u32x4, u32x4, u32x4) { return f32x4{}; }
 #endif
 
@@ -192,7 +221,7 @@ __device__ inline int work_of(int b, int j) {
   return ((i / kRun) * 8 + (b & 7)) * kRun + i % kRun;
 }
 
-// Zeros into the rows behind the last group, all blocks together.
+// Zeros into the rows behind the last group, all blocks (of a grid in x) together.
 __device__ inline void zero_rows(const Args& a, int last) {
   const int64_t wide = a.out_f32 ? 4 : 2;
   uint8_t* p = (uint8_t*)a.out + last * (int64_t)a.N * wide;
@@ -207,10 +236,14 @@ __device__ inline void zero_rows(const Args& a, int last) {
   if (at < rest) reinterpret_cast<uint16_t*>(p + head + body * 16)[at] = 0;
 }
 
-// Byte of 16-byte piece cb of row r of an LDS tile of 128-byte rows.  Rows
-// shift their pieces, so that the 16 rows a fragment reads at one piece spread
-// over the banks.
-__device__ inline int at(int r, int cb) { return r * kChunk + ((cb ^ (r & 7)) << 4); }
+// Byte of 16-byte piece cb of row r of an LDS tile of 128-byte rows.  Rows shift
+// their pieces so that neither a fragment's 16 or 32 consecutive rows nor the
+// permuted ones of the weights (16 * a + 4 * g + b, below) meet in a bank; rows 32
+// apart shift alike.  (SQ_LDS_BANK_CONFLICT of the reads is 0.)
+__device__ inline int at(int r, int cb) {
+  const int shift = (r & 3) | ((r >> 2 ^ r >> 4) & 1) << 2;
+  return r * kChunk + ((cb ^ shift) << 4);
+}
 
 // A tile's outputs, from row row0 of out on: rows behind the tile's are behind
 // the buffer's end, and so is where a column behind N is sent.
@@ -226,57 +259,57 @@ __device__ __attribute__((always_inline)) inline Outputs outputs(const Args& a, 
 }
 constexpr int kNowhere = INT32_MIN;  // an offset behind every end, with any tile's added
 
-// 16 consecutive outputs (4 groups of 4), columns [n, n + 16) of row
-// 16 * t + col.  (The tile's part of the offset is the wave's: per lane, the
-// compiler would hold every tile's in a register through the products.)
-template <bool F32, bool WHOLE>
-__device__ __attribute__((always_inline)) inline void store16(const Outputs& o, int t, int col,
-                                                              int n, const f32x4 (&v)[4]) {
-  const int at = (col * o.N + n) * o.wide, soff = 16 * t * o.N * o.wide;
-  if constexpr (F32) {
+// 4 * G consecutive outputs, columns [n, n + 4 * G) of row t0 + r; WHOLE: N is a
+// whole number of the pieces stored.  (t0, the same for the wave, goes into the
+// scalar offset: per lane, the compiler would hold every tile's offset in a
+// register through the products.)
+template <bool F32, bool WHOLE, int G>
+__device__ __attribute__((always_inline)) inline void store_outputs(const Outputs& o, int t0, int r, int n,
+                                                            const f32x4 (&v)[G]) {
+  const int at = (r * o.N + n) * o.wide, soff = t0 * o.N * o.wide;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      if constexpr (WHOLE) {
-        store16b(__builtin_bit_cast(u32x4, v[g]), o.b, n + 4 * g < o.N ? at + 16 * g : kNowhere,
-                 soff);
-      } else {
+  for (int g = 0; g < G; ++g) {
+    if constexpr (F32 && WHOLE) {
+      store16b(__builtin_bit_cast(u32x4, v[g]), o.b, n + 4 * g < o.N ? at + 16 * g : kNowhere, soff);
+    } else if constexpr (F32) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          store4b(__float_as_uint(v[g][j]), o.b,
-                  n + 4 * g + j < o.N ? at + 16 * g + 4 * j : kNowhere, soff);
+      for (int j = 0; j < 4; ++j)
+        store4b(__float_as_uint(v[g][j]), o.b, n + 4 * g + j < o.N ? at + 16 * g + 4 * j : kNowhere,
+                soff);
+    } else if constexpr (WHOLE && G > 1) {
+      if (g % 2 == 0) {
+        const f32x4 x = v[g], y = v[g + 1];
+        const u32x4 u = {bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(y[0], y[1]),
+                         bf16_pair(y[2], y[3])};
+        store16b(u, o.b, n + 4 * g < o.N ? at + 8 * g : kNowhere, soff);
       }
-    }
-  } else {
+    } else if constexpr (WHOLE) {
+      store8b(u32x2{bf16_pair(v[g][0], v[g][1]), bf16_pair(v[g][2], v[g][3])}, o.b,
+              n < o.N ? at : kNowhere, soff);
+    } else {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const f32x4 x = v[2 * h], y = v[2 * h + 1];
-      const u32x4 u = {bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(y[0], y[1]),
-                       bf16_pair(y[2], y[3])};
-      if constexpr (WHOLE) {
-        store16b(u, o.b, n + 8 * h < o.N ? at + 16 * h : kNowhere, soff);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          store2b((uint16_t)(u[i / 2] >> (16 * (i & 1))), o.b,
-                  n + 8 * h + i < o.N ? at + 16 * h + 2 * i : kNowhere, soff);
-      }
+      for (int j = 0; j < 4; ++j)
+        store2b((uint16_t)(bf16_pair(v[g][j], 0.f) & 0xffff), o.b,
+                n + 4 * g + j < o.N ? at + 8 * g + 2 * j : kNowhere, soff);
     }
   }
 }
 
 // ---------------------------------------------------------------------------
-// The tiles: 256 weight rows by up to 16 * NT rows of x
+// Few rows an expert: 64 * G weight rows by 64 rows of x
 // ---------------------------------------------------------------------------
 //
-// Persistent blocks of four waves.  A wave owns 64 weight rows and reads them
-// from memory straight into its registers, a chunk ahead: no other wave of the
-// block needs them.  The rows of x, which all four need, go through LDS, two
-// chunks a stage.  The loads of a block run ahead over the ends of its tiles.
-// A wave's MFMA row i of group g is weight row 16 * (i / 4) + 4 * g + i % 4, so
-// that a lane ends with 16 consecutive outputs of a row of x.
+// What bounds these calls is the weights' stream.  Persistent blocks of four
+// waves; a wave owns 16 * G weight rows and reads them from memory straight into
+// its registers, one to two chunks ahead: no other wave of the block needs them.
+// The rows of x, which all four need, go through LDS, two chunks a stage.  The
+// loads of a block run ahead over the ends of its tiles.  MFMA row i of a wave's
+// group g is weight row 4 * G * (i / 4) + 4 * g + i % 4, so that a lane ends with
+// 4 * G consecutive outputs of a row of x.
 
-template <int NT>
+template <int NT, int G>
 struct Shape {
+  static constexpr int kPanel = kWaves * 16 * G;  // weight rows
   static constexpr int kToks = 16 * NT;
   static constexpr int kCopies = kToks / 8 / kWaves;  // of a wave, 8 rows each
   static constexpr int kTile = kToks * kChunk;        // one chunk of the rows of x
@@ -288,9 +321,10 @@ struct Shape {
 // float32 (of 4), or single values.
 enum Out { kBf16, kF32, kNarrow };
 
-template <bool FP8, int NT, Out OUT>
-__global__ __launch_bounds__(256, NT == 16 ? 1 : 2) void grouped_tile_kernel(const Args a) {
-  using Sh = Shape<NT>;
+template <bool FP8, int NT, int G, Out OUT>
+__global__ __launch_bounds__(256, 2) void grouped_tile_kernel(const Args a) {
+  using Sh = Shape<NT, G>;
+  constexpr int kPanel = Sh::kPanel;
   extern __shared__ __align__(16) uint8_t smem[];
   float* scales = reinterpret_cast<float*>(smem + 4 * Sh::kTile);
   Table* tab = reinterpret_cast<Table*>(smem + 4 * Sh::kTile + Sh::kScales);
@@ -303,31 +337,36 @@ __global__ __launch_bounds__(256, NT == 16 ? 1 : 2) void grouped_tile_kernel(con
   const int chunks = (a.row_bytes + kChunk - 1) / kChunk, pairs = (chunks + 1) / 2;
 
   // lane offsets into the weights and the rows of x
-  const int wvoff = (16 * (col >> 2) + (col & 3)) * (int)a.w_ld + 16 * quarter;
+  const int wvoff = (4 * G * (col >> 2) + (col & 3)) * (int)a.w_ld + 16 * quarter;
   const int xrow = wave * 8 + (lane >> 3);
   const int xvoff = xrow * (int)a.x_ld + 16 * (lane & 7);
 
-  // the three works in flight: computed, weights loading, rows loading
+  // The three places in flight (computed, weights loading, rows loading): a pair of
+  // chunks of a work, left to go with those behind it.  Each panel starts at a
+  // place of its own and wraps around: blocks that all start at column 0 crowd
+  // a few memory channels (Qwen3 w13, 512 tokens: 179 us, so 147).
   struct Place {
     Work work;
-    int pair;
+    int pair, left;
   };
   int turn = 0;
   auto next = [&](Place p) -> Place {
-    if (p.work.expert >= 0 && ++p.pair < pairs) return p;
+    p.pair = p.pair + 1 == pairs ? 0 : p.pair + 1;
+    if (--p.left > 0) return p;
     do {
       p.work = find_work(tab, work_of(blockIdx.x, turn++), a.E, npanels, Sh::kToks);
     } while (p.work.expert >= 0 && p.work.rows == 0);
-    p.pair = 0;
+    p.pair = p.work.expert < 0 ? 0 : (int)((int64_t)p.work.panel * pairs / npanels);
+    p.left = pairs;
     return p;
   };
 
-  u32x4 wf[2][2][4];            // [chunk of a pair][half of it][group]
+  u32x4 wf[2][2][G];            // [chunk of a pair][half of it][group]
   u32x4 xs[2][Sh::kCopies];
   float xscale[2], wscale[2];
 
   auto load_w = [&](const Place& p, int c) {
-    const int64_t r0 = p.work.panel * kPanel + wave * kWaveRows;
+    const int64_t r0 = p.work.panel * kPanel + wave * 16 * G;
     const int64_t left = a.N - r0;  // (none: every load is behind the end)
     const Buffer b = buffer(a.w + (p.work.expert < 0 ? 0 : p.work.expert * a.w_stride) +
                                 (left > 0 ? r0 * a.w_ld : 0),
@@ -338,7 +377,7 @@ __global__ __launch_bounds__(256, NT == 16 ? 1 : 2) void grouped_tile_kernel(con
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
+      for (int g = 0; g < G; ++g)
         wf[c][h][g] = load16(b, wvoff, 4 * g * (int)a.w_ld + o + 64 * h);
     if constexpr (FP8) {
       const Buffer sb = buffer(a.ws + (p.work.expert < 0 ? 0 : p.work.expert * a.ws_stride),
@@ -386,7 +425,7 @@ __global__ __launch_bounds__(256, NT == 16 ? 1 : 2) void grouped_tile_kernel(con
     }
   };
 
-  f32x4 acc[4][NT];
+  f32x4 acc[G][NT];
 
   // A stage is multiplied in blocks of four 16-byte fragments a lane: bf16, one
   // half chunk of four tiles of 16 rows; FP8, one chunk of two.  The fragments of
@@ -417,14 +456,14 @@ __global__ __launch_bounds__(256, NT == 16 ? 1 : 2) void grouped_tile_kernel(con
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
+        for (int g = 0; g < G; ++g)
           acc[g][t0 + t] = mfma_bf16(wf[step / 2][step & 1][g], f[i][t], acc[g][t0 + t]);
     } else {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const float sc = fs[i][t] * wscale[step];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
+        for (int g = 0; g < G; ++g) {
           const f32x4 d = mfma_fp8(wf[step][0][g], wf[step][1][g], f[i][2 * t], f[i][2 * t + 1]);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -434,7 +473,7 @@ __global__ __launch_bounds__(256, NT == 16 ? 1 : 2) void grouped_tile_kernel(con
     }
   };
 
-  Place cur = next(Place{Work{-1, 0, 0, 0}, 0});
+  Place cur = next(Place{Work{-1, 0, 0, 0}, 0, 0});
   if (cur.work.expert >= 0) {
     load_x(cur);
     load_w(cur, 0);
@@ -447,7 +486,7 @@ __global__ __launch_bounds__(256, NT == 16 ? 1 : 2) void grouped_tile_kernel(con
     int stage = 0;
     do {
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
+      for (int g = 0; g < G; ++g)
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[g][t] = f32x4{0.f, 0.f, 0.f, 0.f};
       const Work work = cur.work;
@@ -456,13 +495,13 @@ __global__ __launch_bounds__(256, NT == 16 ? 1 : 2) void grouped_tile_kernel(con
         const Place xnext = next(wnext);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int left = a.row_bytes - (2 * pair + c) * kChunk;
+          const int left = a.row_bytes - (2 * cur.pair + c) * kChunk;
           if (left < kChunk) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
               if (64 * h + 16 * quarter >= left)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) wf[c][h][g] = u32x4{0, 0, 0, 0};
+                for (int g = 0; g < G; ++g) wf[c][h][g] = u32x4{0, 0, 0, 0};
           }
         }
 #pragma unroll
@@ -489,31 +528,586 @@ __global__ __launch_bounds__(256, NT == 16 ? 1 : 2) void grouped_tile_kernel(con
         wnext = xnext;
       }
       const Outputs o = outputs(a, work.row0, work.rows);
-      const int n = work.panel * kPanel + wave * kWaveRows + 16 * quarter;
+      const int n = work.panel * kPanel + wave * 16 * G + 4 * G * quarter;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const f32x4 v[4] = {acc[0][t], acc[1][t], acc[2][t], acc[3][t]};
+        f32x4 v[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) v[g] = acc[g][t];
         if constexpr (OUT != kNarrow)
-          store16<OUT == kF32, true>(o, t, col, n, v);
+          store_outputs<OUT == kF32, true>(o, 16 * t, col, n, v);
         else if (a.out_f32)
-          store16<true, false>(o, t, col, n, v);
+          store_outputs<true, false>(o, 16 * t, col, n, v);
         else
-          store16<false, false>(o, t, col, n, v);
+          store_outputs<false, false>(o, 16 * t, col, n, v);
       }
     } while (cur.work.expert >= 0);
   }
   if (a.zero_tail) zero_rows(a, tab->last);
 }
 
-template <bool FP8, int NT, Out OUT>
-hipError_t launch_tile(const Args& a, hipStream_t st) {
+// ---------------------------------------------------------------------------
+// bfloat16, many rows an expert: 256 weight rows by 64 * L rows of x
+// ---------------------------------------------------------------------------
+//
+// One block a CU, four waves (2 x 2): a wave owns 128 weight rows and every other
+// 32 rows of x, in 4 x L tiles of v_mfma_f32_32x32x16_bf16.  Both operands go
+// through registers to LDS, 8 lanes a row, loaded three chunks ahead of their
+// use: a wave that read its operands straight from memory (16 rows of 64 bytes a load) would
+// keep the address unit busy for 64 cycles a load instead of 16.  A chunk is four
+// steps of 16 columns; between a step's matrix instructions go the reads of the
+// next step's fragments and a quarter of the chunk's stores and loads.  The
+// second half of a chunk's last step is multiplied behind the barrier.
+// MFMA row 8 * a + 4 * h + b of a group of 32 is weight row 16 * h + 4 * a + b, so
+// that a lane ends with 16 consecutive outputs of a row of x.
+template <int L>
+struct Big {
+  static constexpr int kToks = 64 * L;
+  static constexpr int kRows = kPanel + kToks;       // of a stage
+  static constexpr int kStage = kRows * kChunk;
+  static constexpr int kCopies = kRows / 32;         // of a wave, 8 rows each
+  static constexpr int kLds = 2 * kStage + (int)sizeof(Table);
+};
+
+// TAIL: rows that are not whole pairs of chunks.
+template <int L, bool TAIL>
+__global__ __launch_bounds__(256, 1) void grouped_big_kernel(const Args a) {
+  using Sh = Big<L>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  Table* tab = reinterpret_cast<Table*>(smem + 2 * Sh::kStage);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave >> 1, wt = wave & 1;
+  if (wave == 0) fill_table(tab, a, Sh::kToks);
+  __syncthreads();
+  const int npanels = (a.N + kPanel - 1) / kPanel;
+  const int pairs = (a.row_bytes + 2 * kChunk - 1) / (2 * kChunk);  // of chunks
+
+  // copies: this lane's row and piece of every 32 rows
+  const int crow = wave * 8 + (lane >> 3), ccol = 16 * (lane & 7);
+  uint8_t* const cdst = smem + at(crow, lane & 7);
+  // fragments: this lane's row of every 32
+  const int col = lane & 31, high = lane >> 5;
+  const int frow = 16 * (col >> 2 & 1) + 4 * (col >> 3) + (col & 3);
+
+  // a pair of chunks of a work
+  struct Place {
+    Work work;
+    int pair;
+  };
+  int turn = 0;
+  auto next = [&](Place p) -> Place {
+    if (p.work.expert >= 0 && ++p.pair < pairs) return p;
+    do {
+      p.work = find_work(tab, work_of(blockIdx.x, turn++), a.E, npanels, Sh::kToks);
+    } while (p.work.expert >= 0 && p.work.rows == 0);
+    p.pair = 0;
+    return p;
+  };
+  // Where a work's rows start, and this lane's offsets of its copies from there;
+  // rows behind the last are that one again (what they give is not stored).
+  const uint8_t *wbase, *xbase;
+  uint32_t off[Sh::kCopies];
+  auto aim = [&](const Work& w) {
+    const int64_t r0 = w.panel * kPanel;
+    wbase = uniform(a.w + (w.expert < 0 ? 0 : w.expert * a.w_stride + r0 * a.w_ld));
+    xbase = uniform(a.x + w.row0 * a.x_ld);
+    const int wlast = w.expert < 0 ? 0 : (int)min(a.N - r0, (int64_t)kPanel) - 1;
+    const int xlast = max(w.rows, 1) - 1;
+#pragma unroll
+    for (int i = 0; i < Sh::kCopies; ++i)
+      off[i] = i < 8 ? min(32 * i + crow, wlast) * (uint32_t)a.w_ld
+                     : min(32 * (i - 8) + crow, xlast) * (uint32_t)a.x_ld;
+  };
+
+  u32x4 cp[2][Sh::kCopies];  // two chunks on their way to LDS: weights, then rows of x
+  f32x16 acc[4][L];
+  u32x4 wf[2][4], xf[2][L];
+
+  // Chunk c of a place's pair into cp[c].  (Raw buffer loads would return zeros
+  // behind a range's end by themselves, but pass a CU at one per 47 cycles,
+  // these at one per 26: the loads alone took 350 us where these take 191.)
+  auto load = [&](int pair, int c, int i) {
+    const int o = (2 * pair + c) * kChunk;
+    const uint8_t* base = i < 8 ? wbase : xbase;
+    if constexpr (TAIL)  // (columns behind the row's end: its last ones)
+      cp[c][i] = load_global(base, off[i] + min(o + ccol, a.row_bytes - 16));
+    else
+      cp[c][i] = load_global(base + o, off[i] + ccol);
+  };
+  // chunk c of a pair has stage c
+  auto store = [&](int pair, int c, int i) {
+    u32x4 v = cp[c][i];
+    if constexpr (TAIL) {
+      // columns behind the row's end count as zero, in both operands
+      const uint32_t keep = (2 * pair + c) * kChunk + ccol < a.row_bytes ? ~0u : 0u;
+      v &= u32x4{keep, keep, keep, keep};
+    }
+    *reinterpret_cast<u32x4*>(cdst + c * Sh::kStage + 32 * i * kChunk) = v;
+  };
+  auto read = [&](int c, int step, int i) {
+    const int to = step & 1;
+    if (i < 4)
+      wf[to][i] = *reinterpret_cast<const u32x4*>(
+          smem + c * Sh::kStage + at(128 * wr + 32 * i + frow, 2 * step + high));
+    else
+      xf[to][i - 4] = *reinterpret_cast<const u32x4*>(
+          smem + c * Sh::kStage + kPanel * kChunk +
+          at(32 * wt + 64 * (i - 4) + col, 2 * step + high));
+  };
+
+  Place cur = next(Place{Work{-1, 0, 0, 0}, 0});
+  if (cur.work.expert >= 0) {
+    aim(cur.work);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int i = 0; i < Sh::kCopies; ++i) load(0, c, i);
+    Place n1 = next(cur);
+    if (n1.pair == 0) aim(n1.work);
+#pragma unroll
+    for (int i = 0; i < Sh::kCopies; ++i) {
+      store(0, 0, i);
+      load(n1.pair, 0, i);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4 + L; ++i) read(0, 0, i);
+    do {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int t = 0; t < L; ++t) acc[g][t] = f32x16{};
+      const Work work = cur.work;
+      for (int pair = 0; pair < pairs; ++pair) {
+        const Place n2 = next(n1);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (c == 1 && n2.pair == 0) aim(n2.work);
+#pragma unroll
+          for (int step = 0; step < 4; ++step)
+#pragma unroll
+            for (int i = 0; i < 2 * L; ++i) {  // two matrix instructions each
+              if (step < 3) {
+#pragma unroll
+                for (int k = i * (4 + L) / (2 * L); k < (i + 1) * (4 + L) / (2 * L); ++k)
+                  read(c, step + 1, k);
+              } else if (i == L) {
+                block_lds_sync();
+#pragma unroll
+                for (int k = 0; k < 4 + L; ++k) read(c ^ 1, 0, k);
+              }
+#pragma unroll
+              for (int m = 2 * i; m < 2 * i + 2; ++m)
+                acc[m % 4][m / 4] = mfma_bf16(wf[step & 1][m % 4], xf[step & 1][m / 4],
+                                              acc[m % 4][m / 4]);
+              // This place's share of the copies, all of them before the barrier:
+              // the next chunk leaves for its stage, and the one that follows it
+              // by two is loaded.
+              constexpr int kPlaces = 7 * L;
+              const int place = 2 * L * step + i;
+              if (place < kPlaces) {
+#pragma unroll
+                for (int k = place * Sh::kCopies / kPlaces;
+                     k < (place + 1) * Sh::kCopies / kPlaces; ++k) {
+                  store(c == 0 ? pair : n1.pair, c ^ 1, k);
+                  load(c == 0 ? n1.pair : n2.pair, c ^ 1, k);
+                }
+              }
+              // (the loads stay here: the compiler would sink them to their use)
+              __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        cur = n1;
+        n1 = n2;
+      }
+      const Outputs o = outputs(a, work.row0, work.rows);
+#pragma unroll
+      for (int t = 0; t < L; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          f32x4 v[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            v[q] = f32x4{acc[g][t][4 * q], acc[g][t][4 * q + 1], acc[g][t][4 * q + 2],
+                         acc[g][t][4 * q + 3]};
+          const int n = work.panel * kPanel + 128 * wr + 32 * g + 16 * high;
+          if (a.out_f32)
+            store_outputs<true, true>(o, 64 * t, 32 * wt + col, n, v);
+          else
+            store_outputs<false, true>(o, 64 * t, 32 * wt + col, n, v);
+        }
+    } while (cur.work.expert >= 0);
+  }
+  if (a.zero_tail) zero_rows(a, tab->last);
+}
+
+template <int L, bool TAIL>
+hipError_t launch_big(const Args& a, hipStream_t st) {
   static std::atomic<uint64_t> done{0};
-  const hipError_t e = allow_lds(&grouped_tile_kernel<FP8, NT, OUT>, Shape<NT>::kLds,
-                                 Shape<NT>::kLds, &done);
+  const hipError_t e = allow_lds(&grouped_big_kernel<L, TAIL>, Big<L>::kLds, Big<L>::kLds,
+                                 &done);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((grouped_tile_kernel<FP8, NT, OUT>), dim3(NT == 16 ? 256 : 512), dim3(256),
-                     Shape<NT>::kLds, st, a);
+  hipLaunchKernelGGL((grouped_big_kernel<L, TAIL>), dim3(256), dim3(256), Big<L>::kLds, st, a);
   return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Block FP8, many rows an expert: 256 weight rows by 256 rows of x
+// ---------------------------------------------------------------------------
+//
+// The same copies, two chunks ahead.  The sums are scaled ones, which the vector
+// units add, so they need vector registers: eight waves (2 x 4) of 128 weight rows
+// (one row of blocks of the weights' scales) by 64 rows of x.  A chunk is one
+// column of blocks and one v_mfma_f32_16x16x128_f8f6f4 a tile of 16 x 16, whose
+// result is scaled into the sums while the next weight rows are multiplied.  MFMA
+// row 4 * a + b of group 4 * c + g is weight row 64 * c + 16 * a + 4 * g + b, so
+// that a lane ends with 16 consecutive outputs of a row of x.
+struct Big8 {
+  static constexpr int kWaves = 8;
+  static constexpr int kToks = 256;
+  static constexpr int kRows = kPanel + kToks;
+  static constexpr int kStage = kRows * kChunk + kToks * 4;  // and the rows' scales
+  static constexpr int kCopies = kRows / 64;  // of a wave, 8 rows each
+  static constexpr int kLds = 2 * kStage + (int)sizeof(Table);
+};
+
+template <bool TAIL>
+__global__ __launch_bounds__(512, 2) void grouped_big_fp8_kernel(const Args a) {
+  using Sh = Big8;
+  extern __shared__ __align__(16) uint8_t smem[];
+  Table* tab = reinterpret_cast<Table*>(smem + 2 * Sh::kStage);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave >> 2, wt = wave & 3;
+  if (wave == 0) fill_table(tab, a, Sh::kToks);
+  __syncthreads();
+  const int npanels = (a.N + kPanel - 1) / kPanel;
+  const int pairs = (a.row_bytes + 2 * kChunk - 1) / (2 * kChunk);  // of chunks
+
+  const int crow = wave * 8 + (lane >> 3), ccol = 16 * (lane & 7);
+  uint8_t* const cdst = smem + at(crow, lane & 7);
+  const int col = lane & 15, quarter = lane >> 4;
+  const int frow = 16 * (col >> 2) + (col & 3);
+
+  struct Place {
+    Work work;
+    int pair;
+  };
+  int turn = 0;
+  auto next = [&](Place p) -> Place {
+    if (p.work.expert >= 0 && ++p.pair < pairs) return p;
+    do {
+      p.work = find_work(tab, work_of(blockIdx.x, turn++), a.E, npanels, Sh::kToks);
+    } while (p.work.expert >= 0 && p.work.rows == 0);
+    p.pair = 0;
+    return p;
+  };
+  const uint8_t *wbase, *xbase;
+  const float *sbase, *wsbase;
+  int wlast, xlast;  // (lane offsets are made from these at each load: no register is left)
+  auto aim = [&](const Work& w) {
+    const int64_t r0 = w.panel * kPanel;
+    const int e = max(w.expert, 0);
+    wbase = uniform(a.w + (w.expert < 0 ? 0 : e * a.w_stride + r0 * a.w_ld));
+    xbase = uniform(a.x + w.row0 * a.x_ld);
+    sbase = (const float*)uniform((const uint8_t*)(a.s + w.row0 * a.s_ld));
+    // (a wave whose weight rows are all behind N scales by the last block)
+    const int block = min((int)(r0 / kBlock) + wr, (a.N - 1) / kBlock);
+    wsbase = (const float*)uniform(
+        (const uint8_t*)(a.ws + e * a.ws_stride + (int64_t)block * a.groups));
+    wlast = w.expert < 0 ? 0 : (int)min(a.N - r0, (int64_t)kPanel) - 1;
+    xlast = max(w.rows, 1) - 1;
+  };
+
+  u32x4 cp[Sh::kCopies];
+  float cs, cws, ws;  // scales on their way: of a row of x, of the weights' block
+  f32x4 acc[8][4];
+  auto load = [&](int pair, int c, int i) {
+    const int o = (2 * pair + c) * kChunk;
+    int row = crow;
+    asm volatile("" : "+v"(row));  // (or the compiler holds both chunks' offsets in registers)
+    const uint8_t* base = i < 4 ? wbase : xbase;
+    const uint32_t at = i < 4 ? __umul24(min(64 * i + row, wlast), (uint32_t)a.w_ld)
+                              : __umul24(min(64 * (i - 4) + row, xlast), (uint32_t)a.x_ld);
+    if constexpr (TAIL)  // (columns behind the row's end: its last ones)
+      cp[i] = load_global(base, at + min(o + ccol, a.row_bytes - 16));
+    else
+      cp[i] = load_global(base + o, at + ccol);
+  };
+  auto load_scales = [&](int pair, int c) {
+    const int g = min(2 * pair + c, a.groups - 1);
+    cs = load_global4((const uint8_t*)(sbase + g),
+                      4 * __umul24(min(tid & (Sh::kToks - 1), xlast), (uint32_t)a.s_ld));
+    cws = load_global4((const uint8_t*)(wsbase + g), 0);
+  };
+  auto store = [&](int pair, int c, int i) {
+    u32x4 v = cp[i];
+    if constexpr (TAIL) {
+      const uint32_t keep = (2 * pair + c) * kChunk + ccol < a.row_bytes ? ~0u : 0u;
+      v &= u32x4{keep, keep, keep, keep};
+    }
+    *reinterpret_cast<u32x4*>(cdst + c * Sh::kStage + 64 * i * kChunk) = v;
+  };
+  auto store_scale = [&](int pair, int c) {
+    // (a chunk behind the row's end has no scales: nothing times zero)
+    if (tid < Sh::kToks)
+      reinterpret_cast<float*>(smem + c * Sh::kStage + Sh::kRows * kChunk)[tid] =
+          !TAIL || 2 * pair + c < a.groups ? cs : 0.f;
+  };
+  // 32 columns a lane: pieces quarter and 4 + quarter (of both operands)
+  u32x4 wf[2], xf[4][2];
+  float xscale[4];
+  auto read_w = [&](int c, int g) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      wf[h] = *reinterpret_cast<const u32x4*>(
+          smem + c * Sh::kStage +
+          at(128 * wr + 64 * (g >> 2) + 4 * (g & 3) + frow, 4 * h + quarter));
+  };
+  auto read_x = [&](int c) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        xf[t][h] = *reinterpret_cast<const u32x4*>(
+            smem + c * Sh::kStage + kPanel * kChunk +
+            at(16 * wt + 64 * t + col, 4 * h + quarter));
+      xscale[t] = reinterpret_cast<const float*>(smem + c * Sh::kStage +
+                                                 Sh::kRows * kChunk)[16 * wt + 64 * t + col];
+    }
+  };
+  auto add = [&](int g, int t, const f32x4& d, float sc) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[g][t][j] = __builtin_fmaf(d[j], sc, acc[g][t][j]);
+    // (here and in vector registers: the compiler would gather a chunk's sums
+    // behind its products, and keep them in accumulation registers between)
+    asm volatile("" : "+v"(acc[g][t]));
+  };
+
+  Place cur = next(Place{Work{-1, 0, 0, 0}, 0});
+  if (cur.work.expert >= 0) {
+    aim(cur.work);
+#pragma unroll
+    for (int i = 0; i < Sh::kCopies; ++i) load(0, 0, i);
+    load_scales(0, 0);
+#pragma unroll
+    for (int i = 0; i < Sh::kCopies; ++i) {
+      store(0, 0, i);
+      load(0, 1, i);
+    }
+    store_scale(0, 0);
+    ws = cws;
+    load_scales(0, 1);
+    __syncthreads();
+    read_x(0);
+    read_w(0, 0);
+    do {
+#pragma unroll
+      for (int g = 0; g < 8; ++g)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[g][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const Work work = cur.work;
+      for (int pair = 0; pair < pairs; ++pair) {
+        // (the chunk after this one is on its way, the one after that is loaded)
+        const Place n1 = next(cur);
+        if (n1.pair == 0) aim(n1.work);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float sc[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) sc[t] = xscale[t] * ws;
+          store_scale(c == 0 ? pair : n1.pair, c ^ 1);
+          ws = cws;
+          load_scales(n1.pair, c);
+          f32x4 d[4];
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              if (g > 0) add(g - 1, t, d[t], sc[t]);
+              d[t] = mfma_fp8(wf[0], wf[1], xf[t][0], xf[t][1]);
+            }
+            if (g < 7) read_w(c, g + 1);  // (the SIMD's other wave multiplies meanwhile)
+            // this group's copy
+            store(c == 0 ? pair : n1.pair, c ^ 1, g);
+            load(n1.pair, c, g);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int t = 0; t < 4; ++t) add(7, t, d[t], sc[t]);
+          block_lds_sync();
+          read_x(c ^ 1);
+          read_w(c ^ 1, 0);
+        }
+        cur = n1;
+      }
+      const Outputs o = outputs(a, work.row0, work.rows);
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const f32x4 v[4] = {acc[4 * c][t], acc[4 * c + 1][t], acc[4 * c + 2][t],
+                              acc[4 * c + 3][t]};
+          store_outputs<false, true>(o, 64 * t, 16 * wt + col,
+                               work.panel * kPanel + 128 * wr + 64 * c + 16 * quarter, v);
+        }
+    } while (cur.work.expert >= 0);
+  }
+  if (a.zero_tail) zero_rows(a, tab->last);
+}
+
+template <bool TAIL>
+hipError_t launch_big_fp8(const Args& a, hipStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  const hipError_t e = allow_lds(&grouped_big_fp8_kernel<TAIL>, Big8::kLds, Big8::kLds, &done);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((grouped_big_fp8_kernel<TAIL>), dim3(256), dim3(64 * Big8::kWaves), Big8::kLds, st, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// The fewest rows: 16 weight rows a block, the columns split over its waves
+// ---------------------------------------------------------------------------
+//
+// One token's experts have too few panels to fill the GPU: 8 of Qwen3's w13 have
+// 192 of 64 rows.  A block takes 16 weight rows of one group and each of its
+// waves a fourth of the columns, whose loads are all in flight at once (kBatch
+// chunks of both operands); the partial sums meet in LDS, in wave order.  Blocks go
+// to the groups in use by their number: j-th in y, which ends name.  Qwen3 w13, one
+// token: 17.2 us with the tiles, 12.4 so.
+constexpr int kFewCols = 16;  // rows of x a pass
+
+template <bool FP8, int kBatch>
+__global__ __launch_bounds__(256) void grouped_few_kernel(const Args a) {
+  __shared__ float part[kWaves][16][kFewCols + 1];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, quarter = lane >> 4;
+
+  // The group: the blockIdx.y-th of those with rows (every wave finds it).
+  int expert = -1, row0 = 0, rows = 0, top = 0, seen = 0;
+  for (int e0 = 0; e0 < a.E; e0 += 64) {
+    int end = e0 + lane < a.E ? min(max(a.ends[e0 + lane], 0), a.M) : 0;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(end, d);
+      end = lane >= d ? max(end, o) : end;
+    }
+    end = max(end, top);
+    const int before = __shfl_up(end, 1), start = lane ? before : top;
+    const uint64_t some = __ballot(end > start);
+    const int at = (int)blockIdx.y - seen;  // among these
+    const uint64_t mine = __ballot(end > start && __popcll(some & ((1ull << lane) - 1)) == at);
+    if (mine) {
+      const int l = __builtin_ctzll(mine);
+      expert = e0 + l;
+      row0 = __builtin_amdgcn_readlane(start, l);
+      rows = __builtin_amdgcn_readlane(end, l) - row0;
+    }
+    seen += __popcll(some);
+    top = __builtin_amdgcn_readlane(end, 63);
+  }
+  if (rows > 0) {
+    const int n0 = blockIdx.x * 16;
+    const int chunks = (a.row_bytes + kChunk - 1) / kChunk;
+    const int c0 = chunks * wave / kWaves, c1 = chunks * (wave + 1) / kWaves;
+    const uint8_t* w = a.w + expert * a.w_stride + min(n0 + col, a.N - 1) * a.w_ld;
+    const float* ws = FP8 ? a.ws + expert * a.ws_stride + (int64_t)(n0 / kBlock) * a.groups
+                          : nullptr;
+    for (int m0 = 0; m0 < rows; m0 += kFewCols) {
+      const int64_t r = row0 + min(m0 + col, rows - 1);
+      const uint8_t* x = a.x + r * a.x_ld;
+      const float* s = FP8 ? a.s + r * a.s_ld : nullptr;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      for (int c = c0; c < c1; c += kBatch) {
+        u32x4 wf[kBatch][2], xf[kBatch][2];
+        float sc[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int at = min(c + i, c1 - 1);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int o = min(at * kChunk + 64 * h + 16 * quarter, a.row_bytes - 16);
+            wf[i][h] = *reinterpret_cast<const u32x4*>(w + o);
+            xf[i][h] = *reinterpret_cast<const u32x4*>(x + o);
+          }
+          if constexpr (FP8) sc[i] = s[at] * ws[at];
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          if (c + i >= c1) break;
+          // columns behind the row's end count as zero, in both operands
+          const int left = a.row_bytes - (c + i) * kChunk;
+          if (left < kChunk) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (64 * h + 16 * quarter >= left) wf[i][h] = xf[i][h] = u32x4{0, 0, 0, 0};
+          }
+          if constexpr (FP8) {
+            const f32x4 d = mfma_fp8(wf[i][0], wf[i][1], xf[i][0], xf[i][1]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] = __builtin_fmaf(d[j], sc[i], acc[j]);
+          } else {
+            acc = mfma_bf16(wf[i][0], xf[i][0], acc);
+            acc = mfma_bf16(wf[i][1], xf[i][1], acc);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part[wave][4 * quarter + j][col] = acc[j];
+      __syncthreads();
+      const int n = threadIdx.x & 15, m = threadIdx.x >> 4;
+      float v = part[0][n][m];
+#pragma unroll
+      for (int i = 1; i < kWaves; ++i) v += part[i][n][m];
+      if (n0 + n < a.N && m0 + m < rows) {
+        const int64_t at = (int64_t)(row0 + m0 + m) * a.N + n0 + n;
+        if (a.out_f32)
+          ((float*)a.out)[at] = v;
+        else
+          ((uint16_t*)a.out)[at] = bf16_rne(v);
+      }
+      __syncthreads();
+    }
+  }
+  if (a.zero_tail && blockIdx.y == 0) zero_rows(a, top);
+}
+
+template <bool FP8, int kBatch>
+hipError_t launch_few(const Args& a, hipStream_t st) {
+  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)std::min(a.M, a.E));
+  hipLaunchKernelGGL((grouped_few_kernel<FP8, kBatch>), grid, dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+template <bool FP8>
+hipError_t launch_few(const Args& a, hipStream_t st) {
+  // a wave's chunks in as few batches as registers allow, the last one full (what
+  // it lacks is loaded all the same: Qwen3 w2, 3 chunks a wave in a batch of 8, 13.8
+  // us, of 3 FEW3)
+  const int per = ((a.row_bytes + kChunk - 1) / kChunk + kWaves - 1) / kWaves;
+  if (per <= 2) return launch_few<FP8, 2>(a, st);
+  if (per == 3 || per == 5 || per == 6) return launch_few<FP8, 3>(a, st);
+  if (FP8 || per == 4) return launch_few<FP8, 4>(a, st);
+  return launch_few<FP8, FP8 ? 4 : 8>(a, st);
+}
+
+template <bool FP8, int G, Out OUT>
+hipError_t launch_tile(const Args& a, hipStream_t st) {
+  using Sh = Shape<4, G>;
+  static_assert(Sh::kLds <= 64 * 1024, "LDS beyond the default limit");
+  hipLaunchKernelGGL((grouped_tile_kernel<FP8, 4, G, OUT>), dim3(256 * (G == 4 ? 2 : G == 2 ? 3 : 4)), dim3(256), Sh::kLds, st, a);
+  return hipGetLastError();
+}
+
+template <bool FP8, Out OUT>
+hipError_t launch_tile(const Args& a, hipStream_t st) {
+  // the largest panels that give every CU two blocks
+  const int64_t used = std::min(a.M, a.E);
+  if (used * ((a.N + 255) / 256) >= 768) return launch_tile<FP8, 4, OUT>(a, st);
+  if (used * ((a.N + 127) / 128) >= 768) return launch_tile<FP8, 2, OUT>(a, st);
+  return launch_tile<FP8, 1, OUT>(a, st);
 }
 
 int refuse(int rc, const char* why, const char* where) {
@@ -521,26 +1115,41 @@ int refuse(int rc, const char* why, const char* where) {
   return rc;
 }
 
-template <bool FP8, Out OUT>
-hipError_t launch_of(const Args& a, hipStream_t st) {
-  // rows an expert has if the rows are spread evenly
+template <int L>
+hipError_t launch_big(const Args& a, hipStream_t st) {
+  return a.row_bytes % (2 * kChunk) ? launch_big<L, true>(a, st) : launch_big<L, false>(a, st);
+}
+
+template <bool FP8>
+hipError_t launch(const Args& a, hipStream_t st) {
+  if (a.M <= 32 || (a.M <= 64 && std::min(a.M, a.E) * (int64_t)((a.N + 255) / 256) <= 128))
+    return launch_few<FP8>(a, st);
+  // single values are stored by the small tiles only
+  if (a.N % (a.out_f32 ? 4 : 8)) return launch_tile<FP8, kNarrow>(a, st);
+  // rows an expert has if they are spread evenly
   const int per = a.M / a.E;
-  if constexpr (!FP8) {
-    if (per > 128) return launch_tile<false, 16, OUT>(a, st);
+  if constexpr (FP8) {
+    if (per > 56)
+      return a.row_bytes % (2 * kChunk) ? launch_big_fp8<true>(a, st) : launch_big_fp8<false>(a, st);
+    return launch_tile<true, kBf16>(a, st);
+  } else {
+    // Tiles of 64 weight rows (few rows an expert: one stream of the weights) up to
+    // 56 rows an expert, then large ones of the height that takes the least
+    // time: the rows, and their square root more, in tiles of 30 + 40 L.  Qwen3
+    // w13 of 128 experts at 48, 64, 128, 512 rows each: 183, 203, 282, 700 us in
+    // the first, 189, 192, 222, 479 in tiles of 128 rows, 195, 198, 210, 437 in 192.
+    if (per > 56) {
+      const int m = per + (int)sqrtf((float)per);
+      return (m + 127) / 128 * 110 <= (m + 191) / 192 * 150 ? launch_big<2>(a, st)
+                                                            : launch_big<3>(a, st);
+    }
+    return a.out_f32 ? launch_tile<false, kF32>(a, st) : launch_tile<false, kBf16>(a, st);
   }
-  return launch_tile<FP8, 4, OUT>(a, st);
 }
 
 template <bool FP8>
 int grouped(const Args& a, hipStream_t st) {
-  hipError_t e;
-  if (a.N % (a.out_f32 ? 4 : 8))
-    e = launch_tile<FP8, 4, kNarrow>(a, st);
-  else if (a.out_f32)
-    e = launch_of<false, kF32>(a, st);
-  else
-    e = launch_of<FP8, kBf16>(a, st);
-  WISP_HIP_TRY(e);
+  WISP_HIP_TRY(launch<FP8>(a, st));
   return WISP_OK;
 }
 
@@ -552,8 +1161,9 @@ const char* unsupported(int64_t x_ld, int64_t w_ld, int64_t w_stride, int64_t N,
       (uintptr_t)w % 16)
     return "x, w and their strides must be 16-byte aligned";
   // (32-bit offsets inside a tile of x and inside an expert's weights)
-  if (N * w_ld * elem >= (int64_t)1 << 31 || x_ld * elem >= (int64_t)1 << 22 || N >= 1 << 21)
-    return "an expert's weights of 2 GiB, rows of x 4 MiB apart or 2^21 outputs";
+  if (N * w_ld * elem >= (int64_t)1 << 31 || w_ld * elem >= (int64_t)1 << 24 ||
+      x_ld * elem >= (int64_t)1 << 22 || N >= 1 << 21)
+    return "an expert's weights of 2 GiB, rows of w 16 MiB or of x 4 MiB apart, or 2^21 outputs";
   return nullptr;
 }
 
