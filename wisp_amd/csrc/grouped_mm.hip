@@ -221,6 +221,32 @@ __device__ inline int work_of(int b, int j) {
   return ((i / kRun) * 8 + (b & 7)) * kRun + i % kRun;
 }
 
+// A pair of chunks of a work, left of them to go with this one.
+struct Place {
+  Work work;
+  int pair, left;
+};
+__device__ inline Place nowhere() { return Place{Work{-1, 0, 0, 0}, 0, 0}; }
+
+// The pairs of a block's works, one after the other.  Each panel starts at a pair
+// of its own and wraps around: blocks that all start at column 0 crowd a few
+// memory channels (Qwen3 w13 of 512 tokens: 179 us, so 147; 1024 tokens 194, 162).
+template <int TOKS>
+struct Walk {
+  const Table* tab;
+  int E, npanels, pairs, turn;
+  __device__ __attribute__((always_inline)) inline Place next(Place p) {
+    p.pair = p.pair + 1 == pairs ? 0 : p.pair + 1;
+    if (--p.left > 0) return p;
+    do {
+      p.work = find_work(tab, work_of(blockIdx.x, turn++), E, npanels, TOKS);
+    } while (p.work.expert >= 0 && p.work.rows == 0);
+    p.pair = p.work.expert < 0 ? 0 : (int)((int64_t)p.work.panel * pairs / npanels);
+    p.left = pairs;
+    return p;
+  }
+};
+
 // Zeros into the rows behind the last group, all blocks (of a grid in x) together.
 __device__ inline void zero_rows(const Args& a, int last) {
   const int64_t wide = a.out_f32 ? 4 : 2;
@@ -341,25 +367,9 @@ __global__ __launch_bounds__(256, 2) void grouped_tile_kernel(const Args a) {
   const int xrow = wave * 8 + (lane >> 3);
   const int xvoff = xrow * (int)a.x_ld + 16 * (lane & 7);
 
-  // The three places in flight (computed, weights loading, rows loading): a pair of
-  // chunks of a work, left to go with those behind it.  Each panel starts at a
-  // place of its own and wraps around: blocks that all start at column 0 crowd
-  // a few memory channels (Qwen3 w13, 512 tokens: 179 us, so 147).
-  struct Place {
-    Work work;
-    int pair, left;
-  };
-  int turn = 0;
-  auto next = [&](Place p) -> Place {
-    p.pair = p.pair + 1 == pairs ? 0 : p.pair + 1;
-    if (--p.left > 0) return p;
-    do {
-      p.work = find_work(tab, work_of(blockIdx.x, turn++), a.E, npanels, Sh::kToks);
-    } while (p.work.expert >= 0 && p.work.rows == 0);
-    p.pair = p.work.expert < 0 ? 0 : (int)((int64_t)p.work.panel * pairs / npanels);
-    p.left = pairs;
-    return p;
-  };
+  // (three places in flight: computed, weights loading, rows loading)
+  Walk<Sh::kToks> walk{tab, a.E, npanels, pairs, 0};
+  auto next = [&](const Place& p) { return walk.next(p); };
 
   u32x4 wf[2][2][G];            // [chunk of a pair][half of it][group]
   u32x4 xs[2][Sh::kCopies];
@@ -473,7 +483,7 @@ __global__ __launch_bounds__(256, 2) void grouped_tile_kernel(const Args a) {
     }
   };
 
-  Place cur = next(Place{Work{-1, 0, 0, 0}, 0, 0});
+  Place cur = next(nowhere());
   if (cur.work.expert >= 0) {
     load_x(cur);
     load_w(cur, 0);
@@ -590,20 +600,8 @@ __global__ __launch_bounds__(256, 1) void grouped_big_kernel(const Args a) {
   const int col = lane & 31, high = lane >> 5;
   const int frow = 16 * (col >> 2 & 1) + 4 * (col >> 3) + (col & 3);
 
-  // a pair of chunks of a work
-  struct Place {
-    Work work;
-    int pair;
-  };
-  int turn = 0;
-  auto next = [&](Place p) -> Place {
-    if (p.work.expert >= 0 && ++p.pair < pairs) return p;
-    do {
-      p.work = find_work(tab, work_of(blockIdx.x, turn++), a.E, npanels, Sh::kToks);
-    } while (p.work.expert >= 0 && p.work.rows == 0);
-    p.pair = 0;
-    return p;
-  };
+  Walk<Sh::kToks> walk{tab, a.E, npanels, pairs, 0};
+  auto next = [&](const Place& p) { return walk.next(p); };
   // Where a work's rows start, and this lane's offsets of its copies from there;
   // rows behind the last are that one again (what they give is not stored).
   const uint8_t *wbase, *xbase;
@@ -656,18 +654,18 @@ __global__ __launch_bounds__(256, 1) void grouped_big_kernel(const Args a) {
           at(32 * wt + 64 * (i - 4) + col, 2 * step + high));
   };
 
-  Place cur = next(Place{Work{-1, 0, 0, 0}, 0});
+  Place cur = next(nowhere());
   if (cur.work.expert >= 0) {
     aim(cur.work);
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int i = 0; i < Sh::kCopies; ++i) load(0, c, i);
+      for (int i = 0; i < Sh::kCopies; ++i) load(cur.pair, c, i);
     Place n1 = next(cur);
-    if (n1.pair == 0) aim(n1.work);
+    if (n1.left == pairs) aim(n1.work);
 #pragma unroll
     for (int i = 0; i < Sh::kCopies; ++i) {
-      store(0, 0, i);
+      store(cur.pair, 0, i);
       load(n1.pair, 0, i);
     }
     __syncthreads();
@@ -683,7 +681,7 @@ __global__ __launch_bounds__(256, 1) void grouped_big_kernel(const Args a) {
         const Place n2 = next(n1);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          if (c == 1 && n2.pair == 0) aim(n2.work);
+          if (c == 1 && n2.left == pairs) aim(n2.work);
 #pragma unroll
           for (int step = 0; step < 4; ++step)
 #pragma unroll
@@ -710,7 +708,7 @@ __global__ __launch_bounds__(256, 1) void grouped_big_kernel(const Args a) {
 #pragma unroll
                 for (int k = place * Sh::kCopies / kPlaces;
                      k < (place + 1) * Sh::kCopies / kPlaces; ++k) {
-                  store(c == 0 ? pair : n1.pair, c ^ 1, k);
+                  store(c == 0 ? cur.pair : n1.pair, c ^ 1, k);
                   load(c == 0 ? n1.pair : n2.pair, c ^ 1, k);
                 }
               }
@@ -790,19 +788,8 @@ __global__ __launch_bounds__(512, 2) void grouped_big_fp8_kernel(const Args a) {
   const int col = lane & 15, quarter = lane >> 4;
   const int frow = 16 * (col >> 2) + (col & 3);
 
-  struct Place {
-    Work work;
-    int pair;
-  };
-  int turn = 0;
-  auto next = [&](Place p) -> Place {
-    if (p.work.expert >= 0 && ++p.pair < pairs) return p;
-    do {
-      p.work = find_work(tab, work_of(blockIdx.x, turn++), a.E, npanels, Sh::kToks);
-    } while (p.work.expert >= 0 && p.work.rows == 0);
-    p.pair = 0;
-    return p;
-  };
+  Walk<Sh::kToks> walk{tab, a.E, npanels, pairs, 0};
+  auto next = [&](const Place& p) { return walk.next(p); };
   const uint8_t *wbase, *xbase;
   const float *sbase, *wsbase;
   int wlast, xlast;  // (lane offsets are made from these at each load: no register is left)
@@ -885,20 +872,20 @@ __global__ __launch_bounds__(512, 2) void grouped_big_fp8_kernel(const Args a) {
     asm volatile("" : "+v"(acc[g][t]));
   };
 
-  Place cur = next(Place{Work{-1, 0, 0, 0}, 0});
+  Place cur = next(nowhere());
   if (cur.work.expert >= 0) {
     aim(cur.work);
 #pragma unroll
-    for (int i = 0; i < Sh::kCopies; ++i) load(0, 0, i);
-    load_scales(0, 0);
+    for (int i = 0; i < Sh::kCopies; ++i) load(cur.pair, 0, i);
+    load_scales(cur.pair, 0);
 #pragma unroll
     for (int i = 0; i < Sh::kCopies; ++i) {
-      store(0, 0, i);
-      load(0, 1, i);
+      store(cur.pair, 0, i);
+      load(cur.pair, 1, i);
     }
-    store_scale(0, 0);
+    store_scale(cur.pair, 0);
     ws = cws;
-    load_scales(0, 1);
+    load_scales(cur.pair, 1);
     __syncthreads();
     read_x(0);
     read_w(0, 0);
@@ -911,13 +898,13 @@ __global__ __launch_bounds__(512, 2) void grouped_big_fp8_kernel(const Args a) {
       for (int pair = 0; pair < pairs; ++pair) {
         // (the chunk after this one is on its way, the one after that is loaded)
         const Place n1 = next(cur);
-        if (n1.pair == 0) aim(n1.work);
+        if (n1.left == pairs) aim(n1.work);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float sc[4];
 #pragma unroll
           for (int t = 0; t < 4; ++t) sc[t] = xscale[t] * ws;
-          store_scale(c == 0 ? pair : n1.pair, c ^ 1);
+          store_scale(c == 0 ? cur.pair : n1.pair, c ^ 1);
           ws = cws;
           load_scales(n1.pair, c);
           f32x4 d[4];
@@ -930,7 +917,7 @@ __global__ __launch_bounds__(512, 2) void grouped_big_fp8_kernel(const Args a) {
             }
             if (g < 7) read_w(c, g + 1);  // (the SIMD's other wave multiplies meanwhile)
             // this group's copy
-            store(c == 0 ? pair : n1.pair, c ^ 1, g);
+            store(c == 0 ? cur.pair : n1.pair, c ^ 1, g);
             load(n1.pair, c, g);
             __builtin_amdgcn_sched_barrier(0);
           }
@@ -1129,7 +1116,9 @@ hipError_t launch(const Args& a, hipStream_t st) {
   // rows an expert has if they are spread evenly
   const int per = a.M / a.E;
   if constexpr (FP8) {
-    if (per > 56)
+    // (Qwen3 w13 at 64, 96, 128 rows an expert: 113, 128, 158 us in the tiles of the
+    // weights' stream, 117, 120, 124 in the large ones)
+    if (per > 88)
       return a.row_bytes % (2 * kChunk) ? launch_big_fp8<true>(a, st) : launch_big_fp8<false>(a, st);
     return launch_tile<true, kBf16>(a, st);
   } else {
