@@ -31,19 +31,21 @@ from .rows_fp8 import FP8, GROUP, _DTYPES, _check_apart, _on_device, _stream
 
 def _sizes(x, w, ends) -> tuple[int, int, int, int]:
     """``(M, E, N, K)`` of rows, weights and ends."""
-    if x.dim() != 2 or w.dim() != 3 or ends.dim() != 1 or w.shape[2] != x.shape[1] or \
-            ends.shape[0] != w.shape[0] or not w.shape[0]:
+    if x.dim() != 2 or w.dim() != 3 or ends.dim() != 1:
+        raise ValueError("wisp: grouped products take rows [M, K], weights [E, N, K] and ends [E]")
+    (M, C), (E, N, K), (groups,) = x.shape, w.shape, ends.shape
+    if K != C or groups != E or not E:
         raise ValueError("wisp: grouped products take rows [M, K], weights [E, N, K] and ends "
-                         f"[E], got {tuple(x.shape)}, {tuple(w.shape)}, {tuple(ends.shape)}")
+                         f"[E], got {(M, C)}, {(E, N, K)}, {(groups,)}")
     if ends.dtype != torch.int32:
         raise ValueError("wisp: ends are int32")
     dev = x.get_device()
-    for t, name in ((w, "w"), (ends, "ends")):
-        if t.get_device() != dev:
-            _require_device(t, x.device, name)
-    if w.stride(2) != 1 and w.shape[2] > 1:
+    if w.get_device() != dev or ends.get_device() != dev:
+        _require_device(w, x.device, "w")
+        _require_device(ends, x.device, "ends")
+    if K > 1 and w.stride(2) != 1:
         raise ValueError("wisp: each row of w must be contiguous")
-    return x.shape[0], w.shape[0], w.shape[1], w.shape[2]
+    return M, E, N, K
 
 
 def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
@@ -58,7 +60,7 @@ def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
 
 def _output(x, N, dtype, out, inputs) -> torch.Tensor:
     if out is None:
-        return torch.empty((x.shape[0], N), dtype=dtype, device=x.device)
+        return x.new_empty((x.shape[0], N), dtype=dtype)
     if out.shape != (x.shape[0], N) or out.dtype != dtype or not out.is_contiguous():
         raise ValueError(f"wisp: out must be a contiguous {(x.shape[0], N)} {dtype} tensor")
     if out.get_device() != x.get_device():
@@ -84,9 +86,11 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, *,
     given = out is not None
     out = _output(x, N, dtype, out, (x, ends) if given else ())
     if M and N:
-        check(lib().wisp_grouped_mm(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
-                                    w.stride(1), ends.data_ptr(), E, M, N, K, out.data_ptr(),
-                                    _DTYPES[dtype], int(not given), _stream(x)), "grouped_mm")
+        rc = lib().wisp_grouped_mm(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
+                                   w.stride(1), ends.data_ptr(), E, M, N, K, out.data_ptr(),
+                                   _DTYPES[dtype], not given, _stream(x))
+        if rc:
+            check(rc, "grouped_mm")
     return out
 
 
@@ -107,10 +111,10 @@ def grouped_mm_fp8(q: torch.Tensor, s: torch.Tensor, w: torch.Tensor, ws: torch.
     if s.shape != (M, G) or ws.shape != (E, B, G) or s.dtype != torch.float32 or \
             ws.dtype != torch.float32:
         raise ValueError(f"wisp: scales are float32, s {(M, G)} and ws {(E, B, G)}")
-    for t, name in ((s, "s"), (ws, "ws")):
-        if t.get_device() != q.get_device():
-            _require_device(t, q.device, name)
-    if E and B and G and not ws[0].is_contiguous():
+    if s.get_device() != q.get_device() or ws.get_device() != q.get_device():
+        _require_device(s, q.device, "s")
+        _require_device(ws, q.device, "ws")
+    if not ws.is_contiguous() and not ws[0].is_contiguous():
         raise ValueError("wisp: each expert's block scales must be contiguous")
     q, ends = _aligned_rows(q), ends.contiguous()
     if (s.stride(1) != 1 and G > 1) or s.stride(0) < G:
@@ -118,10 +122,12 @@ def grouped_mm_fp8(q: torch.Tensor, s: torch.Tensor, w: torch.Tensor, ws: torch.
     given = out is not None
     out = _output(q, N, torch.bfloat16, out, (q, s, ends) if given else ())
     if M and N:
-        check(lib().wisp_grouped_mm_fp8(
+        rc = lib().wisp_grouped_mm_fp8(
             q.data_ptr(), q.stride(0), s.data_ptr(), s.stride(0), w.data_ptr(), w.stride(0),
             w.stride(1), ws.data_ptr(), ws.stride(0), ends.data_ptr(), E, M, N, K, out.data_ptr(),
-            int(not given), _stream(q)), "grouped_mm_fp8")
+            not given, _stream(q))
+        if rc:
+            check(rc, "grouped_mm_fp8")
     return out
 
 

@@ -83,64 +83,71 @@ def _check_apart(name: str, t: torch.Tensor, others) -> None:
             raise ValueError(f"wisp: {name} overlaps another tensor of the call")
 
 
-def _norm(x, weight, eps, residual, residual_out, out, want_out, want_fp8):
+def _check_norm(x, weight, residual, residual_out, out):
+    """Raises for what the call does not take."""
     if x.dim() != 2 or weight.dim() != 1 or weight.shape[0] != x.shape[1]:
         raise ValueError("wisp: x is [rows, cols] and weight [cols]")
     if x.dtype not in _DTYPES:
         raise NotImplementedError(f"wisp: rows of {x.dtype} (float32 and bfloat16)")
-    dev = x.get_device()
-    for t in (weight, residual):
-        if t is None:
-            continue
-        if t.dtype != x.dtype and t.dtype != torch.float32:
+    for t, name in ((weight, "weight"), (residual, "residual")):
+        if t is not None and t.dtype != x.dtype and t.dtype != torch.float32:
             raise NotImplementedError("wisp: weight and residual are of x's type or float32")
-        if t.get_device() != dev:
-            _require_device(t, x.device, "weight" if t is weight else "residual")
+    for t, name in ((weight, "weight"), (residual, "residual"), (residual_out, "residual_out"),
+                    (out, "out")):
+        if t is not None:
+            _require_device(t, x.device, name)
+    if residual is None:
+        if residual_out is not None:
+            raise ValueError("wisp: residual_out without a residual")
+    elif residual.shape != x.shape:
+        raise ValueError(f"wisp: residual must be {tuple(x.shape)}")
     rows, cols = x.shape
-    x, weight = _rows(x), weight.contiguous()
-    res = None
-    if residual is not None:
-        if residual.shape != x.shape:
-            raise ValueError(f"wisp: residual must be {tuple(x.shape)}")
-        res = _rows(residual)
-        if residual_out is None:
-            residual_out = torch.empty_like(x, dtype=residual.dtype,
-                                            memory_format=torch.contiguous_format)
-        else:
-            if residual_out.shape != x.shape or residual_out.dtype != residual.dtype or \
-                    (cols > 1 and residual_out.stride(1) != 1) or \
-                    (rows > 1 and residual_out.stride(0) < cols):
-                raise ValueError(f"wisp: residual_out must be {tuple(x.shape)} {residual.dtype} "
-                                 "with contiguous rows")
-            if residual_out.get_device() != dev:
-                _require_device(residual_out, x.device, "residual_out")
-            _check_apart("residual_out", residual_out,
-                         ((x, True), (res, True), (weight, False)))
-    elif residual_out is not None:
-        raise ValueError("wisp: residual_out without a residual")
+    if residual_out is not None:
+        if residual_out.shape != x.shape or residual_out.dtype != residual.dtype or \
+                (cols > 1 and residual_out.stride(1) != 1) or \
+                (rows > 1 and residual_out.stride(0) < cols):
+            raise ValueError(f"wisp: residual_out must be {tuple(x.shape)} {residual.dtype} "
+                             "with contiguous rows")
+        _check_apart("residual_out", residual_out, ((x, True), (residual, True), (weight, False)))
     if out is not None:
         if out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
             raise ValueError(f"wisp: out must be a contiguous {tuple(x.shape)} {x.dtype} tensor")
-        if out.get_device() != dev:
-            _require_device(out, x.device, "out")
-        _check_apart("out", out, ((x, True), (res, True), (weight, False),
+        _check_apart("out", out, ((x, True), (residual, True), (weight, False),
                                   (residual_out, False)))
-    elif want_out:
-        out = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-    q = s = None
-    if want_fp8:
-        q = torch.empty((rows, cols), dtype=FP8, device=x.device)
-        s = torch.empty((rows, -(-cols // GROUP)), dtype=torch.float32, device=x.device)
+
+
+def _norm(x, weight, eps, residual, residual_out, out, q, s):
+    """The call: checks, then one launch.  (The common call is recognised first:
+    the checks take microseconds, as long as a small call's kernel.)"""
+    dtype, dev = x.dtype, x.get_device()
+    if residual_out is not None or out is not None or x.dim() != 2 or dtype not in _DTYPES or \
+            weight.dtype != dtype or weight.get_device() != dev or \
+            weight.shape != x.shape[1:] or (residual is not None and (
+                residual.dtype != dtype or residual.get_device() != dev or
+                residual.shape != x.shape)):
+        _check_norm(x, weight, residual, residual_out, out)
+    rows, cols = x.shape
+    # (a copy of rows that are not contiguous comes after the check for overlaps)
+    x, weight = _rows(x), weight.contiguous()
+    if out is None and not q:
+        out = x.new_empty((rows, cols))
+    if q:
+        q = x.new_empty((rows, cols), dtype=FP8)
+        s = x.new_empty((rows, -(-cols // GROUP)), dtype=torch.float32)
+    r = rdt = rs = ro = ros = 0
+    if residual is not None:
+        residual = _rows(residual)
+        if residual_out is None:
+            residual_out = residual.new_empty((rows, cols))
+        r, rdt, rs = residual.data_ptr(), _DTYPES[residual.dtype], residual.stride(0)
+        ro, ros = residual_out.data_ptr(), residual_out.stride(0)
     if rows and cols:
-        check(lib().wisp_add_rms_norm(
-            x.data_ptr(), _DTYPES[x.dtype], rows, cols, x.stride(0),
-            None if res is None else res.data_ptr(),
-            0 if res is None else _DTYPES[res.dtype], 0 if res is None else res.stride(0),
-            None if res is None else residual_out.data_ptr(),
-            0 if res is None else residual_out.stride(0),
-            weight.data_ptr(), _DTYPES[weight.dtype], eps,
-            None if out is None else out.data_ptr(), None if q is None else q.data_ptr(),
-            None if s is None else s.data_ptr(), _stream(x)), "add_rms_norm")
+        rc = lib().wisp_add_rms_norm(
+            x.data_ptr(), _DTYPES[dtype], rows, cols, x.stride(0), r, rdt, rs, ro, ros,
+            weight.data_ptr(), _DTYPES[weight.dtype], eps, 0 if out is None else out.data_ptr(),
+            q.data_ptr() if s is not None else 0, s.data_ptr() if s is not None else 0, _stream(x))
+        if rc:
+            check(rc, "add_rms_norm")
     return out, q, s, residual_out
 
 
@@ -155,7 +162,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     the residual are of ``x``'s type or float32.  Rows may lie any distance
     apart; up to 32768 columns.  ``out`` may be ``x`` or ``residual``, and
     ``residual_out`` may be ``residual`` or ``x``, but not one the other."""
-    out, _, _, residual_out = _norm(x, weight, eps, residual, residual_out, out, True, False)
+    out, _, _, residual_out = _norm(x, weight, eps, residual, residual_out, out, False, None)
     return out, residual_out
 
 
@@ -166,7 +173,7 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     """:func:`add_rms_norm` in 8 bits: ``(codes, scales, residual_out)``.  With
     ``out`` the normalised rows also go there in ``x``'s type (for a router
     that reads them), from the same float32 values."""
-    _, q, s, residual_out = _norm(x, weight, eps, residual, residual_out, out, False, True)
+    _, q, s, residual_out = _norm(x, weight, eps, residual, residual_out, out, True, None)
     return q, s, residual_out
 
 
@@ -181,11 +188,13 @@ def silu_mul_fp8(h: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise NotImplementedError(f"wisp: rows of {h.dtype} (float32 and bfloat16)")
     h = _rows(h)
     rows, inter = h.shape[0], h.shape[1] // 2
-    q = torch.empty((rows, inter), dtype=FP8, device=h.device)
-    s = torch.empty((rows, -(-inter // GROUP)), dtype=torch.float32, device=h.device)
+    q = h.new_empty((rows, inter), dtype=FP8)
+    s = h.new_empty((rows, -(-inter // GROUP)), dtype=torch.float32)
     if rows and inter:
-        check(lib().wisp_silu_mul_fp8(h.data_ptr(), _DTYPES[h.dtype], rows, inter, h.stride(0),
-                                      q.data_ptr(), s.data_ptr(), _stream(h)), "silu_mul_fp8")
+        rc = lib().wisp_silu_mul_fp8(h.data_ptr(), _DTYPES[h.dtype], rows, inter, h.stride(0),
+                                     q.data_ptr(), s.data_ptr(), _stream(h))
+        if rc:
+            check(rc, "silu_mul_fp8")
     return q, s
 
 

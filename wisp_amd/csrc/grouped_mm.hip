@@ -1113,25 +1113,27 @@ hipError_t launch(const Args& a, hipStream_t st) {
     return launch_few<FP8>(a, st);
   // single values are stored by the small tiles only
   if (a.N % (a.out_f32 ? 4 : 8)) return launch_tile<FP8, kNarrow>(a, st);
-  // rows an expert has if they are spread evenly
+  // rows an expert has if they are spread evenly, and its panels of 256
   const int per = a.M / a.E;
+  const int64_t panels = (int64_t)a.E * ((a.N + kPanel - 1) / kPanel);
+  // Tiles of the weights' stream while the experts have few rows (or the large ones
+  // would leave CUs idle: Qwen3 w2 of 16 experts, 60 rows each, 128 works, 21.6 us,
+  // 16.7 in tiles of 64 weight rows), then large ones.
   if constexpr (FP8) {
-    // (Qwen3 w13 at 64, 96, 128 rows an expert: 113, 128, 158 us in the tiles of the
-    // weights' stream, 117, 120, 124 in the large ones)
-    if (per > 88)
+    // Qwen3 w13 of 128 experts at 64, 96, 128 rows each: 113, 128, 158 us in the
+    // first, 117, 120, 124 in the large ones.
+    if (per > 88 && panels * ((per + 255) / 256) >= 192)
       return a.row_bytes % (2 * kChunk) ? launch_big_fp8<true>(a, st) : launch_big_fp8<false>(a, st);
     return launch_tile<true, kBf16>(a, st);
   } else {
-    // Tiles of 64 weight rows (few rows an expert: one stream of the weights) up to
-    // 56 rows an expert, then large ones of the height that takes the least
-    // time: the rows, and their square root more, in tiles of 30 + 40 L.  Qwen3
-    // w13 of 128 experts at 48, 64, 128, 512 rows each: 183, 203, 282, 700 us in
-    // the first, 189, 192, 222, 479 in tiles of 128 rows, 195, 198, 210, 437 in 192.
-    if (per > 56) {
-      const int m = per + (int)sqrtf((float)per);
-      return (m + 127) / 128 * 110 <= (m + 191) / 192 * 150 ? launch_big<2>(a, st)
-                                                            : launch_big<3>(a, st);
-    }
+    // Of two heights the one that takes less: the rows, and their square root more, in
+    // tiles of 30 + 40 L.  Qwen3 w13 at 48, 64, 128, 187, 512 rows an expert: 183, 203,
+    // 282, 362, 841 us in the first, 189, 192, 222, 253, 479 in tiles of 128 rows, 195, 198,
+    // 210, 249, 437 in tiles of 192.
+    const int m = per + (int)sqrtf((float)per), two = (m + 127) / 128, three = (m + 191) / 192;
+    const bool low = two * 110 <= three * 150;
+    if (per > 56 && panels * (low ? two : three) >= 192)
+      return low ? launch_big<2>(a, st) : launch_big<3>(a, st);
     return a.out_f32 ? launch_tile<false, kF32>(a, st) : launch_tile<false, kBf16>(a, st);
   }
 }
