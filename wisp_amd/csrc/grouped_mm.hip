@@ -263,11 +263,19 @@ __device__ inline void zero_rows(const Args& a, int last) {
 }
 
 // Byte of 16-byte piece cb of row r of an LDS tile of 128-byte rows.  Rows shift
-// their pieces so that neither a fragment's 16 or 32 consecutive rows nor the
-// permuted ones of the weights (16 * a + 4 * g + b, below) meet in a bank; rows 32
-// apart shift alike.  (SQ_LDS_BANK_CONFLICT of the reads is 0.)
+// their pieces so that no two of 16 lanes that a read serves in one cycle meet in a
+// bank: lanes 0-3, 12-15, 20-27 of each half, the other 16 of it.  at: fragments of
+// 16 rows, in order or 16 * a + 4 * g + b (below), lane l / 16 at its own piece.
+// at32x and at32w: of 32 rows at one piece, in order, and 16 * h + 4 * a + b.
+// (SQ_LDS_BANK_CONFLICT of the reads is 0; with one rule for all, the reads of
+// 32 rows took 8 cycles instead of 4.)
 __device__ inline int at(int r, int cb) {
   const int shift = (r & 3) | ((r >> 2 ^ r >> 4) & 1) << 2;
+  return r * kChunk + ((cb ^ shift) << 4);
+}
+__device__ inline int at32x(int r, int cb) { return r * kChunk + ((cb ^ (r >> 1 & 7)) << 4); }
+__device__ inline int at32w(int r, int cb) {
+  const int shift = (r >> 1 & 1) | (r >> 4 & 1) << 1 | (r >> 2 & 1) << 2;
   return r * kChunk + ((cb ^ shift) << 4);
 }
 
@@ -595,7 +603,8 @@ __global__ __launch_bounds__(256, 1) void grouped_big_kernel(const Args a) {
 
   // copies: this lane's row and piece of every 32 rows
   const int crow = wave * 8 + (lane >> 3), ccol = 16 * (lane & 7);
-  uint8_t* const cdst = smem + at(crow, lane & 7);
+  uint8_t* const wdst = smem + at32w(crow, lane & 7);
+  uint8_t* const xdst = smem + kPanel * kChunk + at32x(crow, lane & 7);
   // fragments: this lane's row of every 32
   const int col = lane & 31, high = lane >> 5;
   const int frow = 16 * (col >> 2 & 1) + 4 * (col >> 3) + (col & 3);
@@ -622,9 +631,7 @@ __global__ __launch_bounds__(256, 1) void grouped_big_kernel(const Args a) {
   f32x16 acc[4][L];
   u32x4 wf[2][4], xf[2][L];
 
-  // Chunk c of a place's pair into cp[c].  (Raw buffer loads would return zeros
-  // behind a range's end by themselves, but pass a CU at one per 47 cycles,
-  // these at one per 26: the loads alone took 350 us where these take 191.)
+  // Chunk c of a place's pair into cp[c].
   auto load = [&](int pair, int c, int i) {
     const int o = (2 * pair + c) * kChunk;
     const uint8_t* base = i < 8 ? wbase : xbase;
@@ -641,17 +648,18 @@ __global__ __launch_bounds__(256, 1) void grouped_big_kernel(const Args a) {
       const uint32_t keep = (2 * pair + c) * kChunk + ccol < a.row_bytes ? ~0u : 0u;
       v &= u32x4{keep, keep, keep, keep};
     }
-    *reinterpret_cast<u32x4*>(cdst + c * Sh::kStage + 32 * i * kChunk) = v;
+    *reinterpret_cast<u32x4*>((i < 8 ? wdst + 32 * i * kChunk : xdst + 32 * (i - 8) * kChunk) +
+                              c * Sh::kStage) = v;
   };
   auto read = [&](int c, int step, int i) {
     const int to = step & 1;
     if (i < 4)
       wf[to][i] = *reinterpret_cast<const u32x4*>(
-          smem + c * Sh::kStage + at(128 * wr + 32 * i + frow, 2 * step + high));
+          smem + c * Sh::kStage + at32w(128 * wr + 32 * i + frow, 2 * step + high));
     else
       xf[to][i - 4] = *reinterpret_cast<const u32x4*>(
           smem + c * Sh::kStage + kPanel * kChunk +
-          at(32 * wt + 64 * (i - 4) + col, 2 * step + high));
+          at32x(32 * wt + 64 * (i - 4) + col, 2 * step + high));
   };
 
   Place cur = next(nowhere());
@@ -962,7 +970,7 @@ hipError_t launch_big_fp8(const Args& a, hipStream_t st) {
 // waves a fourth of the columns, whose loads are all in flight at once (kBatch
 // chunks of both operands); the partial sums meet in LDS, in wave order.  Blocks go
 // to the groups in use by their number: j-th in y, which ends name.  Qwen3 w13, one
-// token: 17.2 us with the tiles, 12.4 so.
+// token: 17.2 us with the tiles, 11.2 so.
 constexpr int kFewCols = 16;  // rows of x a pass
 
 template <bool FP8, int kBatch>
@@ -1071,8 +1079,8 @@ hipError_t launch_few(const Args& a, hipStream_t st) {
 template <bool FP8>
 hipError_t launch_few(const Args& a, hipStream_t st) {
   // a wave's chunks in as few batches as registers allow, the last one full (what
-  // it lacks is loaded all the same: Qwen3 w2, 3 chunks a wave in a batch of 8, 13.8
-  // us, of 3 FEW3)
+  // it lacks is loaded all the same: Qwen3 w2 of one token, 3 chunks a wave, takes
+  // 13.8 us in a batch of 8 and 7.5 in one of 3)
   const int per = ((a.row_bytes + kChunk - 1) / kChunk + kWaves - 1) / kWaves;
   if (per <= 2) return launch_few<FP8, 2>(a, st);
   if (per == 3 || per == 5 || per == 6) return launch_few<FP8, 3>(a, st);
