@@ -296,9 +296,9 @@ int wisp_silu_mul_fp8(const void* h, int dtype, int64_t rows, int inter, int64_t
  * or zeroed with zero_tail.  x [M, K] bfloat16, rows x_ld elements apart; W of
  * expert e at w + e*w_stride, [N, K] bfloat16, rows w_ld elements apart; out
  * [M, N] contiguous, WISP_BF16 or WISP_F32: float32 sums, rounded once.
- * E <= 512, K a multiple of 8, x, w and their strides 16-byte aligned, an
- * expert's weights below 2 GiB, rows of x less than 4 MiB apart.  No reference
- * counterpart (its experts run over one GPU's pairs). */
+ * E <= 512, N < 2^21, K a multiple of 8, x, w and their strides 16-byte aligned,
+ * an expert's weights below 2 GiB, rows of w less than 16 MiB and of x less than
+ * 4 MiB apart.  No reference counterpart (its experts run over one GPU's pairs). */
 int wisp_grouped_mm(const void* x, int64_t x_ld, const void* w, int64_t w_stride, int64_t w_ld,
                     const int32_t* ends, int E, int M, int N, int K, void* out, int out_dtype,
                     int zero_tail, wisp_stream_t stream);
@@ -309,7 +309,8 @@ int wisp_grouped_mm(const void* x, int64_t x_ld, const void* w, int64_t w_stride
  * ceil(K / 128)] contiguous.  Per 128 columns
  * acc += dot(q, w) * (s * ws) in float32; the dot is the fp8 matrix
  * instruction's, off by up to some 2^-16 of the sum of its products' sizes on
- * ordinary rows.  K a multiple of 16; otherwise as above. */
+ * ordinary rows.  K a multiple of 16, rows of s less than 4 MiB apart; otherwise
+ * as above. */
 int wisp_grouped_mm_fp8(const uint8_t* q, int64_t q_ld, const float* s, int64_t s_ld,
                         const uint8_t* w, int64_t w_stride, int64_t w_ld, const float* ws,
                         int64_t ws_stride, const int32_t* ends, int E, int M, int N, int K,

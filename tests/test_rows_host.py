@@ -54,6 +54,9 @@ def test_silu_arguments(hiplib, kw, rc):
     (dict(K=60), UNSUPPORTED), (dict(x=P + 8), UNSUPPORTED), (dict(w=P + 2), UNSUPPORTED),
     (dict(x_ld=68), UNSUPPORTED), (dict(w_ld=68), UNSUPPORTED), (dict(ws=4100), UNSUPPORTED),
     (dict(N=1 << 24), UNSUPPORTED), (dict(x_ld=1 << 21), UNSUPPORTED), (dict(dt=FP8), INVALID),
+    (dict(N=1 << 21), UNSUPPORTED), (dict(w_ld=1 << 23), UNSUPPORTED),
+    (dict(N=2 ** 31 - 1, w_ld=1 << 61), UNSUPPORTED), (dict(x_ld=1 << 61), UNSUPPORTED),
+    (dict(w_ld=1 << 22, N=256), UNSUPPORTED),
 ])
 def test_grouped_arguments(hiplib, kw, rc):
     a = dict(x=P, x_ld=64, w=P, ws=4096, w_ld=64, ends=P, E=2, M=4, N=64, K=64, out=P, dt=BF16)
@@ -73,7 +76,8 @@ def test_grouped_arguments(hiplib, kw, rc):
     (dict(K=136), UNSUPPORTED), (dict(q=P + 8), UNSUPPORTED), (dict(w=P + 8), UNSUPPORTED),
     (dict(q_ld=152), UNSUPPORTED), (dict(w_ld=152), UNSUPPORTED), (dict(wst=1032), UNSUPPORTED),
     (dict(s_ld=1 << 20), UNSUPPORTED), (dict(q_ld=1 << 22), UNSUPPORTED),
-    (dict(N=1 << 24), UNSUPPORTED),
+    (dict(N=1 << 24), UNSUPPORTED), (dict(N=1 << 21), UNSUPPORTED),
+    (dict(w_ld=1 << 24), UNSUPPORTED), (dict(w_ld=1 << 23, N=256), UNSUPPORTED),
 ])
 def test_grouped_fp8_arguments(hiplib, kw, rc):
     a = dict(q=P, q_ld=144, s=P, s_ld=2, w=P, wst=64 * 144, w_ld=144, ws=P, wsst=2, ends=P, E=2,

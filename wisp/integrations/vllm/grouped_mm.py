@@ -15,9 +15,10 @@ only; these products are the parts of such a rank's experts::
 rows ``[ends[e - 1], ends[e])``, from 0 for the first.  An end outside ``[0,
 rows]`` counts as 0 or ``rows``, one below an earlier end as that one, so groups
 never overlap.  Rows behind the last group are left as they are in a given
-``out`` and are zero in a new one.  Up to 512 experts; weights are ``[E, N, K]``
-(``w13``, ``w2`` as the MoE layers hold them), each row contiguous; an expert's
-are less than 2 GiB.
+``out`` and are zero in a new one.  Up to 512 experts of fewer than 2^21 outputs;
+weights are ``[E, N, K]`` (``w13``, ``w2`` as the MoE layers hold them), each row
+contiguous, an expert's less than 2 GiB and its rows less than 16 MiB apart (rows of
+``x``, and of its scales, less than 4 MiB).
 """
 from __future__ import annotations
 

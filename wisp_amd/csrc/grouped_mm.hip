@@ -569,15 +569,24 @@ __global__ __launch_bounds__(256, 2) void grouped_tile_kernel(const Args a) {
 // ---------------------------------------------------------------------------
 //
 // One block a CU, four waves (2 x 2): a wave owns 128 weight rows and every other
-// 32 rows of x, in 4 x L tiles of v_mfma_f32_32x32x16_bf16.  Both operands go
-// through registers to LDS, 8 lanes a row, loaded three chunks ahead of their
-// use: a wave that read its operands straight from memory (16 rows of 64 bytes a load) would
-// keep the address unit busy for 64 cycles a load instead of 16.  A chunk is four
-// steps of 16 columns; between a step's matrix instructions go the reads of the
-// next step's fragments and a quarter of the chunk's stores and loads.  The
-// second half of a chunk's last step is multiplied behind the barrier.
+// 32 rows of x, in 4 x L tiles of v_mfma_f32_32x32x16_bf16, the instruction that
+// one wave a SIMD feeds best (on random values 2016 TFLOP/s, 1777 with 16x16x32).
+// Both operands go through registers to LDS, 8 lanes a row, loaded three chunks
+// ahead of their use: a wave that read its operands straight from memory, 16 rows
+// of 64 bytes a load, would keep the address unit busy for 64 cycles a load
+// instead of 16.  A chunk is four steps of 16 columns; between a step's matrix
+// instructions go the reads of the next step's fragments, as early as they can,
+// and a share of the chunk's stores and loads.  The last matrix instructions of a
+// chunk's last step are multiplied behind the barrier, over the next reads.
 // MFMA row 8 * a + 4 * h + b of a group of 32 is weight row 16 * h + 4 * a + b, so
 // that a lane ends with 16 consecutive outputs of a row of x.
+//
+// Qwen3 w13 of 65536 rows, 128 experts (412 GFLOP): 470 us, 875 TFLOP/s; Mixtral
+// w13 of 4000 rows (940 GFLOP): 977 us, 962 TFLOP/s.  Of 100 cycles the matrix units
+// are busy for 58 and LDS for 34; the clock falls to 1.74 GHz for the power that
+// takes.  Without the loads the products take 287 us, the loads alone 345
+// (what the L2s miss: each line is read by the two or three blocks that share it).
+// One more 64 rows of x a tile (L 4) spills registers and takes 465 us and more.
 template <int L>
 struct Big {
   static constexpr int kToks = 64 * L;
@@ -696,9 +705,9 @@ __global__ __launch_bounds__(256, 1) void grouped_big_kernel(const Args a) {
             for (int i = 0; i < 2 * L; ++i) {  // two matrix instructions each
               if (step < 3) {
 #pragma unroll
-                for (int k = i * (4 + L) / (2 * L); k < (i + 1) * (4 + L) / (2 * L); ++k)
-                  read(c, step + 1, k);
-              } else if (i == L) {
+                for (int k = 2 * i; k < 2 * i + 2; ++k)
+                  if (k < 4 + L) read(c, step + 1, k);
+              } else if (i == 2 * L - 2) {
                 block_lds_sync();
 #pragma unroll
                 for (int k = 0; k < 4 + L; ++k) read(c ^ 1, 0, k);
@@ -710,7 +719,7 @@ __global__ __launch_bounds__(256, 1) void grouped_big_kernel(const Args a) {
               // This place's share of the copies, all of them before the barrier:
               // the next chunk leaves for its stage, and the one that follows it
               // by two is loaded.
-              constexpr int kPlaces = 7 * L;
+              constexpr int kPlaces = 8 * L - 2;
               const int place = 2 * L * step + i;
               if (place < kPlaces) {
 #pragma unroll
@@ -769,6 +778,12 @@ hipError_t launch_big(const Args& a, hipStream_t st) {
 // result is scaled into the sums while the next weight rows are multiplied.  MFMA
 // row 4 * a + b of group 4 * c + g is weight row 64 * c + 16 * a + 4 * g + b, so
 // that a lane ends with 16 consecutive outputs of a row of x.
+//
+// Mixtral w13 of 4000 rows (940 GFLOP): 560 us, 1680 TFLOP/s.  Of 100 cycles the
+// matrix units are busy for 56 and LDS for 37; the scaling (four fused adds behind a
+// matrix instruction of 32 cycles) takes half as many vector cycles as that again,
+// and all of it overlaps only as two waves a SIMD let it.  Four waves of 256 x 128 take 706 us; the 32 x 32
+// instruction's 16 sums a tile do not fit the registers (3826 us with spills).
 struct Big8 {
   static constexpr int kWaves = 8;
   static constexpr int kToks = 256;
@@ -957,7 +972,8 @@ hipError_t launch_big_fp8(const Args& a, hipStream_t st) {
   static std::atomic<uint64_t> done{0};
   const hipError_t e = allow_lds(&grouped_big_fp8_kernel<TAIL>, Big8::kLds, Big8::kLds, &done);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((grouped_big_fp8_kernel<TAIL>), dim3(256), dim3(64 * Big8::kWaves), Big8::kLds, st, a);
+  hipLaunchKernelGGL((grouped_big_fp8_kernel<TAIL>), dim3(256), dim3(64 * Big8::kWaves),
+                     Big8::kLds, st, a);
   return hipGetLastError();
 }
 
@@ -1084,15 +1100,18 @@ hipError_t launch_few(const Args& a, hipStream_t st) {
   const int per = ((a.row_bytes + kChunk - 1) / kChunk + kWaves - 1) / kWaves;
   if (per <= 2) return launch_few<FP8, 2>(a, st);
   if (per == 3 || per == 5 || per == 6) return launch_few<FP8, 3>(a, st);
-  if (FP8 || per == 4) return launch_few<FP8, 4>(a, st);
-  return launch_few<FP8, FP8 ? 4 : 8>(a, st);
+  if constexpr (!FP8)
+    if (per > 4) return launch_few<FP8, 8>(a, st);
+  return launch_few<FP8, 4>(a, st);
 }
 
 template <bool FP8, int G, Out OUT>
 hipError_t launch_tile(const Args& a, hipStream_t st) {
   using Sh = Shape<4, G>;
   static_assert(Sh::kLds <= 64 * 1024, "LDS beyond the default limit");
-  hipLaunchKernelGGL((grouped_tile_kernel<FP8, 4, G, OUT>), dim3(256 * (G == 4 ? 2 : G == 2 ? 3 : 4)), dim3(256), Sh::kLds, st, a);
+  constexpr int kBlocks = G == 4 ? 2 : G == 2 ? 3 : 4;  // a CU, as registers allow
+  hipLaunchKernelGGL((grouped_tile_kernel<FP8, 4, G, OUT>), dim3(256 * kBlocks), dim3(256),
+                     Sh::kLds, st, a);
   return hipGetLastError();
 }
 
@@ -1159,10 +1178,11 @@ const char* unsupported(int64_t x_ld, int64_t w_ld, int64_t w_stride, int64_t N,
   if (x_ld * elem % 16 || w_ld * elem % 16 || w_stride * elem % 16 || (uintptr_t)x % 16 ||
       (uintptr_t)w % 16)
     return "x, w and their strides must be 16-byte aligned";
-  // (32-bit offsets inside a tile of x and inside an expert's weights)
-  if (N * w_ld * elem >= (int64_t)1 << 31 || w_ld * elem >= (int64_t)1 << 24 ||
-      x_ld * elem >= (int64_t)1 << 22 || N >= 1 << 21)
-    return "an expert's weights of 2 GiB, rows of w 16 MiB or of x 4 MiB apart, or 2^21 outputs";
+  // (32-bit offsets inside a tile of x, inside an expert's weights and in a tile's outputs)
+  if (w_ld * elem >= (int64_t)1 << 24 || N * w_ld * elem >= (int64_t)1 << 31)
+    return "rows of w 16 MiB apart, or an expert's weights of 2 GiB";
+  if (x_ld * elem >= (int64_t)1 << 22) return "rows of x 4 MiB apart";
+  if (N >= 1 << 21) return "2^21 outputs of a row";
   return nullptr;
 }
 
