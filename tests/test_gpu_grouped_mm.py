@@ -359,6 +359,152 @@ def test_the_same_bytes_again(fp8):
         assert torch.equal(_bits(call(*ins, ends)), _bits(first))
 
 
+# The variants beyond the smallest tiles.  Few rows: one wave's columns in one
+# and in several batches, groups of more rows than a pass takes.
+@pytest.mark.parametrize("M,E,N", [(1, 4, 40), (32, 3, 100), (64, 2, 129)])
+@pytest.mark.parametrize("K", [496, 512, 528, 768, 1008, 1296, 1536, 1808, 2064, 4112])
+def test_few_rows_by_columns(M, E, N, K):
+    counts = _spread_counts(M, E, K) if M > 1 else [0, 1, 0, 0]
+    _check(M, E, N, K, counts, K)
+    _check8(M, E, N, K, counts, K)
+
+
+# rows, experts, outputs: 128 and 256 weight rows a tile, whole and ragged
+WIDE = [(70, 60, 1664), (300, 60, 1672), (1100, 60, 1660), (101, 100, 2048), (700, 110, 1800),
+        (2000, 100, 1804), (90, 60, 1667), (333, 100, 1801)]
+
+
+@pytest.mark.parametrize("K", [16, 136, 256, 464])
+@pytest.mark.parametrize("M,E,N", WIDE)
+def test_wide_panels(M, E, N, K):
+    counts = _spread_counts(M - 3, E, M + K)
+    for dtype in (BF, F32):
+        _check(M, E, N, K, counts, M, dtype)
+    _check8(M, E, N, K - K % 16, counts, M)
+
+
+# rows per expert, outputs, columns: of 24 experts, enough to fill the GPU with
+# the large tiles.  Columns: one chunk and less, whole pairs of chunks, an odd
+# number of chunks, a piece more.
+LARGE = [(60, 2048, 128), (60, 1800, 176), (61, 1796, 64), (90, 1800, 256), (95, 2048, 144),
+         (100, 1928, 16), (125, 2048, 384), (130, 1800, 1040), (131, 1800, 512), (190, 2040, 272),
+         (200, 1808, 400)]
+
+
+@pytest.mark.parametrize("kind", ["even", "ragged", "one", "edges"])
+@pytest.mark.parametrize("per,N,K", LARGE)
+def test_large_tiles(per, N, K, kind):
+    E = 24
+    M = E * per
+    if kind == "even":
+        counts = [per] * E
+    elif kind == "one":
+        counts = [0] * 5 + [M - 9] + [0] * 18
+    elif kind == "edges":   # around the tiles' heights, as many as there is room for
+        counts, left = [], M
+        for n in ([255, 0, 257, 1, 192, 193, 127, 129, 16, 17, 0, 31] * 2):
+            counts.append(min(n, left))
+            left -= counts[-1]
+    else:
+        counts = _spread_counts(M - 70, E, per)
+    if N % 8 == 0:
+        _check(M, E, N, K, counts, per)
+        _check8(M, E, N, K, counts, per)
+    _check(M, E, N, K, counts, per, F32)
+
+
+@pytest.mark.parametrize("per", [60, 130])
+def test_large_tiles_values_stay_in_their_rows_and_columns(per):
+    """As above: other groups' rows, rows behind the last group, other experts'
+    weights, columns behind a row's end."""
+    E, N, K = 24, 1800, 200
+    M = E * per
+    counts = _spread_counts(M - 33, E, per)
+    counts[3], counts[4] = counts[3] + counts[4], 0
+    ends = _ends(counts)
+    x, w = _randn((M, K), per), _randn((E, N, K), per + 1)
+    want = G.grouped_mm(x, w, ends)
+    big_x = torch.full((M, 264), float("nan"), dtype=BF, device=DEV)
+    big_w = torch.full((E, N + 3, 328), float("nan"), dtype=BF, device=DEV)
+    big_x[:, :K], big_w[:, :N, :K] = x, w
+    big_x[M - 33:] = float("inf")
+    big_w[4] = float("nan")
+    xs, ws = big_x[:, :K], big_w[:, :N, :K]
+    assert torch.equal(G.grouped_mm(xs, ws, ends), want)
+    out = torch.full((M, N), 7.0, dtype=BF, device=DEV)
+    G.grouped_mm(xs, ws, ends, out=out)
+    assert torch.equal(out[:M - 33], want[:M - 33]) and bool((out[M - 33:] == 7).all())
+    e = int(np.argmax(counts))
+    first, n = int(sum(counts[:e])), int(counts[e])
+    big_x[first + n // 2, 9], big_w[e, 1799, 199] = float("inf"), float("nan")
+    got = G.grouped_mm(xs, ws, ends)
+    bad = torch.zeros((M, N), dtype=torch.bool, device=DEV)
+    bad[first + n // 2] = True
+    bad[first:first + n, 1799] = True
+    assert torch.equal(got[~bad], want[~bad]) and not torch.isfinite(got[bad]).any()
+
+
+@pytest.mark.parametrize("K", [144, 400])
+def test_large_fp8_tiles_values_stay_in_their_rows_and_columns(K):
+    E, N, per = 24, 1800, 100
+    M = E * per
+    counts = _spread_counts(M - 33, E, K)
+    counts[3], counts[4] = counts[3] + counts[4], 0
+    ends = _ends(counts)
+    q, s, w, ws = _case8(M, E, N, K, K)
+    g = s.shape[1]
+    want = G.grouped_mm_fp8(q, s, w, ws, ends)
+    big_q = torch.full((M, 528), 0x7f, dtype=torch.uint8, device=DEV).view(FP8)
+    big_w = torch.full((E, N + 3, 448), 0x7f, dtype=torch.uint8, device=DEV).view(FP8)
+    big_s = torch.full((M, g + 2), float("nan"), device=DEV)
+    big_q.view(torch.uint8)[:, :K], big_w.view(torch.uint8)[:, :N, :K] = \
+        q.view(torch.uint8), w.view(torch.uint8)
+    big_s[:, :g] = s
+    big_q.view(torch.uint8)[M - 33:] = 0x7f
+    big_s[M - 33:] = float("inf")
+    big_w.view(torch.uint8)[4] = 0x7f
+    ws = ws.clone()
+    ws[4] = float("nan")
+    args = big_q[:, :K], big_s[:, :g], big_w[:, :N, :K], ws, ends
+    assert torch.equal(G.grouped_mm_fp8(*args), want)
+    out = torch.full((M, N), 7.0, dtype=BF, device=DEV)
+    G.grouped_mm_fp8(*args, out=out)
+    assert torch.equal(out[:M - 33], want[:M - 33]) and bool((out[M - 33:] == 7).all())
+    e = int(np.argmax(counts))
+    first, n = int(sum(counts[:e])), int(counts[e])
+    big_s[first + n // 2, g - 1], ws[e, 14, 0] = float("inf"), float("nan")
+    got = G.grouped_mm_fp8(*args)
+    bad = torch.zeros((M, N), dtype=torch.bool, device=DEV)
+    bad[first + n // 2] = True
+    bad[first:first + n, 14 * 128:] = True
+    assert torch.equal(got[~bad], want[~bad]) and not torch.isfinite(got[bad]).any()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("per", [60, 130])
+def test_large_tiles_in_a_graph_and_again(per, fp8):
+    """Replayed with other ends, beside eager calls: the same bytes each time."""
+    E, N, K = 24, 1800, 400
+    M = E * per
+    ins = _case8(M, E, N, K, 70) if fp8 else (_randn((M, K), 71), _randn((E, N, K), 72))
+    call = G.grouped_mm_fp8 if fp8 else G.grouped_mm
+    sets = [_ends(_spread_counts(M - 50 * k, E, k)) for k in range(4)]
+    ends = sets[0].clone()
+    call(*ins, ends)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call(*ins, ends)
+    for e in sets + sets[:2]:
+        ends.copy_(e)
+        want = call(*ins, e)
+        out.fill_(7)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(_bits(out), _bits(want))
+        assert torch.equal(_bits(call(*ins, e)), _bits(want))
+
+
 def test_empty():
     w = _randn((2, 16, 32), 50)
     out = G.grouped_mm(torch.empty((0, 32), dtype=BF, device=DEV), w, _ends([0, 0]))
