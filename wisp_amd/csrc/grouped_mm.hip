@@ -897,18 +897,20 @@ __global__ __launch_bounds__(512, 2) void grouped_big_fp8_kernel(const Args a) {
 
   Place cur = next(nowhere());
   if (cur.work.expert >= 0) {
+    // (in the loop's order: a wait counts the loads behind the one it is for, the
+    // fewest on any way there)
     aim(cur.work);
+    load_scales(cur.pair, 0);
 #pragma unroll
     for (int i = 0; i < Sh::kCopies; ++i) load(cur.pair, 0, i);
-    load_scales(cur.pair, 0);
+    store_scale(cur.pair, 0);
+    ws = cws;
+    load_scales(cur.pair, 1);
 #pragma unroll
     for (int i = 0; i < Sh::kCopies; ++i) {
       store(cur.pair, 0, i);
       load(cur.pair, 1, i);
     }
-    store_scale(cur.pair, 0);
-    ws = cws;
-    load_scales(cur.pair, 1);
     __syncthreads();
     read_x(0);
     read_w(0, 0);
