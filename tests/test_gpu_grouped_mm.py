@@ -413,6 +413,16 @@ def test_large_tiles(per, N, K, kind):
     _check(M, E, N, K, counts, per, F32)
 
 
+@pytest.mark.parametrize("E,per,N", [(6, 200, 2056), (6, 400, 2056), (3, 900, 2056),
+                                     (9, 330, 1800), (20, 260, 2048), (40, 130, 1544)])
+@pytest.mark.parametrize("K", [136, 256])
+def test_large_tiles_that_do_not_fill_the_gpu(E, per, N, K):
+    """Tiles for a part of the GPU, and for one turn of it and a part."""
+    for counts in ([per] * E, _spread_counts(E * per - 5, E, per)):
+        _check(E * per, E, N, K, counts, K)
+        _check8(E * per, E, N, K - K % 16, counts, K)
+
+
 @pytest.mark.parametrize("per", [60, 130])
 def test_large_tiles_values_stay_in_their_rows_and_columns(per):
     """As above: other groups' rows, rows behind the last group, other experts'

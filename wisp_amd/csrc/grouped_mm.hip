@@ -213,12 +213,17 @@ __device__ inline Work find_work(const Table* tab, int w, int E, int npanels, in
   return Work{-1, 0, 0, 0};
 }
 
-// Blocks go to the XCDs round-robin; each XCD takes runs of kRun consecutive
-// works, so blocks that read the same weights or rows share an L2.
-constexpr int kRun = 32;
-__device__ inline int work_of(int b, int j) {
-  const int i = (b >> 3) + j * ((int)gridDim.x >> 3);
-  return ((i / kRun) * 8 + (b & 7)) * kRun + i % kRun;
+// Blocks go to the XCDs round-robin; each XCD takes runs of up to 32 consecutive
+// works, so blocks that read the same weights or rows share an L2.  The runs are
+// as many for every XCD, and as long: with runs of 32 always, 128 works would
+// leave four XCDs with their L2 and their share of the memory's rate idle.
+__device__ inline int run_length(int works) {
+  const int turns = (works + 255) / 256;
+  return max((works + 8 * turns - 1) / max(8 * turns, 1), 1);
+}
+__device__ inline int work_of(int b, int j, int run) {
+  const int i = (b >> 3) + j * ((int)gridDim.x >> 3), turn = i / run;
+  return (turn * 8 + (b & 7)) * run + i - turn * run;
 }
 
 // A pair of chunks of a work, left of them to go with this one.
@@ -234,12 +239,12 @@ __device__ inline Place nowhere() { return Place{Work{-1, 0, 0, 0}, 0, 0}; }
 template <int TOKS>
 struct Walk {
   const Table* tab;
-  int E, npanels, pairs, turn;
+  int E, npanels, pairs, run, turn;
   __device__ __attribute__((always_inline)) inline Place next(Place p) {
     p.pair = p.pair + 1 == pairs ? 0 : p.pair + 1;
     if (--p.left > 0) return p;
     do {
-      p.work = find_work(tab, work_of(blockIdx.x, turn++), E, npanels, TOKS);
+      p.work = find_work(tab, work_of(blockIdx.x, turn++, run), E, npanels, TOKS);
     } while (p.work.expert >= 0 && p.work.rows == 0);
     p.pair = p.work.expert < 0 ? 0 : (int)((int64_t)p.work.panel * pairs / npanels);
     p.left = pairs;
@@ -376,7 +381,7 @@ __global__ __launch_bounds__(256, 2) void grouped_tile_kernel(const Args a) {
   const int xvoff = xrow * (int)a.x_ld + 16 * (lane & 7);
 
   // (three places in flight: computed, weights loading, rows loading)
-  Walk<Sh::kToks> walk{tab, a.E, npanels, pairs, 0};
+  Walk<Sh::kToks> walk{tab, a.E, npanels, pairs, run_length(tab->base[a.E] * npanels), 0};
   auto next = [&](const Place& p) { return walk.next(p); };
 
   u32x4 wf[2][2][G];            // [chunk of a pair][half of it][group]
@@ -618,7 +623,7 @@ __global__ __launch_bounds__(256, 1) void grouped_big_kernel(const Args a) {
   const int col = lane & 31, high = lane >> 5;
   const int frow = 16 * (col >> 2 & 1) + 4 * (col >> 3) + (col & 3);
 
-  Walk<Sh::kToks> walk{tab, a.E, npanels, pairs, 0};
+  Walk<Sh::kToks> walk{tab, a.E, npanels, pairs, run_length(tab->base[a.E] * npanels), 0};
   auto next = [&](const Place& p) { return walk.next(p); };
   // Where a work's rows start, and this lane's offsets of its copies from there;
   // rows behind the last are that one again (what they give is not stored).
@@ -811,7 +816,7 @@ __global__ __launch_bounds__(512, 2) void grouped_big_fp8_kernel(const Args a) {
   const int col = lane & 15, quarter = lane >> 4;
   const int frow = 16 * (col >> 2) + (col & 3);
 
-  Walk<Sh::kToks> walk{tab, a.E, npanels, pairs, 0};
+  Walk<Sh::kToks> walk{tab, a.E, npanels, pairs, run_length(tab->base[a.E] * npanels), 0};
   auto next = [&](const Place& p) { return walk.next(p); };
   const uint8_t *wbase, *xbase;
   const float *sbase, *wsbase;
@@ -1117,12 +1122,27 @@ hipError_t launch_tile(const Args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+// Tiles of t rows of an expert, on average over experts of per rows give or take
+// their square root: one, and one more for every k * t rows that it has.
+float tiles_of(float per, int t) {
+  const float h = 1.73f * sqrtf(per);  // (as if evenly spread, of that deviation)
+  const int sure = std::max((int)((per - h) / t), 0);
+  float n = 1.f + sure;
+  for (int k = sure + 1; (float)k * t < per + h; ++k)
+    n += std::min((per + h - (float)k * t) / (2 * h), 1.f);
+  return n;
+}
+
 template <bool FP8, Out OUT>
 hipError_t launch_tile(const Args& a, hipStream_t st) {
-  // the largest panels that give every CU two blocks
-  const int64_t used = std::min(a.M, a.E);
+  // The largest panels that give the GPU's blocks a tile each; where experts have
+  // several tiles of rows, and the products count too, panels of 128 from fewer on
+  // (fp8, 8 experts of 75 rows, 4096 x 14336: 170 us in panels of 64, 151 in 128;
+  // 16 of 64 rows, 1536 x 2048: 22.3 and 23.4).
+  const int64_t used = std::min(a.M, a.E), works = used * ((a.N + 127) / 128);
+  const int64_t rows = (int64_t)(tiles_of((float)a.M / a.E, 64) + 0.5f);
   if (used * ((a.N + 255) / 256) >= 768) return launch_tile<FP8, 4, OUT>(a, st);
-  if (used * ((a.N + 127) / 128) >= 768) return launch_tile<FP8, 2, OUT>(a, st);
+  if (works >= 768 || (rows > 1 && works * rows >= 400)) return launch_tile<FP8, 2, OUT>(a, st);
   return launch_tile<FP8, 1, OUT>(a, st);
 }
 
@@ -1142,27 +1162,34 @@ hipError_t launch(const Args& a, hipStream_t st) {
     return launch_few<FP8>(a, st);
   // single values are stored by the small tiles only
   if (a.N % (a.out_f32 ? 4 : 8)) return launch_tile<FP8, kNarrow>(a, st);
-  // rows an expert has if they are spread evenly, and its panels of 256
-  const int per = a.M / a.E;
-  const int64_t panels = (int64_t)a.E * ((a.N + kPanel - 1) / kPanel);
-  // Tiles of the weights' stream while the experts have few rows (or the large ones
-  // would leave CUs idle: Qwen3 w2 of 16 experts, 60 rows each, 128 works, 21.6 us,
-  // 16.7 in tiles of 64 weight rows), then large ones.
+  // What a chunk of columns takes in each kernel, in 1/100 us, from the works that a
+  // CU gets: w on average, as whole turns in the large tiles.  (Works of the small
+  // ones: 128 weight rows.  Measured over 4 to 128 experts, 8 sizes of weights, 32
+  // to 2000 rows each; the choice is the faster one or within some 5 %, 15 at most.)
+  //                        bf16, us: small  128 rows  192 rows   fp8: small  large
+  //   128 x 1536 x 2048,  32 rows      146    147       152             81     97
+  //                       64           194    161       163            107    102
+  //                      128           284    203       189            158    112
+  //                      200           401    241       282            222    124
+  //   8 x 4096 x 14336,   40           180    207       235            110    168
+  //                      100           273    231       241            158    169
+  //                      300           719    417       322            390    223
+  //   24 x 704 x 1056,    64          13.7   19.5      26.0           12.5   21.3
+  //                      375          31.9   24.3      29.5           25.4   24.8
+  const float per = (float)a.M / a.E, panels = (float)(a.E * (int64_t)((a.N + kPanel - 1) / kPanel));
+  const float w = a.E * (float)((a.N + 127) / 128) * floorf(tiles_of(per, 64) + 0.5f) / 256;
+  auto large = [&](int rows, float turn, float work) {
+    const float w = panels * tiles_of(per, rows) / 256;
+    return turn * ceilf(w) + work * w;
+  };
   if constexpr (FP8) {
-    // Qwen3 w13 of 128 experts at 64, 96, 128 rows each: 113, 128, 158 us in the
-    // first, 117, 120, 124 in the large ones.
-    if (per > 88 && panels * ((per + 255) / 256) >= 192)
+    if (large(256, 140, 80) < 50 + 52 * w)
       return a.row_bytes % (2 * kChunk) ? launch_big_fp8<true>(a, st) : launch_big_fp8<false>(a, st);
     return launch_tile<true, kBf16>(a, st);
   } else {
-    // Of two heights the one that takes less: the rows, and their square root more, in
-    // tiles of 30 + 40 L.  Qwen3 w13 at 48, 64, 128, 187, 512 rows an expert: 183, 203,
-    // 282, 362, 841 us in the first, 189, 192, 222, 253, 479 in tiles of 128 rows, 195, 198,
-    // 210, 249, 437 in tiles of 192.
-    const int m = per + (int)sqrtf((float)per), two = (m + 127) / 128, three = (m + 191) / 192;
-    const bool low = two * 110 <= three * 150;
-    if (per > 56 && panels * (low ? two : three) >= 192)
-      return low ? launch_big<2>(a, st) : launch_big<3>(a, st);
+    const float two = large(128, 80, 34), three = large(192, 100, 40);
+    if (std::min(two, three) < 30 + 44 * w)
+      return two <= three ? launch_big<2>(a, st) : launch_big<3>(a, st);
     return a.out_f32 ? launch_tile<false, kF32>(a, st) : launch_tile<false, kBf16>(a, st);
   }
 }
