@@ -1140,7 +1140,7 @@ hipError_t launch_tile(const Args& a, hipStream_t st) {
   // (fp8, 8 experts of 75 rows, 4096 x 14336: 170 us in panels of 64, 151 in 128;
   // 16 of 64 rows, 1536 x 2048: 22.3 and 23.4).
   const int64_t used = std::min(a.M, a.E), works = used * ((a.N + 127) / 128);
-  const int64_t rows = (int64_t)(tiles_of((float)a.M / a.E, 64) + 0.5f);
+  const int64_t rows = (int64_t)(tiles_of((float)a.M / a.E, 64) + 0.6f);
   if (used * ((a.N + 255) / 256) >= 768) return launch_tile<FP8, 4, OUT>(a, st);
   if (works >= 768 || (rows > 1 && works * rows >= 400)) return launch_tile<FP8, 2, OUT>(a, st);
   return launch_tile<FP8, 1, OUT>(a, st);
@@ -1158,7 +1158,25 @@ hipError_t launch_big(const Args& a, hipStream_t st) {
 
 template <bool FP8>
 hipError_t launch(const Args& a, hipStream_t st) {
-  if (a.M <= 32 || (a.M <= 64 && std::min(a.M, a.E) * (int64_t)((a.N + 255) / 256) <= 128))
+  // The kernel for the fewest rows (a) against the small tiles (b), in us:
+  //                     rows  bf16 a    b   fp8 a    b
+  //   128 x 1536 x 2048,  32   37.2  37.4   21.0  21.5
+  //                       64   60.9  68.0   36.2  38.5
+  //                      128  101.7 100.8   60.2  55.3
+  //   128 x 2048 x 768,   96   44.2  52.8   32.7  28.0
+  //   8 x 28672 x 4096,   32    304   328    178   174
+  //   8 x 4096 x 14336,   64    175   158    111    91
+  // and where the tiles cannot fill the GPU, while a group is one pass:
+  //   24 x 704 x 1056,   120   10.6  14.0    6.7  12.0
+  //                      231   12.1  13.8    7.5  12.0
+  //                      360   15.6  13.8    9.9  12.1
+  //   16 x 1536 x 2048,  160   24.4  25.0   14.7  16.5
+  //   16 x 2048 x 768,    80   12.8  12.4    9.7   9.8
+  // (at most 256 rows: all of them may be one expert's, a pass per 16)
+  const int most = FP8 ? std::max(16, std::min(32, 2 * a.E)) : std::max(32, std::min(96, 4 * a.E));
+  const int64_t works = std::min(a.M, a.E) * (int64_t)((a.N + 63) / 64);
+  if (a.M <= most || (a.M <= 64 && works <= 512) ||
+      (a.M <= 256 && works < 512 && tiles_of((float)a.M / a.E, kFewCols) == 1.f))
     return launch_few<FP8>(a, st);
   // single values are stored by the small tiles only
   if (a.N % (a.out_f32 ? 4 : 8)) return launch_tile<FP8, kNarrow>(a, st);
@@ -1176,19 +1194,24 @@ hipError_t launch(const Args& a, hipStream_t st) {
   //                      300           719    417       322            390    223
   //   24 x 704 x 1056,    64          13.7   19.5      26.0           12.5   21.3
   //                      375          31.9   24.3      29.5           25.4   24.8
-  const float per = (float)a.M / a.E, panels = (float)(a.E * (int64_t)((a.N + kPanel - 1) / kPanel));
-  const float w = a.E * (float)((a.N + 127) / 128) * floorf(tiles_of(per, 64) + 0.5f) / 256;
+  // None is faster than the weights' stream; where all are that fast, tiles of more
+  // rows read x fewer times (bf16, the first layer at 48 rows: 172 us small, 155).
+  const float per = (float)a.M / a.E, w1 = a.E * (float)((a.N + 127) / 128) / 256;
+  const float panels = (float)(a.E * (int64_t)((a.N + kPanel - 1) / kPanel));
+  const float stream = 76 * w1, w = w1 * floorf(tiles_of(per, 64) + 0.6f);
   auto large = [&](int rows, float turn, float work) {
     const float w = panels * tiles_of(per, rows) / 256;
-    return turn * ceilf(w) + work * w;
+    const float start = 150.f * kChunk / a.row_bytes;  // 1.5 us more than a small one's
+    return std::max(turn * ceilf(w) + work * w + start, stream);
   };
   if constexpr (FP8) {
-    if (large(256, 140, 80) < 50 + 52 * w)
+    if (large(256, 140, 80) < std::max(50 + 52 * w, stream))
       return a.row_bytes % (2 * kChunk) ? launch_big_fp8<true>(a, st) : launch_big_fp8<false>(a, st);
     return launch_tile<true, kBf16>(a, st);
   } else {
+    const float small = std::max(30 + 44 * w, stream);
     const float two = large(128, 80, 34), three = large(192, 100, 40);
-    if (std::min(two, three) < 30 + 44 * w)
+    if (std::min(two, three) < small || (std::min(two, three) == stream && per > 40))
       return two <= three ? launch_big<2>(a, st) : launch_big<3>(a, st);
     return a.out_f32 ? launch_tile<false, kF32>(a, st) : launch_tile<false, kBf16>(a, st);
   }
