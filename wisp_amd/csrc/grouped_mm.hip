@@ -233,9 +233,12 @@ struct Place {
 };
 __device__ inline Place nowhere() { return Place{Work{-1, 0, 0, 0}, 0, 0}; }
 
-// The pairs of a block's works, one after the other.  Each panel starts at a pair
-// of its own and wraps around: blocks that all start at column 0 crowd a few
-// memory channels (Qwen3 w13 of 512 tokens: 179 us, so 147; 1024 tokens 194, 162).
+// The pairs of a block's works, one after the other.  Every 24 panels in a row
+// start at a pair of their own and wrap around: blocks that all start at column 0
+// crowd a few memory channels (Qwen3 w13 of 512 tokens 179 us, so 144), and panels
+// that each start elsewhere read the rows of x that they share at different times,
+// out of the L2 again (1024 tokens 161 us, so 154; 8192 tokens 463, 449).
+constexpr uint32_t kGolden = 2654435769u;  // 2^32 / 1.618..: any first n are spread evenly
 template <int TOKS>
 struct Walk {
   const Table* tab;
@@ -246,7 +249,8 @@ struct Walk {
     do {
       p.work = find_work(tab, work_of(blockIdx.x, turn++, run), E, npanels, TOKS);
     } while (p.work.expert >= 0 && p.work.rows == 0);
-    p.pair = p.work.expert < 0 ? 0 : (int)((int64_t)p.work.panel * pairs / npanels);
+    const uint32_t set = (uint32_t)(max(p.work.expert, 0) * npanels + p.work.panel) / 24;
+    p.pair = (int)((uint64_t)(set * kGolden) * (uint32_t)pairs >> 32);
     p.left = pairs;
     return p;
   }
@@ -586,7 +590,7 @@ __global__ __launch_bounds__(256, 2) void grouped_tile_kernel(const Args a) {
 // MFMA row 8 * a + 4 * h + b of a group of 32 is weight row 16 * h + 4 * a + b, so
 // that a lane ends with 16 consecutive outputs of a row of x.
 //
-// Qwen3 w13 of 65536 rows, 128 experts (412 GFLOP): 470 us, 875 TFLOP/s; Mixtral
+// Qwen3 w13 of 65536 rows, 128 experts (412 GFLOP): 450 us, 916 TFLOP/s; Mixtral
 // w13 of 4000 rows (940 GFLOP): 977 us, 962 TFLOP/s.  Of 100 cycles the matrix units
 // are busy for 58 and LDS for 34; the clock falls to 1.74 GHz for the power that
 // takes.  Without the loads the products take 287 us, the loads alone 345
@@ -784,7 +788,7 @@ hipError_t launch_big(const Args& a, hipStream_t st) {
 // row 4 * a + b of group 4 * c + g is weight row 64 * c + 16 * a + 4 * g + b, so
 // that a lane ends with 16 consecutive outputs of a row of x.
 //
-// Mixtral w13 of 4000 rows (940 GFLOP): 560 us, 1680 TFLOP/s.  Of 100 cycles the
+// Mixtral w13 of 4000 rows (940 GFLOP): 525 to 570 us, 1650 to 1790 TFLOP/s.  Of 100 cycles the
 // matrix units are busy for 56 and LDS for 37; the scaling (four fused adds behind a
 // matrix instruction of 32 cycles) takes half as many vector cycles as that again,
 // and all of it overlaps only as two waves a SIMD let it.  Four waves of 256 x 128 take 706 us; the 32 x 32
