@@ -490,6 +490,29 @@ def test_large_fp8_tiles_values_stay_in_their_rows_and_columns(K):
     assert torch.equal(got[~bad], want[~bad]) and not torch.isfinite(got[bad]).any()
 
 
+@pytest.mark.parametrize("M,E,N", [(12, 3, 300), (90, 3, 300), (2400, 24, 1800), (4800, 24, 1800)])
+@pytest.mark.parametrize("K", [80, 272, 384])
+def test_fp8_scales_stay_in_their_blocks(M, E, N, K):
+    """A block's scale that is no number touches that block's columns only, and
+    an infinite one makes infinities of its sign, also where the row's last
+    columns fill no pair of blocks."""
+    q, s, w, ws = _case8(M, E, N, K, M + K)
+    q, w = (torch.where(t.float() == 0, 1.0, t.float()).abs().to(FP8) for t in (q, w))
+    ends = _ends(_spread_counts(M, E, K))
+    want = G.grouped_mm_fp8(q, s, w, ws, ends)
+    first, last = next((a, b) for a, b in O.groups(ends.tolist(), M) if b > a)
+    e = [b > a for a, b in O.groups(ends.tolist(), M)].index(True)
+    for block in range(ws.shape[1]):
+        for value in (float("nan"), float("inf")):
+            bad = ws.clone()
+            bad[e, block, block % ws.shape[2]] = value
+            got = G.grouped_mm_fp8(q, s, w, bad, ends)
+            at = torch.zeros((M, N), dtype=torch.bool, device=DEV)
+            at[first:last, 128 * block:128 * block + 128] = True
+            assert torch.equal(got[~at], want[~at])
+            assert bool(got[at].isnan().all() if value != value else got[at].isposinf().all())
+
+
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("per", [60, 130])
 def test_large_tiles_in_a_graph_and_again(per, fp8):

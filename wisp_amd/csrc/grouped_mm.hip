@@ -411,7 +411,9 @@ __global__ __launch_bounds__(256, 2) void grouped_tile_kernel(const Args a) {
                                p.work.expert < 0 ? 0u
                                                  : (uint32_t)(4 * a.groups *
                                                               ((a.N + kBlock - 1) / kBlock)));
-      wscale[c] = load4(sb, 0, 4 * ((int)(r0 / kBlock) * a.groups + 2 * p.pair + c));
+      // (behind the row's end the next block's would follow: none)
+      wscale[c] = load4(sb, 2 * p.pair + c < a.groups ? 0 : kNowhere,
+                        4 * ((int)(r0 / kBlock) * a.groups + 2 * p.pair + c));
     }
   };
   auto load_x = [&](const Place& p) {
@@ -936,6 +938,8 @@ __global__ __launch_bounds__(512, 2) void grouped_big_fp8_kernel(const Args a) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float sc[4];
+          // (nothing times zero where neither has a scale; ws is the last group's there)
+          if (TAIL && 2 * cur.pair + c >= a.groups) ws = 0.f;
 #pragma unroll
           for (int t = 0; t < 4; ++t) sc[t] = xscale[t] * ws;
           store_scale(c == 0 ? cur.pair : n1.pair, c ^ 1);
