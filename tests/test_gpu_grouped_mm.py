@@ -546,6 +546,23 @@ def test_empty():
     assert out.shape == (4, 0)
 
 
+def test_single_rows_of_any_stride():
+    """One row, one expert, one output: their strides say nothing."""
+    buf = _randn((3, 70000), 80)
+    x, ends = buf[1:2, :64], _ends([1])
+    w = _randn((1, 1, 64), 81)
+    odd = torch.empty(100000, dtype=BF, device=DEV).as_strided((1, 1, 64), (7, 3, 1))
+    odd.copy_(w)
+    want = G.grouped_mm(x.contiguous(), w, ends)
+    assert torch.equal(G.grouped_mm(x, odd, ends), want)
+    assert torch.equal(G.grouped_mm(x.as_strided((1, 64), (2 ** 40, 1)), odd, ends), want)
+    q, s, w8, ws = _case8(1, 1, 1, 64, 82)
+    want = G.grouped_mm_fp8(q, s, w8, ws, ends)
+    assert torch.equal(G.grouped_mm_fp8(
+        q.as_strided((1, 64), (2 ** 40, 1)), s.as_strided((1, 1), (2 ** 40, 1)),
+        w8.as_strided((1, 1, 64), (9, 5, 1)), ws, ends), want)
+
+
 def test_refusals():
     x, w, ends = _randn((6, 64), 60), _randn((2, 16, 64), 61), _ends([3, 3])
     q, s, w8, ws = _case8(6, 2, 16, 64, 62)
@@ -563,6 +580,26 @@ def test_refusals():
                 lambda: G.grouped_mm_fp8(q, s.cpu(), w8, ws, ends),
                 lambda: G.grouped_mm_fp8(q, s, w8, ws, ends, out=torch.empty((6, 16), device=DEV))):
         with pytest.raises(ValueError):
+            bad()
+    # out in the rows, the ends or the weights of the call
+    slab = torch.zeros(4096, dtype=BF, device=DEV)
+    for bad in (lambda: G.grouped_mm(x, slab[:2048].view(2, 16, 64), ends,
+                                     out=slab[2000:2096].view(6, 16)),
+                lambda: G.grouped_mm_fp8(q, s, slab.view(FP8)[:2048].view(2, 16, 64), ws, ends,
+                                         out=slab[1000:1096].view(6, 16)),
+                lambda: G.grouped_mm_fp8(q, slab.view(F32)[:6].view(6, 1), w8, ws, ends,
+                                         out=slab[8:104].view(6, 16)),
+                lambda: G.grouped_mm_fp8(q, s, w8, slab.view(F32)[:2].view(2, 1, 1), ends,
+                                         out=slab[:96].view(6, 16))):
+        with pytest.raises(ValueError, match="overlaps"):
+            bad()
+    # more rows or columns than a call counts
+    one = torch.zeros(16, dtype=BF, device=DEV)
+    for bad in (lambda: G.grouped_mm(one.expand(2 ** 31, 16), one.expand(1, 8, 16), ends[:1]),
+                lambda: G.grouped_mm(one.expand(4, 16), one.expand(1, 2 ** 32 + 8, 16), ends[:1]),
+                lambda: G.grouped_mm(one[:1].expand(4, 2 ** 32 + 8),
+                                     one.as_strided((1, 8, 2 ** 32 + 8), (0, 0, 0)), ends[:1])):
+        with pytest.raises((NotImplementedError, ValueError)):
             bad()
     for bad in (lambda: G.grouped_mm(x.float(), w, ends), lambda: G.grouped_mm(x, w.float(), ends),
                 lambda: G.grouped_mm(x, w, ends, dtype=torch.float16),

@@ -332,6 +332,9 @@ def test_refusals():
             bad()
     for bad in (lambda: R.add_rms_norm(x.half(), w.half()), lambda: R.add_rms_norm(x.float(), w),
                 lambda: R.add_rms_norm(x, w.half()), lambda: R.silu_mul_fp8(x.half()),
-                lambda: R.add_rms_norm(x[:, :1].expand(4, 40000), w[:1].expand(40000))):
+                lambda: R.add_rms_norm(x[:, :1].expand(4, 40000), w[:1].expand(40000)),
+                lambda: R.add_rms_norm(x[:, :1].expand(4, 2 ** 32 + 64),
+                                       w[:1].expand(2 ** 32 + 64)),
+                lambda: R.silu_mul_fp8(x[:, :1].expand(4, 2 ** 33 + 128))):
         with pytest.raises(NotImplementedError):
             bad()

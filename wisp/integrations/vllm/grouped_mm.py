@@ -46,7 +46,24 @@ def _sizes(x, w, ends) -> tuple[int, int, int, int]:
         _require_device(ends, x.device, "ends")
     if K > 1 and w.stride(2) != 1:
         raise ValueError("wisp: each row of w must be contiguous")
+    if M >= 1 << 31 or N >= 1 << 21 or K >= 1 << 31:
+        raise NotImplementedError("wisp: grouped products take fewer than 2^31 rows and columns "
+                                  "and 2^21 outputs")
     return M, E, N, K
+
+
+def _steps(w: torch.Tensor) -> tuple[int, int]:
+    """The elements from expert to expert and from row to row (a single one's
+    stride may be anything)."""
+    E, N, K = w.shape
+    return w.stride(0) if E > 1 else 0, w.stride(1) if N > 1 else K
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """First and one past the last byte that ``t`` may touch."""
+    first = t.data_ptr()
+    return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * \
+        t.element_size()
 
 
 def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
@@ -59,7 +76,7 @@ def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
     return x.clone() if x.data_ptr() % 16 else x
 
 
-def _output(x, N, dtype, out, inputs) -> torch.Tensor:
+def _output(x, N, dtype, out, inputs, weights) -> torch.Tensor:
     if out is None:
         return x.new_empty((x.shape[0], N), dtype=dtype)
     if out.shape != (x.shape[0], N) or out.dtype != dtype or not out.is_contiguous():
@@ -67,6 +84,12 @@ def _output(x, N, dtype, out, inputs) -> torch.Tensor:
     if out.get_device() != x.get_device():
         _require_device(out, x.device, "out")
     _check_apart("out", out, [(t, False) for t in inputs])
+    if out.numel():
+        first, last = _span(out)
+        for t in weights:  # (also the room between their experts)
+            a, b = _span(t)
+            if t.numel() and a < last and first < b:
+                raise ValueError("wisp: out overlaps another tensor of the call")
     return out
 
 
@@ -77,7 +100,8 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, *,
     """``out[i] = w[e] @ x[i]`` for the rows ``i`` of group ``e``: bfloat16
     ``x [M, K]`` and ``w [E, N, K]``, float32 sums, rounded once to ``dtype``
     (bfloat16 or float32; a given ``out`` is of that type).  K is a multiple of
-    8; rows of ``x`` and experts of ``w`` may lie any distance apart."""
+    8; rows of ``x`` may lie any distance apart, experts and rows of ``w`` any
+    multiple of 16 bytes, and ``w`` starts at one."""
     M, E, N, K = _sizes(x, w, ends)
     if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
         raise NotImplementedError("wisp: grouped_mm takes bfloat16 rows and weights")
@@ -85,10 +109,10 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, *,
         raise NotImplementedError(f"wisp: grouped_mm cannot give {dtype} (float32 and bfloat16)")
     x, ends = _aligned_rows(x), ends.contiguous()
     given = out is not None
-    out = _output(x, N, dtype, out, (x, ends) if given else ())
+    out = _output(x, N, dtype, out, (x, ends), (w,))
     if M and N:
-        rc = lib().wisp_grouped_mm(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
-                                   w.stride(1), ends.data_ptr(), E, M, N, K, out.data_ptr(),
+        rc = lib().wisp_grouped_mm(x.data_ptr(), x.stride(0) if M > 1 else K, w.data_ptr(),
+                                   *_steps(w), ends.data_ptr(), E, M, N, K, out.data_ptr(),
                                    _DTYPES[dtype], not given, _stream(x))
         if rc:
             check(rc, "grouped_mm")
@@ -121,12 +145,12 @@ def grouped_mm_fp8(q: torch.Tensor, s: torch.Tensor, w: torch.Tensor, ws: torch.
     if (s.stride(1) != 1 and G > 1) or s.stride(0) < G:
         s = s.contiguous()
     given = out is not None
-    out = _output(q, N, torch.bfloat16, out, (q, s, ends) if given else ())
+    out = _output(q, N, torch.bfloat16, out, (q, s, ends), (w, ws))
     if M and N:
         rc = lib().wisp_grouped_mm_fp8(
-            q.data_ptr(), q.stride(0), s.data_ptr(), s.stride(0), w.data_ptr(), w.stride(0),
-            w.stride(1), ws.data_ptr(), ws.stride(0), ends.data_ptr(), E, M, N, K, out.data_ptr(),
-            not given, _stream(q))
+            q.data_ptr(), q.stride(0) if M > 1 else K, s.data_ptr(), s.stride(0) if M > 1 else G,
+            w.data_ptr(), *_steps(w), ws.data_ptr(), ws.stride(0), ends.data_ptr(), E, M, N, K,
+            out.data_ptr(), not given, _stream(q))
         if rc:
             check(rc, "grouped_mm_fp8")
     return out

@@ -127,6 +127,8 @@ def _norm(x, weight, eps, residual, residual_out, out, q, s):
                 residual.shape != x.shape)):
         _check_norm(x, weight, residual, residual_out, out)
     rows, cols = x.shape
+    if cols > 32768:
+        raise NotImplementedError("wisp: norms of more than 32768 columns")
     # (a copy of rows that are not contiguous comes after the check for overlaps)
     x, weight = _rows(x), weight.contiguous()
     if out is None and not q:
@@ -186,6 +188,8 @@ def silu_mul_fp8(h: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise ValueError("wisp: h is [rows, 2 * I]")
     if h.dtype not in _DTYPES:
         raise NotImplementedError(f"wisp: rows of {h.dtype} (float32 and bfloat16)")
+    if h.shape[1] >= 1 << 31:
+        raise NotImplementedError("wisp: rows of 2^31 columns")
     h = _rows(h)
     rows, inter = h.shape[0], h.shape[1] // 2
     q = h.new_empty((rows, inter), dtype=FP8)
