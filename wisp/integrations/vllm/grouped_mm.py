@@ -30,11 +30,15 @@ from .fused_moe import _require_device
 from .rows_fp8 import FP8, GROUP, _DTYPES, _check_apart, _on_device, _stream
 
 
-def _sizes(x, w, ends) -> tuple[int, int, int, int]:
-    """``(M, E, N, K)`` of rows, weights and ends."""
-    if x.dim() != 2 or w.dim() != 3 or ends.dim() != 1:
-        raise ValueError("wisp: grouped products take rows [M, K], weights [E, N, K] and ends [E]")
-    (M, C), (E, N, K), (groups,) = x.shape, w.shape, ends.shape
+def _sizes(x, w, ends) -> tuple[int, int, int, int, int, int]:
+    """``(M, E, N, K)`` of rows, weights and ends, and the elements from expert to
+    expert and from row to row of the weights (a single one's stride may be
+    anything)."""
+    try:
+        (M, C), (E, N, K), (groups,) = x.shape, w.shape, ends.shape
+    except ValueError:
+        raise ValueError("wisp: grouped products take rows [M, K], weights [E, N, K] and "
+                         "ends [E]") from None
     if K != C or groups != E or not E:
         raise ValueError("wisp: grouped products take rows [M, K], weights [E, N, K] and ends "
                          f"[E], got {(M, C)}, {(E, N, K)}, {(groups,)}")
@@ -44,19 +48,13 @@ def _sizes(x, w, ends) -> tuple[int, int, int, int]:
     if w.get_device() != dev or ends.get_device() != dev:
         _require_device(w, x.device, "w")
         _require_device(ends, x.device, "ends")
-    if K > 1 and w.stride(2) != 1:
+    step, ld, one = w.stride()
+    if K > 1 and one != 1:
         raise ValueError("wisp: each row of w must be contiguous")
     if M >= 1 << 31 or N >= 1 << 21 or K >= 1 << 31:
         raise NotImplementedError("wisp: grouped products take fewer than 2^31 rows and columns "
                                   "and 2^21 outputs")
-    return M, E, N, K
-
-
-def _steps(w: torch.Tensor) -> tuple[int, int]:
-    """The elements from expert to expert and from row to row (a single one's
-    stride may be anything)."""
-    E, N, K = w.shape
-    return w.stride(0) if E > 1 else 0, w.stride(1) if N > 1 else K
+    return M, E, N, K, step if E > 1 else 0, ld if N > 1 else K
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
@@ -68,9 +66,8 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
 
 def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` with contiguous rows that start 16-byte aligned."""
-    size = x.element_size()
-    if x.stride(1) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) * size % 16 == 0 and \
-            x.stride(0) >= x.shape[1]:
+    step, one = x.stride()
+    if one == 1 and step >= x.shape[1] and (x.data_ptr() | step * x.element_size()) % 16 == 0:
         return x
     x = x.contiguous()
     return x.clone() if x.data_ptr() % 16 else x
@@ -102,7 +99,7 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, *,
     (bfloat16 or float32; a given ``out`` is of that type).  K is a multiple of
     8; rows of ``x`` may lie any distance apart, experts and rows of ``w`` any
     multiple of 16 bytes, and ``w`` starts at one."""
-    M, E, N, K = _sizes(x, w, ends)
+    M, E, N, K, step, w_ld = _sizes(x, w, ends)
     if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
         raise NotImplementedError("wisp: grouped_mm takes bfloat16 rows and weights")
     if dtype not in _DTYPES:
@@ -112,7 +109,7 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, *,
     out = _output(x, N, dtype, out, (x, ends), (w,))
     if M and N:
         rc = lib().wisp_grouped_mm(x.data_ptr(), x.stride(0) if M > 1 else K, w.data_ptr(),
-                                   *_steps(w), ends.data_ptr(), E, M, N, K, out.data_ptr(),
+                                   step, w_ld, ends.data_ptr(), E, M, N, K, out.data_ptr(),
                                    _DTYPES[dtype], not given, _stream(x))
         if rc:
             check(rc, "grouped_mm")
@@ -129,7 +126,7 @@ def grouped_mm_fp8(q: torch.Tensor, s: torch.Tensor, w: torch.Tensor, ws: torch.
     multiple of 16.  The products of 128 columns are summed by the matrix
     instruction, scaled and summed in float32 (to some 2^-16 of the sum of the
     products' sizes: there is no float32 output), and rounded once."""
-    M, E, N, K = _sizes(q, w, ends)
+    M, E, N, K, step, w_ld = _sizes(q, w, ends)
     if q.dtype != FP8 or w.dtype != FP8:
         raise NotImplementedError("wisp: grouped_mm_fp8 takes float8_e4m3fn codes")
     G, B = -(-K // GROUP), -(-N // GROUP)
@@ -149,7 +146,7 @@ def grouped_mm_fp8(q: torch.Tensor, s: torch.Tensor, w: torch.Tensor, ws: torch.
     if M and N:
         rc = lib().wisp_grouped_mm_fp8(
             q.data_ptr(), q.stride(0) if M > 1 else K, s.data_ptr(), s.stride(0) if M > 1 else G,
-            w.data_ptr(), *_steps(w), ws.data_ptr(), ws.stride(0), ends.data_ptr(), E, M, N, K,
+            w.data_ptr(), step, w_ld, ws.data_ptr(), ws.stride(0), ends.data_ptr(), E, M, N, K,
             out.data_ptr(), not given, _stream(q))
         if rc:
             check(rc, "grouped_mm_fp8")

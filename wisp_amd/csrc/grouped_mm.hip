@@ -65,7 +65,8 @@ __device__ __attribute__((always_inline)) inline u32x4 load_global(const uint8_t
   typedef const __attribute__((address_space(1))) uint8_t* Bytes;
   return *(const __attribute__((address_space(1))) u32x4*)((Bytes)p + off);
 }
-__device__ __attribute__((always_inline)) inline float load_global4(const uint8_t* p, uint32_t off) {
+__device__ __attribute__((always_inline)) inline float load_global4(const uint8_t* p,
+                                                                     uint32_t off) {
   typedef const __attribute__((address_space(1))) uint8_t* Bytes;
   return *(const __attribute__((address_space(1))) float*)((Bytes)p + off);
 }
@@ -307,13 +308,15 @@ constexpr int kNowhere = INT32_MIN;  // an offset behind every end, with any til
 // scalar offset: per lane, the compiler would hold every tile's offset in a
 // register through the products.)
 template <bool F32, bool WHOLE, int G>
-__device__ __attribute__((always_inline)) inline void store_outputs(const Outputs& o, int t0, int r, int n,
-                                                            const f32x4 (&v)[G]) {
+__device__ __attribute__((always_inline)) inline void store_outputs(const Outputs& o, int t0,
+                                                                    int r, int n,
+                                                                    const f32x4 (&v)[G]) {
   const int at = (r * o.N + n) * o.wide, soff = t0 * o.N * o.wide;
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     if constexpr (F32 && WHOLE) {
-      store16b(__builtin_bit_cast(u32x4, v[g]), o.b, n + 4 * g < o.N ? at + 16 * g : kNowhere, soff);
+      store16b(__builtin_bit_cast(u32x4, v[g]), o.b, n + 4 * g < o.N ? at + 16 * g : kNowhere,
+               soff);
     } else if constexpr (F32) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -342,7 +345,8 @@ __device__ __attribute__((always_inline)) inline void store_outputs(const Output
 // Few rows an expert: 64 * G weight rows by 64 rows of x
 // ---------------------------------------------------------------------------
 //
-// What bounds these calls is the weights' stream.  Persistent blocks of four
+// What bounds these calls is the weights' stream (Qwen3 w13 of 512 tokens: 144 us,
+// 5.6 TB/s; Mixtral's of 200 tokens 355 us, 5.3).  Persistent blocks of four
 // waves; a wave owns 16 * G weight rows and reads them from memory straight into
 // its registers, one to two chunks ahead: no other wave of the block needs them.
 // The rows of x, which all four need, go through LDS, two chunks a stage.  The
@@ -595,8 +599,8 @@ __global__ __launch_bounds__(256, 2) void grouped_tile_kernel(const Args a) {
 // Qwen3 w13 of 65536 rows, 128 experts (412 GFLOP): 450 us, 916 TFLOP/s; Mixtral
 // w13 of 4000 rows (940 GFLOP): 977 us, 962 TFLOP/s.  Of 100 cycles the matrix units
 // are busy for 58 and LDS for 34; the clock falls to 1.74 GHz for the power that
-// takes.  Without the loads the products take 287 us, the loads alone 345
-// (what the L2s miss: each line is read by the two or three blocks that share it).
+// takes.  Without the loads the products take 287 us; memory is read 1.25 GB of
+// 1.07 needed.
 // One more 64 rows of x a tile (L 4) spills registers and takes 465 us and more.
 template <int L>
 struct Big {
@@ -793,8 +797,9 @@ hipError_t launch_big(const Args& a, hipStream_t st) {
 // Mixtral w13 of 4000 rows (940 GFLOP): 525 to 570 us, 1650 to 1790 TFLOP/s.  Of 100 cycles the
 // matrix units are busy for 56 and LDS for 37; the scaling (four fused adds behind a
 // matrix instruction of 32 cycles) takes half as many vector cycles as that again,
-// and all of it overlaps only as two waves a SIMD let it.  Four waves of 256 x 128 take 706 us; the 32 x 32
-// instruction's 16 sums a tile do not fit the registers (3826 us with spills).
+// and all of it overlaps only as two waves a SIMD let it.  Without the loads 389 us.
+// Four waves of 256 x 128 take 706 us; the 32 x 32 instruction's 16 sums a tile do
+// not fit the registers (3826 us with spills).
 struct Big8 {
   static constexpr int kWaves = 8;
   static constexpr int kToks = 256;
@@ -1001,7 +1006,7 @@ hipError_t launch_big_fp8(const Args& a, hipStream_t st) {
 // waves a fourth of the columns, whose loads are all in flight at once (kBatch
 // chunks of both operands); the partial sums meet in LDS, in wave order.  Blocks go
 // to the groups in use by their number: j-th in y, which ends name.  Qwen3 w13, one
-// token: 17.2 us with the tiles, 11.2 so.
+// token: 17.2 us with the tiles, 10.9 so (4.6 TB/s; one round of blocks).
 constexpr int kFewCols = 16;  // rows of x a pass
 
 template <bool FP8, int kBatch>
@@ -1214,7 +1219,8 @@ hipError_t launch(const Args& a, hipStream_t st) {
   };
   if constexpr (FP8) {
     if (large(256, 140, 80) < std::max(50 + 52 * w, stream))
-      return a.row_bytes % (2 * kChunk) ? launch_big_fp8<true>(a, st) : launch_big_fp8<false>(a, st);
+      return a.row_bytes % (2 * kChunk) ? launch_big_fp8<true>(a, st)
+                                        : launch_big_fp8<false>(a, st);
     return launch_tile<true, kBf16>(a, st);
   } else {
     const float small = std::max(30 + 44 * w, stream);
