@@ -51,7 +51,7 @@ def _stream(t: torch.Tensor) -> int:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` with contiguous rows (any distance between them)."""
-    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+    return t if t.stride()[1] == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
 def _overlap(t: torch.Tensor, other: torch.Tensor) -> bool:
@@ -116,38 +116,49 @@ def _check_norm(x, weight, residual, residual_out, out):
                                   (residual_out, False)))
 
 
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A new contiguous tensor of ``x``'s shape and type (the quicker way where
+    there is one)."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
 def _norm(x, weight, eps, residual, residual_out, out, q, s):
     """The call: checks, then one launch.  (The common call is recognised first:
     the checks take microseconds, as long as a small call's kernel.)"""
-    dtype, dev = x.dtype, x.get_device()
-    if residual_out is not None or out is not None or x.dim() != 2 or dtype not in _DTYPES or \
+    dtype, dev, shape = x.dtype, x.get_device(), x.shape
+    if residual_out is not None or out is not None or len(shape) != 2 or dtype not in _DTYPES or \
             weight.dtype != dtype or weight.get_device() != dev or \
-            weight.shape != x.shape[1:] or (residual is not None and (
+            weight.shape != shape[1:] or (residual is not None and (
                 residual.dtype != dtype or residual.get_device() != dev or
-                residual.shape != x.shape)):
+                residual.shape != shape)):
         _check_norm(x, weight, residual, residual_out, out)
-    rows, cols = x.shape
+    rows, cols = shape
     if cols > 32768:
         raise NotImplementedError("wisp: norms of more than 32768 columns")
     # (a copy of rows that are not contiguous comes after the check for overlaps)
     x, weight = _rows(x), weight.contiguous()
-    if out is None and not q:
-        out = x.new_empty((rows, cols))
+    codes = scales = to = 0
     if q:
-        q = x.new_empty((rows, cols), dtype=FP8)
+        q = x.new_empty(shape, dtype=FP8)
         s = x.new_empty((rows, -(-cols // GROUP)), dtype=torch.float32)
+        codes, scales = q.data_ptr(), s.data_ptr()
+    elif out is None:
+        out = _like(x)
+    if out is not None:
+        to = out.data_ptr()
     r = rdt = rs = ro = ros = 0
     if residual is not None:
         residual = _rows(residual)
         if residual_out is None:
-            residual_out = residual.new_empty((rows, cols))
-        r, rdt, rs = residual.data_ptr(), _DTYPES[residual.dtype], residual.stride(0)
-        ro, ros = residual_out.data_ptr(), residual_out.stride(0)
+            residual_out, ros = _like(residual), cols
+        else:
+            ros = residual_out.stride(0)
+        r, rdt, rs, ro = residual.data_ptr(), _DTYPES[residual.dtype], residual.stride(0), \
+            residual_out.data_ptr()
     if rows and cols:
-        rc = lib().wisp_add_rms_norm(
-            x.data_ptr(), _DTYPES[dtype], rows, cols, x.stride(0), r, rdt, rs, ro, ros,
-            weight.data_ptr(), _DTYPES[weight.dtype], eps, 0 if out is None else out.data_ptr(),
-            q.data_ptr() if s is not None else 0, s.data_ptr() if s is not None else 0, _stream(x))
+        rc = lib().wisp_add_rms_norm(x.data_ptr(), _DTYPES[dtype], rows, cols, x.stride(0), r, rdt,
+                                     rs, ro, ros, weight.data_ptr(), _DTYPES[weight.dtype], eps,
+                                     to, codes, scales, _stream(x))
         if rc:
             check(rc, "add_rms_norm")
     return out, q, s, residual_out
