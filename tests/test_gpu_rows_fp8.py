@@ -241,6 +241,58 @@ def test_silu_beyond_the_exponential():
     assert torch.isfinite(s).all() and torch.isfinite(q.float()).all()
 
 
+def _check_silu_values(g, u, rel, low=0.0):
+    """The SwiGLU of gates ``g`` and factors ``u`` (1-D) to ``rel`` of each value
+    and ``low`` more: alone in its group a value is its scale's maximum, so the
+    scale shows it to two roundings; once in rows of one value, once in groups
+    that hold it 128 times."""
+    gate = _f64(g)
+    with np.errstate(over="ignore"):
+        want = np.abs(gate / (1.0 + np.exp(-gate)) * _f64(u))
+    assert want.min() >= 2 * O.LEAST and want.max() < 3e38
+    for wide in (1, 128):
+        h = torch.cat([g[:, None].expand(-1, wide), u[:, None].expand(-1, wide)], dim=1)
+        q, s = R.silu_mul_fp8(h)
+        off = np.abs(_f64(s)[:, 0] * 448 - want) / (rel * want + low + 2 * O.STEP * want)
+        assert off.max() <= 1, (float(off.max()), float(g[int(off.argmax())]))
+        sign = np.sign(_f64(g) * _f64(u))[:, None]
+        assert np.array_equal(_f64(q.float()), np.broadcast_to(448.0 * sign, q.shape))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_silu_largest_gates(dtype):
+    """Gates up to the largest finite value: the SiLU is the gate itself, and with a
+    small factor the value is finite."""
+    top = float(torch.finfo(dtype).max)
+    g = torch.tensor([129.0, 1e4, 1e30, 2.3e38, 2.36e38, 2.37e38, 2.5e38, 3e38, top] * 4,
+                     device=DEV).to(dtype)
+    u = torch.tensor([1e-3, -1e-3, 0.5, 2.0 ** -126], device=DEV).to(dtype).repeat_interleave(9)
+    keep = (g.double() * u.double()).abs() > 1e-9
+    # the sigmoid is 1, its reciprocal within a step (two half ones), two products
+    _check_silu_values(g[keep], u[keep], 4 * O.STEP)
+    # an infinite gate: codes that are no numbers, and the largest value's scale
+    h = _randn((3, 512), 23, dtype)
+    h[1, 130] = float("inf")
+    q, s = R.silu_mul_fp8(h)
+    assert q[1, 128:].float().isnan().all() and bool(s[1, 1] == float("inf"))
+    h[1, 130] = top
+    h[1, 386] = 1.0
+    q, s = R.silu_mul_fp8(h)
+    assert bool(s[1, 1] == torch.tensor(top) / 448) and q[1, 130].float() == 448
+    assert torch.isfinite(q.float()).all() and torch.isfinite(s).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_silu_to_some_half_steps(dtype):
+    """Ordinary gates to -87: an exponential within a step (two half ones), the product
+    with what its exponent's rounding left, the sum, the reciprocal within a step, two
+    products: seven half steps at every gate, and one for what those leave out."""
+    g = torch.linspace(-87, 87, 4001, device=DEV).to(dtype)
+    g = g[g != 0]
+    u = torch.exp2(-torch.floor(torch.log2(g.double().abs() / (1 + torch.exp(-g.double())))))
+    _check_silu_values(g, u.to(dtype), 8 * O.STEP)
+
+
 def test_silu_infinities_and_nans():
     h = _randn((5, 768), 21)
     h[0, 2], h[1, 384 + 130], h[2, 300] = float("nan"), float("inf"), float("inf")

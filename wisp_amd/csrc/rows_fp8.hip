@@ -307,10 +307,13 @@ constexpr int kMaxCols = 1024 * 4 * kPer;
 // exponential of the rounded exponent, times what the rounding left, and the
 // hardware's reciprocal with one step of Newton.  The library's functions would
 // take twice the instructions, and the vector units would bound the kernel.
+// (The exponent is made from g within [-128, 128]: g * log2(e) of the largest g is
+// infinite, and what its rounding left is no number.)
 __device__ inline float silu_fast(float g) {
   constexpr float kLog2e = 1.44269504088896340736f, kRest = 1.92596299e-8f, kLn2 = 0.69314718f;
-  const float p = g * -kLog2e;
-  const float rest = __builtin_fmaf(g, -kRest, __builtin_fmaf(g, -kLog2e, -p)) * kLn2;
+  const float t = __builtin_amdgcn_fmed3f(g, -128.f, 128.f);
+  const float p = t * -kLog2e;
+  const float rest = __builtin_fmaf(t, -kRest, __builtin_fmaf(t, -kLog2e, -p)) * kLn2;
   const float e = __builtin_amdgcn_exp2f(fminf(p, 126.f));
   const float d = 1.f + __builtin_fmaf(e, rest, e);
   float r = __builtin_amdgcn_rcpf(d);
