@@ -293,6 +293,33 @@ def test_silu_to_some_half_steps(dtype):
     _check_silu_values(g, u.to(dtype), 8 * O.STEP)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_silu_gates_to_the_end_of_float32(dtype):
+    """Gates whose SiLU is at the lower end of float32, with factors that bring the value
+    back: to the last of its subnormal numbers (seven half steps as above, and half a
+    subnormal step of the SiLU, twice for the product before it)."""
+    g = torch.linspace(-100, -80, 2001, device=DEV).to(dtype)
+    u = torch.full_like(g, 2.0 ** 126)
+    _check_silu_values(g, u, 8 * O.STEP, 2 * 2.0 ** -150 * 2.0 ** 126)
+    # beyond: nothing is left, whatever the factor
+    h = torch.full((4, 256), 2.0 ** 126, device=DEV, dtype=dtype)
+    h[0, :128], h[1, :128], h[2, :128] = -128, -1e30, -float(torch.finfo(dtype).max)
+    h[3, :128] = torch.linspace(-300, -115, 128, device=DEV)
+    q, s = R.silu_mul_fp8(h)
+    # (the quotient of the host: on the device torch multiplies by the scalar's reciprocal)
+    assert not q.float().any() and bool((s.cpu() == torch.tensor(1e-10) / 448).all())
+    # beside them what is no number: -inf / (1 + inf) and a NaN, in their groups only
+    h = torch.cat([h, h], dim=1).view(4, 2, 2, 128).transpose(1, 2).reshape(4, 512)
+    want = R.silu_mul_fp8(h)
+    h[1, 130], h[2, 5] = -float("inf"), float("nan")
+    got = R.silu_mul_fp8(h)
+    for bits, clean in ((_bits(got[0]).view(4, 2, 128), _bits(want[0]).view(4, 2, 128)),
+                        (_bits(got[1]), _bits(want[1]))):
+        same = (bits == clean).view(4, 2, -1).all(dim=2)
+        assert same.tolist() == [[True, True], [True, False], [False, True], [True, True]]
+    assert got[0][1, 128:].float().isnan().all() and got[0][2, :128].float().isnan().all()
+
+
 def test_silu_infinities_and_nans():
     h = _randn((5, 768), 21)
     h[0, 2], h[1, 384 + 130], h[2, 300] = float("nan"), float("inf"), float("inf")
