@@ -280,6 +280,38 @@ def test_rows_beyond_32_bits():
     assert not got[-70:, :-64].any() and not got[M - 2000:M - 70].any() and not got[:300].any()
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_as_many_rows_as_are_counted(fp8):
+    """2^31 - 1 rows, all but three of them one group's: tiles and rows are counted
+    beyond 2^31.  (Values that every order of the sum gives exactly.)"""
+    M, N, K = 2 ** 31 - 1, 8, 16 if fp8 else 8
+    if torch.cuda.get_device_properties(0).total_memory < 120 * 2 ** 30:
+        pytest.skip("needs 90 GB")
+    kind = FP8 if fp8 else BF
+    g = torch.Generator().manual_seed(17)
+    block = torch.randint(-3, 4, (2 ** 24, K), generator=g).to(DEV).float()
+    w = torch.randint(-3, 4, (3, N, K), generator=g).to(DEV).float()
+    want = [(block @ w[e].t()).to(BF) for e in (0, 2)]
+    x = torch.empty((M, K), dtype=kind, device=DEV)
+    part = block.to(kind)
+    for i in range(0, M, 2 ** 24):
+        x[i:i + 2 ** 24] = part[:min(2 ** 24, M - i)]
+    ends = torch.tensor([M - 3, 0, M - 1], dtype=torch.int32, device=DEV)
+    if fp8:
+        out = G.grouped_mm_fp8(x, torch.ones((M, 1), device=DEV), w.to(FP8),
+                               torch.ones((3, 1, 1), device=DEV), ends)
+    else:
+        out = G.grouped_mm(x, w.to(BF), ends)
+    del x
+    for i in range(0, M, 2 ** 24):
+        n = min(2 ** 24, M - 3 - i)
+        assert torch.equal(out[i:i + n], want[0][:n]), i
+    assert torch.equal(out[M - 3:M - 1], want[1][2 ** 24 - 4:2 ** 24 - 2])
+    assert not out[M - 1].any()
+    del out
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("M", [12, 200, 900])
 def test_runs_together(M):
     """The operators as a rank uses them, against the oracle's own chain from

@@ -150,7 +150,8 @@ struct Table {
 
 // Ends outside [0, M] count as 0 or M, one below an earlier one as that one:
 // groups never overlap and stay inside the buffer whatever ends holds.  Called
-// by one wave.
+// by one wave.  (Sums behind a group's rows are unsigned, here and in find_work: of
+// 2^31 - 1 rows they pass 2^31, at most by a fourth.)
 __device__ inline void fill_table(Table* tab, const Args& a, int toks) {
   const int lane = threadIdx.x & 63;
   int top = 0, base = 0;
@@ -164,7 +165,7 @@ __device__ inline void fill_table(Table* tab, const Args& a, int toks) {
     end = max(end, top);
     const int before = __shfl_up(end, 1);
     const int start = lane ? before : top;
-    const int n = (end - start + toks - 1) / toks;
+    const int n = (int)(((uint32_t)(end - start) + toks - 1) / toks);
     int incl = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -192,7 +193,7 @@ struct Work {
 
 // Works are ordered by expert, then panel, then tile of rows; a group of n
 // tiles splits into equal ones (rounded up to 16 rows).
-__device__ inline Work find_work(const Table* tab, int w, int E, int npanels, int toks) {
+__device__ inline Work find_work(const Table* tab, int w, int E, int npanels) {
   const int lane = threadIdx.x & 63;
   const int j = w / npanels;  // a tile of the work's expert
   for (int e0 = 0; e0 < E; e0 += 64) {
@@ -202,13 +203,13 @@ __device__ inline Work find_work(const Table* tab, int w, int E, int npanels, in
       const int e = e0 + __builtin_ctzll(hit);
       const int b = __builtin_amdgcn_readfirstlane(tab->base[e]);
       const int n = __builtin_amdgcn_readfirstlane(tab->base[e + 1]) - b;
-      const int m = __builtin_amdgcn_readfirstlane(tab->rows[e]);
+      const uint32_t m = __builtin_amdgcn_readfirstlane(tab->rows[e]);
       const int start = __builtin_amdgcn_readfirstlane(tab->start[e]);
       const int off = w - b * npanels;
-      const int per = ((m + n - 1) / n + 15) & ~15;
-      const int m0 = (off % n) * per;
+      const uint32_t per = ((m + n - 1) / n + 15) & ~15u;
+      const uint32_t m0 = min((off % n) * per, m);
       // (rounding up may leave the last tiles fewer rows, or none)
-      return Work{e, off / n, start + min(m0, m), max(min(per, m - m0), 0)};
+      return Work{e, off / n, start + (int)m0, (int)min(per, m - m0)};
     }
   }
   return Work{-1, 0, 0, 0};
@@ -248,7 +249,7 @@ struct Walk {
     p.pair = p.pair + 1 == pairs ? 0 : p.pair + 1;
     if (--p.left > 0) return p;
     do {
-      p.work = find_work(tab, work_of(blockIdx.x, turn++, run), E, npanels, TOKS);
+      p.work = find_work(tab, work_of(blockIdx.x, turn++, run), E, npanels);
     } while (p.work.expert >= 0 && p.work.rows == 0);
     const uint32_t set = (uint32_t)(max(p.work.expert, 0) * npanels + p.work.panel) / 24;
     p.pair = (int)((uint64_t)(set * kGolden) * (uint32_t)pairs >> 32);
