@@ -316,6 +316,20 @@ int wisp_grouped_mm_fp8(const uint8_t* q, int64_t q_ld, const float* s, int64_t 
                         int64_t ws_stride, const int32_t* ends, int E, int M, int N, int K,
                         void* out, int zero_tail, wisp_stream_t stream);
 
+/* The kernel that the two calls above run for these sizes and this output (a test
+ * or a profile names it; fp8: 0 or 1), or -1 for sizes that they refuse or that are
+ * empty.  Nothing is read or launched.  Tiles are so many weight rows by 64 rows of x, large ones 256 by
+ * so many rows of x. */
+#define WISP_GROUPED_FEW 1        /* 16 weight rows a block, the columns shared */
+#define WISP_GROUPED_TILE_64 2
+#define WISP_GROUPED_TILE_128 3
+#define WISP_GROUPED_TILE_256 4
+#define WISP_GROUPED_LARGE_128 5  /* bfloat16 */
+#define WISP_GROUPED_LARGE_192 6  /* bfloat16 */
+#define WISP_GROUPED_LARGE_256 7  /* FP8 */
+#define WISP_GROUPED_NARROW 16    /* with a tile: outputs are stored one by one */
+int wisp_grouped_mm_kernel(int fp8, int E, int M, int N, int K, const void* out, int out_dtype);
+
 /* Bytes of the device array wisp_moe_experts_noalloc works in, per GPU, in
  * a default build; building with WISP_NOALLOC_SCRATCH_MIB=n sets n MiB, and
  * wisp_noalloc_scratch_bytes() returns the size the library was built with.

@@ -8,6 +8,7 @@ import torch
 from oracle import rows as O
 from wisp.integrations.vllm import grouped_mm as G
 from wisp.integrations.vllm import rows_fp8 as R
+from wisp_amd import _lib
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -640,3 +641,152 @@ def test_refusals():
                 lambda: G.grouped_mm(x[:, :4], w[:, :, :4], ends)):
         with pytest.raises(NotImplementedError):
             bad()
+
+
+# Every kernel by name, so that another choice of kernels cannot leave one untested:
+# the kernel, FP8, output type, experts, rows an expert, outputs, columns (large tiles:
+# whole pairs of chunks, and columns behind a row's end within one and after a whole one).
+KERNELS = [
+    (_lib.WISP_GROUPED_FEW, False, BF, 3, 10, 72, 136),
+    (_lib.WISP_GROUPED_FEW, False, F32, 3, 10, 75, 136),
+    (_lib.WISP_GROUPED_FEW, True, BF, 3, 10, 72, 144),
+    (_lib.WISP_GROUPED_TILE_64, False, BF, 4, 100, 264, 200),
+    (_lib.WISP_GROUPED_TILE_64, False, F32, 4, 100, 260, 256),
+    (_lib.WISP_GROUPED_TILE_64, True, BF, 4, 100, 264, 272),
+    (_lib.WISP_GROUPED_TILE_64 | _lib.WISP_GROUPED_NARROW, False, BF, 4, 100, 261, 200),
+    (_lib.WISP_GROUPED_TILE_64 | _lib.WISP_GROUPED_NARROW, False, F32, 4, 100, 261, 200),
+    (_lib.WISP_GROUPED_TILE_64 | _lib.WISP_GROUPED_NARROW, True, BF, 4, 100, 262, 272),
+    (_lib.WISP_GROUPED_TILE_128, False, BF, 60, 5, 1672, 200),
+    (_lib.WISP_GROUPED_TILE_128, True, BF, 24, 100, 1800, 400),
+    (_lib.WISP_GROUPED_TILE_256, False, F32, 110, 5, 1800, 200),
+    (_lib.WISP_GROUPED_TILE_256, True, BF, 110, 5, 1800, 208),
+    (_lib.WISP_GROUPED_LARGE_128, False, BF, 24, 100, 1800, 200),
+    (_lib.WISP_GROUPED_LARGE_128, False, BF, 24, 90, 1800, 256),
+    (_lib.WISP_GROUPED_LARGE_128, False, F32, 24, 100, 1796, 272),
+    (_lib.WISP_GROUPED_LARGE_192, False, BF, 24, 130, 1800, 200),
+    (_lib.WISP_GROUPED_LARGE_192, False, BF, 24, 125, 1800, 512),
+    (_lib.WISP_GROUPED_LARGE_192, False, F32, 24, 130, 1796, 144),
+    (_lib.WISP_GROUPED_LARGE_256, True, BF, 24, 200, 1800, 144),
+    (_lib.WISP_GROUPED_LARGE_256, True, BF, 24, 200, 1800, 272),
+    (_lib.WISP_GROUPED_LARGE_256, True, BF, 24, 200, 1800, 384),
+    (_lib.WISP_GROUPED_LARGE_256, True, BF, 24, 130, 1800, 512),
+]
+_kernels = pytest.mark.parametrize("kernel,fp8,dtype,E,per,N,K", KERNELS)
+
+
+def _runs(kernel, fp8, dtype, E, M, N, K, out=1 << 20):
+    """Asserts that a call of these sizes runs ``kernel``."""
+    got = _lib.lib().wisp_grouped_mm_kernel(fp8, E, M, N, K, out, G._DTYPES[dtype])
+    assert got == kernel, got
+
+
+def _inputs(fp8, dtype, M, E, N, K, seed):
+    """Rows and weights, and the call over them."""
+    if fp8:
+        return _case8(M, E, N, K, seed), G.grouped_mm_fp8
+    return (_randn((M, K), seed), _randn((E, N, K), seed + 1, BF, 0.1)), \
+        lambda *a, **kw: G.grouped_mm(*a, dtype=dtype, **kw)
+
+
+@_kernels
+def test_every_kernel_keeps_values_in_their_rows_and_columns(kernel, fp8, dtype, E, per, N, K):
+    """What is no number in other groups' rows and scales, behind the last group, in other
+    experts' weights and scales, behind a row's last column and behind the last output
+    touches nothing else; a given output keeps its rows behind the last group."""
+    M, tail = E * per, 7
+    _runs(kernel, fp8, dtype, E, M, N, K)
+    counts = _spread_counts(M - tail, E, K)
+    counts[1], counts[2] = counts[1] + counts[2], 0   # (an expert that no row is for)
+    ends = _ends(counts)
+    ins, call = _inputs(fp8, dtype, M, E, N, K, per)
+    want = call(*ins, ends)
+    kind, pad = (torch.uint8, 0x7f) if fp8 else (BF, float("nan"))
+    raw = [t.view(kind) if t.element_size() < 4 else t for t in ins]
+    x, w = raw[0], raw[2 if fp8 else 1]
+    big_x = torch.full((M, K + 96), pad, dtype=kind, device=DEV)
+    big_w = torch.full((E, N + 3, K + 160), pad, dtype=kind, device=DEV)
+    big_x[:, :K], big_w[:, :N, :K] = x, w
+    big_x[M - tail:], big_w[2] = pad, pad
+    if fp8:
+        g = ins[1].shape[1]
+        big_s = torch.full((M, g + 2), float("nan"), device=DEV)
+        big_s[:, :g] = ins[1]
+        big_s[M - tail:] = float("inf")
+        ws = ins[3].clone()
+        ws[2] = float("nan")
+        args = big_x.view(FP8)[:, :K], big_s[:, :g], big_w.view(FP8)[:, :N, :K], ws, ends
+    else:
+        args = big_x[:, :K], big_w[:, :N, :K], ends
+    assert torch.equal(_bits(call(*args)), _bits(want))
+    out = torch.full((M, N), 7.0, dtype=dtype, device=DEV)
+    call(*args, out=out)
+    assert torch.equal(_bits(out[:M - tail]), _bits(want[:M - tail]))
+    assert bool((out[M - tail:] == 7).all()) and not want[M - tail:].any()
+    # one row and one weight row of the largest group, one row of the group's last
+    e = int(np.argmax(counts))
+    first, n = int(sum(counts[:e])), int(counts[e])
+    rows = [first + n // 2, first + n - 1]
+    bad = torch.zeros((M, N), dtype=torch.bool, device=DEV)
+    bad[rows], bad[first:first + n, N - 2] = True, True
+    big_x[rows, K - 1], big_w[e, N - 2, K - 1] = pad, pad
+    got = call(*args)
+    assert torch.equal(_bits(got[~bad]), _bits(want[~bad])) and got[bad].isnan().all()
+    if fp8:   # and scales of a row and of a block of weights
+        row, block = first + n // 3, (N - 1) // 128
+        big_s[row, g - 1] = float("nan")
+        ws[e, block, g - 1] = float("nan")
+        bad[row], bad[first:first + n, 128 * block:] = True, True
+        got = call(*args)
+        assert torch.equal(_bits(got[~bad]), _bits(want[~bad])) and got[bad].isnan().all()
+
+
+@_kernels
+def test_every_kernel_in_a_graph(kernel, fp8, dtype, E, per, N, K):
+    """Replayed with other ends, rows, weights and scales in the captured buffers, beside
+    eager calls: the eager call's bytes each time."""
+    M = E * per
+    _runs(kernel, fp8, dtype, E, M, N, K)
+    sets = [(*_inputs(fp8, dtype, M, E, N, K, 10 * k)[0], _ends(_spread_counts(M - 3 * k, E, k)))
+            for k in range(3)]
+    ins, call = [t.clone() for t in sets[0]], _inputs(fp8, dtype, 1, 1, 8, 16, 0)[1]
+    call(*ins)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call(*ins)
+    for new in sets + sets[:2]:
+        for t, v in zip(ins, new):
+            t.copy_(v)
+        want = call(*new)
+        out.fill_(7)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(_bits(out), _bits(want))
+
+
+@_kernels
+def test_every_kernel_against_rows_of_their_own(kernel, fp8, dtype, E, per, N, K):
+    """Rows of a group and the same rows in calls of their own (1, 16, 17 and 60 of them,
+    one expert): each within its bound of the exact values, so within two of each other."""
+    M = E * per
+    _runs(kernel, fp8, dtype, E, M, N, K)
+    counts = _spread_counts(M, E, per)
+    ins, call = _inputs(fp8, dtype, M, E, N, K, per + 5)
+    got = call(*ins, _ends(counts))
+    e = int(np.argmax(counts))
+    first, n = int(sum(counts[:e])), int(counts[e])
+    if fp8:
+        x, w = _values8(ins[0][first:first + n], ins[1][first:first + n], ins[2][e:e + 1],
+                        ins[3][e:e + 1])
+    else:
+        x, w = _f64(ins[0][first:first + n]), _f64(ins[1][e:e + 1])
+    want, bound = O.grouped_mm(x, w, [n], DOT8 if fp8 else 0.0)
+    _near(got[first:first + n], want, bound, dtype)
+    bound = 2 * (bound + (O.BF16 if dtype == BF else O.STEP) * (np.abs(want) + bound) + O.TINY)
+    for rows in (1, 16, 17, 60):
+        for at in {0, n // 2, max(n - rows, 0)}:
+            part = slice(first + at, first + min(at + rows, n))
+            mine = [t[part] if i < (2 if fp8 else 1) else t[e:e + 1] for i, t in enumerate(ins)]
+            alone = call(*mine, _ends([part.stop - part.start]))
+            off = np.abs(_f64(alone) - _f64(got[part]))
+            assert np.all(off <= bound[at:at + rows])

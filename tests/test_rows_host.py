@@ -116,3 +116,21 @@ def test_overlaps():
     R._check_apart("out", b[:0], ((b, False),))
     with pytest.raises(ValueError, match="overlaps"):
         R._check_apart("out", b, ((b.view(torch.int32), True),))
+
+
+@pytest.mark.parametrize("kw,kernel", [
+    (dict(), _lib.WISP_GROUPED_FEW), (dict(M=0), -1), (dict(N=0), -1), (dict(E=0), -1),
+    (dict(E=513), -1), (dict(K=0), -1), (dict(K=60), -1), (dict(fp8=1, K=136), -1),
+    (dict(dt=FP8), -1), (dict(fp8=1, dt=F32), -1), (dict(N=1 << 21), -1), (dict(K=1 << 21), -1),
+    (dict(M=8192 * 8, E=128, N=1536, K=2048), _lib.WISP_GROUPED_LARGE_192),
+    (dict(M=64, E=128, N=1536, K=2048), _lib.WISP_GROUPED_FEW),
+    (dict(M=256, E=128, N=1536, K=2048, fp8=1), _lib.WISP_GROUPED_TILE_256),
+    (dict(M=4000, E=8, N=28672, K=4096, fp8=1), _lib.WISP_GROUPED_LARGE_256),
+    (dict(M=4000, E=8, N=28667, K=4096, fp8=1),
+     _lib.WISP_GROUPED_TILE_256 | _lib.WISP_GROUPED_NARROW),
+])
+def test_the_kernel_of_a_call(hiplib, kw, kernel):
+    a = dict(fp8=0, E=2, M=4, N=64, K=64, dt=BF16)
+    a.update(kw)
+    assert hiplib.wisp_grouped_mm_kernel(a["fp8"], a["E"], a["M"], a["N"], a["K"], P,
+                                         a["dt"]) == kernel

@@ -30,6 +30,14 @@ WISP_ALGO_GEMV = 1
 WISP_ALGO_MFMA = 2
 WISP_PAGEIN_MEMCPY = 0
 WISP_PAGEIN_KERNEL = 1
+WISP_GROUPED_FEW = 1
+WISP_GROUPED_TILE_64 = 2
+WISP_GROUPED_TILE_128 = 3
+WISP_GROUPED_TILE_256 = 4
+WISP_GROUPED_LARGE_128 = 5
+WISP_GROUPED_LARGE_192 = 6
+WISP_GROUPED_LARGE_256 = 7
+WISP_GROUPED_NARROW = 16
 WISP_NOALLOC_SCRATCH_BYTES = 64 << 20  # a default build's; the library's: noalloc_scratch_bytes()
 
 # Decision-record header words (wisp_amd/csrc/pager_core.h).
@@ -118,6 +126,7 @@ SIGNATURES = {
                                _i32, _vp]),
     "wisp_grouped_mm_fp8": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i32,
                                    _i32, _i32, _i32, _vp, _i32, _vp]),
+    "wisp_grouped_mm_kernel": (_i32, [_i32, _i32, _i32, _i32, _i32, _vp, _i32]),
     "wisp_silu_mul_fp8": (_i32, [_vp, _i32, _i64, _i32, _i64, _vp, _vp, _vp]),
     "wisp_layer_create": (_i32, [C.POINTER(LayerDesc), C.POINTER(_vp)]),
     "wisp_layer_destroy": (_i32, [_vp]),

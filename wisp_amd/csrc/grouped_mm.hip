@@ -1147,16 +1147,23 @@ float tiles_of(float per, int t) {
   return n;
 }
 
-template <bool FP8, Out OUT>
-hipError_t launch_tile(const Args& a, hipStream_t st) {
+// The weight rows of the small tiles.
+int tile_rows(const Args& a) {
   // The largest panels that give the GPU's blocks a tile each; where experts have
   // several tiles of rows, and the products count too, panels of 128 from fewer on
   // (fp8, 8 experts of 75 rows, 4096 x 14336: 170 us in panels of 64, 151 in 128;
   // 16 of 64 rows, 1536 x 2048: 22.3 and 23.4).
   const int64_t used = std::min(a.M, a.E), works = used * ((a.N + 127) / 128);
   const int64_t rows = (int64_t)(tiles_of((float)a.M / a.E, 64) + 0.6f);
-  if (used * ((a.N + 255) / 256) >= 768) return launch_tile<FP8, 4, OUT>(a, st);
-  if (works >= 768 || (rows > 1 && works * rows >= 400)) return launch_tile<FP8, 2, OUT>(a, st);
+  if (used * ((a.N + 255) / 256) >= 768) return WISP_GROUPED_TILE_256;
+  if (works >= 768 || (rows > 1 && works * rows >= 400)) return WISP_GROUPED_TILE_128;
+  return WISP_GROUPED_TILE_64;
+}
+
+template <bool FP8, Out OUT>
+hipError_t launch_tile(int kernel, const Args& a, hipStream_t st) {
+  if (kernel == WISP_GROUPED_TILE_256) return launch_tile<FP8, 4, OUT>(a, st);
+  if (kernel == WISP_GROUPED_TILE_128) return launch_tile<FP8, 2, OUT>(a, st);
   return launch_tile<FP8, 1, OUT>(a, st);
 }
 
@@ -1170,8 +1177,10 @@ hipError_t launch_big(const Args& a, hipStream_t st) {
   return a.row_bytes % (2 * kChunk) ? launch_big<L, true>(a, st) : launch_big<L, false>(a, st);
 }
 
+// The kernel of a call: WISP_GROUPED_*, with WISP_GROUPED_NARROW where single values
+// are stored, which the small tiles do.
 template <bool FP8>
-hipError_t launch(const Args& a, hipStream_t st) {
+int choose(const Args& a) {
   // The kernel for the fewest rows (a) against the small tiles (b), in us:
   //                     rows  bf16 a    b   fp8 a    b
   //   128 x 1536 x 2048,  32   37.2  37.4   21.0  21.5
@@ -1191,9 +1200,8 @@ hipError_t launch(const Args& a, hipStream_t st) {
   const int64_t works = std::min(a.M, a.E) * (int64_t)((a.N + 63) / 64);
   if (a.M <= most || (a.M <= 64 && works <= 512) ||
       (a.M <= 256 && works < 512 && tiles_of((float)a.M / a.E, kFewCols) == 1.f))
-    return launch_few<FP8>(a, st);
-  // single values are stored by the small tiles only
-  if (a.N % (a.out_f32 ? 4 : 8)) return launch_tile<FP8, kNarrow>(a, st);
+    return WISP_GROUPED_FEW;
+  if (a.N % (a.out_f32 ? 4 : 8)) return tile_rows(a) | WISP_GROUPED_NARROW;
   // What a chunk of columns takes in each kernel, in 1/100 us, from the works that a
   // CU gets: w on average, as whole turns in the large tiles.  (Works of the small
   // ones: 128 weight rows.  Measured over 4 to 128 experts, 8 sizes of weights, 32
@@ -1219,17 +1227,39 @@ hipError_t launch(const Args& a, hipStream_t st) {
     return std::max(turn * ceilf(w) + work * w + start, stream);
   };
   if constexpr (FP8) {
-    if (large(256, 140, 80) < std::max(50 + 52 * w, stream))
-      return a.row_bytes % (2 * kChunk) ? launch_big_fp8<true>(a, st)
-                                        : launch_big_fp8<false>(a, st);
-    return launch_tile<true, kBf16>(a, st);
+    if (large(256, 140, 80) < std::max(50 + 52 * w, stream)) return WISP_GROUPED_LARGE_256;
   } else {
     const float small = std::max(30 + 44 * w, stream);
     const float two = large(128, 80, 34), three = large(192, 100, 40);
     if (std::min(two, three) < small || (std::min(two, three) == stream && per > 40))
-      return two <= three ? launch_big<2>(a, st) : launch_big<3>(a, st);
-    return a.out_f32 ? launch_tile<false, kF32>(a, st) : launch_tile<false, kBf16>(a, st);
+      return two <= three ? WISP_GROUPED_LARGE_128 : WISP_GROUPED_LARGE_192;
   }
+  return tile_rows(a);
+}
+
+template <bool FP8>
+hipError_t launch(const Args& a, hipStream_t st) {
+  const int kernel = choose<FP8>(a);
+  switch (kernel) {
+    case WISP_GROUPED_FEW:
+      return launch_few<FP8>(a, st);
+    case WISP_GROUPED_LARGE_128:
+      if constexpr (!FP8) return launch_big<2>(a, st);
+      break;
+    case WISP_GROUPED_LARGE_192:
+      if constexpr (!FP8) return launch_big<3>(a, st);
+      break;
+    case WISP_GROUPED_LARGE_256:
+      if constexpr (FP8)
+        return a.row_bytes % (2 * kChunk) ? launch_big_fp8<true>(a, st)
+                                          : launch_big_fp8<false>(a, st);
+      break;
+  }
+  const int tile = kernel & ~WISP_GROUPED_NARROW;
+  if (kernel != tile) return launch_tile<FP8, kNarrow>(tile, a, st);
+  if constexpr (!FP8)
+    if (a.out_f32) return launch_tile<false, kF32>(tile, a, st);
+  return launch_tile<FP8, kBf16>(tile, a, st);
 }
 
 template <bool FP8>
@@ -1296,4 +1326,19 @@ extern "C" int wisp_grouped_mm_fp8(const uint8_t* q, int64_t q_ld, const float* 
   const Args a = {q, s, w, ws, ends, out, q_ld, w_stride, w_ld, ws_stride, s_ld, E, M, N, K,
                   groups, false, zero_tail != 0};
   return grouped<true>(a, (hipStream_t)stream);
+}
+
+extern "C" int wisp_grouped_mm_kernel(int fp8, int E, int M, int N, int K, const void* out,
+                                      int out_dtype) {
+  using namespace wisp;
+  const int elem = fp8 ? 1 : 2;
+  if (E < 1 || E > kMaxExperts || M < 1 || N < 1 || K < 1 ||
+      (out_dtype != WISP_BF16 && (fp8 || out_dtype != WISP_F32)) ||
+      unsupported(K, K, 0, N, K, elem, nullptr, nullptr))
+    return -1;
+  Args a{};
+  a.out = const_cast<void*>(out);
+  a.E = E, a.M = M, a.N = N, a.row_bytes = K * elem;
+  a.out_f32 = out_dtype == WISP_F32;
+  return fp8 ? choose<true>(a) : choose<false>(a);
 }
