@@ -295,7 +295,9 @@ int wisp_silu_mul_fp8(const void* h, int dtype, int64_t rows, int inter, int64_t
  * below an earlier end as that one.  Rows behind the last group: left alone,
  * or zeroed with zero_tail.  x [M, K] bfloat16, rows x_ld elements apart; W of
  * expert e at w + e*w_stride, [N, K] bfloat16, rows w_ld elements apart; out
- * [M, N] contiguous, WISP_BF16 or WISP_F32: float32 sums, rounded once.
+ * [M, N] contiguous from any element on, WISP_BF16 or WISP_F32: float32 sums, rounded
+ * once (a bfloat16 out that starts between two dwords is stored value by value, by the
+ * small tiles).
  * E <= 512, N < 2^21, K a multiple of 8, x, w and their strides 16-byte aligned,
  * an expert's weights below 2 GiB, rows of w less than 16 MiB and of x less than
  * 4 MiB apart.  No reference counterpart (its experts run over one GPU's pairs). */

@@ -790,3 +790,31 @@ def test_every_kernel_against_rows_of_their_own(kernel, fp8, dtype, E, per, N, K
             alone = call(*mine, _ends([part.stop - part.start]))
             off = np.abs(_f64(alone) - _f64(got[part]))
             assert np.all(off <= bound[at:at + rows])
+
+
+@_kernels
+@pytest.mark.parametrize("at", [1, 2, 4])
+def test_outputs_from_any_element_on(kernel, fp8, dtype, E, per, N, K, at):
+    """A given output at any element of a larger buffer: its values within their bound, and
+    what lies before and behind it as it was."""
+    M, few = E * per, 16
+    _runs(kernel, fp8, dtype, E, M, N, K)
+    counts = _spread_counts(M - 5, E, per)
+    ins, call = _inputs(fp8, dtype, M, E, N, K, per + 9)
+    slab = torch.full((M * N + 2 * few,), 7.0, dtype=dtype, device=DEV)
+    assert slab.data_ptr() % 16 == 0
+    out = slab[at:at + M * N].view(M, N)
+    want = call(*ins, _ends(counts))
+    call(*ins, _ends(counts), out=out)
+    # rows that the same kernel stores: the same bytes; those of another: twice the bound
+    if dtype == F32 or at % 2 == 0 or kernel == _lib.WISP_GROUPED_FEW:
+        assert torch.equal(_bits(out[:M - 5]), _bits(want[:M - 5]))
+    else:
+        e = int(np.argmax(counts))
+        first, n = int(sum(counts[:e])), int(counts[e])
+        part = slice(first, first + n)
+        x, w = _values8(ins[0][part], ins[1][part], ins[2][e:e + 1], ins[3][e:e + 1]) if fp8 \
+            else (_f64(ins[0][part]), _f64(ins[1][e:e + 1]))
+        _near(out[part], *O.grouped_mm(x, w, [n], DOT8 if fp8 else 0.0), dtype)
+    assert bool((slab[:at] == 7).all()) and bool((out[M - 5:] == 7).all())
+    assert bool((slab[at + M * N:] == 7).all())

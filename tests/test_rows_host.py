@@ -134,3 +134,21 @@ def test_the_kernel_of_a_call(hiplib, kw, kernel):
     a.update(kw)
     assert hiplib.wisp_grouped_mm_kernel(a["fp8"], a["E"], a["M"], a["N"], a["K"], P,
                                          a["dt"]) == kernel
+
+
+@pytest.mark.parametrize("fp8,E,M,N,K", [(0, 128, 65536, 1536, 2048), (1, 8, 4000, 28672, 4096),
+                                         (0, 4, 400, 264, 256), (1, 4, 400, 264, 256),
+                                         (0, 24, 2400, 1800, 200)])
+def test_outputs_between_two_dwords_are_stored_one_by_one(hiplib, fp8, E, M, N, K):
+    """8- and 16-byte stores go to whole dwords: a bfloat16 output at an odd element takes
+    none, one at an even element the same kernel as an aligned one."""
+    def kernel(at, dt=BF16):
+        return hiplib.wisp_grouped_mm_kernel(fp8, E, M, N, K, P + at, dt)
+
+    assert kernel(0) == kernel(4) == kernel(8) and not kernel(0) & _lib.WISP_GROUPED_NARROW
+    for at in (2, 6, 14):
+        assert kernel(at) & _lib.WISP_GROUPED_NARROW
+        assert kernel(at) & ~_lib.WISP_GROUPED_NARROW in (
+            _lib.WISP_GROUPED_TILE_64, _lib.WISP_GROUPED_TILE_128, _lib.WISP_GROUPED_TILE_256)
+    if not fp8:
+        assert kernel(4, F32) == kernel(0, F32)

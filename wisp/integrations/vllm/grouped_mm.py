@@ -98,7 +98,9 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, *,
     ``x [M, K]`` and ``w [E, N, K]``, float32 sums, rounded once to ``dtype``
     (bfloat16 or float32; a given ``out`` is of that type).  K is a multiple of
     8; rows of ``x`` may lie any distance apart, experts and rows of ``w`` any
-    multiple of 16 bytes, and ``w`` starts at one."""
+    multiple of 16 bytes, and ``w`` starts at one.  A given ``out`` may start
+    anywhere (a bfloat16 one between two dwords is stored value by value,
+    which takes longer)."""
     M, E, N, K, step, w_ld = _sizes(x, w, ends)
     if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
         raise NotImplementedError("wisp: grouped_mm takes bfloat16 rows and weights")

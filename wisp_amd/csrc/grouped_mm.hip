@@ -1201,7 +1201,9 @@ int choose(const Args& a) {
   if (a.M <= most || (a.M <= 64 && works <= 512) ||
       (a.M <= 256 && works < 512 && tiles_of((float)a.M / a.E, kFewCols) == 1.f))
     return WISP_GROUPED_FEW;
-  if (a.N % (a.out_f32 ? 4 : 8)) return tile_rows(a) | WISP_GROUPED_NARROW;
+  // (pieces of 8 and 16 bytes go to whole dwords: a bfloat16 output that starts between
+  // two of them, at an odd element of its buffer, takes single values too)
+  if (a.N % (a.out_f32 ? 4 : 8) || (uintptr_t)a.out % 4) return tile_rows(a) | WISP_GROUPED_NARROW;
   // What a chunk of columns takes in each kernel, in 1/100 us, from the works that a
   // CU gets: w on average, as whole turns in the large tiles.  (Works of the small
   // ones: 128 weight rows.  Measured over 4 to 128 experts, 8 sizes of weights, 32
