@@ -570,7 +570,7 @@ __global__ __launch_bounds__(256, 2) void grouped_tile_kernel(const Args a) {
         for (int g = 0; g < G; ++g) v[g] = acc[g][t];
         if constexpr (OUT != kNarrow)
           store_outputs<OUT == kF32, true>(o, 16 * t, col, n, v);
-        else if (a.out_f32)
+        else if (!FP8 && a.out_f32)
           store_outputs<true, false>(o, 16 * t, col, n, v);
         else
           store_outputs<false, false>(o, 16 * t, col, n, v);
@@ -1095,7 +1095,7 @@ __global__ __launch_bounds__(256) void grouped_few_kernel(const Args a) {
       for (int i = 1; i < kWaves; ++i) v += part[i][n][m];
       if (n0 + n < a.N && m0 + m < rows) {
         const int64_t at = (int64_t)(row0 + m0 + m) * a.N + n0 + n;
-        if (a.out_f32)
+        if (!FP8 && a.out_f32)
           ((float*)a.out)[at] = v;
         else
           ((uint16_t*)a.out)[at] = bf16_rne(v);
