@@ -19,6 +19,15 @@ never overlap.  Rows behind the last group are left as they are in a given
 weights are ``[E, N, K]`` (``w13``, ``w2`` as the MoE layers hold them), each row
 contiguous, an expert's less than 2 GiB and its rows less than 16 MiB apart (rows of
 ``x``, and of its scales, less than 4 MiB).
+
+The kernel goes by the sizes that the host knows: experts, outputs, columns and
+the rows of the buffer, however few of them ``ends`` puts into groups.  A buffer
+much larger than its rows takes the kernel of a full one: where a program can,
+it passes as many rows as it may have.  The order of a row's sum goes by the
+kernel and by its expert's number in the call, so the same call gives the same
+bytes again, but a token's row may have other last bits (each within the bound
+of a float32 sum) in another batch or on a rank that numbers its experts
+otherwise.
 """
 from __future__ import annotations
 
@@ -126,8 +135,10 @@ def grouped_mm_fp8(q: torch.Tensor, s: torch.Tensor, w: torch.Tensor, ws: torch.
     and codes ``w [E, N, K]`` with block scales ``ws [E, ceil(N / 128),
     ceil(K / 128)]``, all codes ``float8_e4m3fn`` and scales float32.  K is a
     multiple of 16.  The products of 128 columns are summed by the matrix
-    instruction, scaled and summed in float32 (to some 2^-16 of the sum of the
-    products' sizes: there is no float32 output), and rounded once."""
+    instruction, scaled and summed in float32, and rounded once.  The
+    instruction's sums are right to some 2^-16 of the products' sizes on
+    ordinary quantised rows, to 2^-12 on codes of the full range: there is no
+    float32 output."""
     M, E, N, K, step, w_ld = _sizes(q, w, ends)
     if q.dtype != FP8 or w.dtype != FP8:
         raise NotImplementedError("wisp: grouped_mm_fp8 takes float8_e4m3fn codes")

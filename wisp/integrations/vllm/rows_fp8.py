@@ -11,7 +11,8 @@ owners of their experts moves half the bytes.
 row and group of 128 columns, ``[rows, ceil(cols / 128)]`` (the format of
 ``wisp_quant_fp8_groups``; here a row's last group may be shorter):
 ``s = max(max|y|, 1e-10) / 448`` and ``q = y / s`` to the nearest code, from
-the float32 ``y``.  A group that holds an infinity or a NaN gets NaN codes.
+the float32 ``y``.  A group that holds an infinity or a NaN gets NaN codes.  Rows
+of any width are made; the products take those of whole 16 columns.
 """
 from __future__ import annotations
 

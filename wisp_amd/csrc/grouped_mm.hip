@@ -239,7 +239,10 @@ __device__ inline Place nowhere() { return Place{Work{-1, 0, 0, 0}, 0, 0}; }
 // start at a pair of their own and wrap around: blocks that all start at column 0
 // crowd a few memory channels (Qwen3 w13 of 512 tokens 179 us, so 144), and panels
 // that each start elsewhere read the rows of x that they share at different times,
-// out of the L2 again (1024 tokens 161 us, so 154; 8192 tokens 463, 449).
+// out of the L2 again (1024 tokens 161 us, so 154; 8192 tokens 463, 449).  24 is four
+// experts of that layer in the large tiles, measured there; other sizes take it as it
+// is.  So the order of a sum, and the last bits of its row, go by the expert's place in
+// the call as well as by the kernel.
 constexpr uint32_t kGolden = 2654435769u;  // 2^32 / 1.618..: any first n are spread evenly
 template <int TOKS>
 struct Walk {
@@ -597,11 +600,11 @@ __global__ __launch_bounds__(256, 2) void grouped_tile_kernel(const Args a) {
 // MFMA row 8 * a + 4 * h + b of a group of 32 is weight row 16 * h + 4 * a + b, so
 // that a lane ends with 16 consecutive outputs of a row of x.
 //
-// Qwen3 w13 of 65536 rows, 128 experts (412 GFLOP): 450 us, 916 TFLOP/s; Mixtral
-// w13 of 4000 rows (940 GFLOP): 977 us, 962 TFLOP/s.  Of 100 cycles the matrix units
-// are busy for 58 and LDS for 34; the clock falls to 1.74 GHz for the power that
-// takes.  Without the loads the products take 287 us; memory is read 1.25 GB of
-// 1.07 needed.
+// Qwen3 w13 of 65536 rows, 128 experts (412 GFLOP): 449 to 457 us, 902 to 916 TFLOP/s;
+// Mixtral w13 of 4000 rows (940 GFLOP): 977 us, 962 TFLOP/s.  Of 100 cycles the matrix
+// units are busy for 58 and LDS for 34, at 1.74 GHz.  Without the loads the products
+// take 287 us: the copies, which wait in registers and cost a write of 16 cycles a KB
+// into LDS, are covered in part only; memory is read 1.25 GB of 1.07 needed.
 // One more 64 rows of x a tile (L 4) spills registers and takes 465 us and more.
 template <int L>
 struct Big {

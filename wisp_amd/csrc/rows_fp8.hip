@@ -9,9 +9,9 @@
 //     s = max(max|y|, 1e-10) / 448,  q = e4m3fn(y / s), nearest, ties to even
 // The codes come from the float32 y: one rounding a value, where a norm that
 // writes bfloat16 and a quantiser that reads it make two.  y / s is
-// y * (448 / max|y|), one division a group; against a division a value only
-// what lies within 2^-23 of a border between two codes differs.  A group that
-// holds an infinity or a NaN gets NaN codes.
+// y * (448 / max|y|), one division a group; against a division a value (both
+// round twice) only what lies within 2^-22 of a border between two codes differs.
+// A group that holds an infinity or a NaN gets NaN codes.
 //
 // A thread holds eight consecutive values of a row, so a group is 16 lanes
 // (its maximum four DPP steps) and every access of a wave one contiguous run.
@@ -330,7 +330,7 @@ __device__ inline float silu_fast(float g) {
   return g * r * (far ? (g <= -128.f ? 0.f : 0x1p-64f) : 1.f);
 }
 
-// One group a DPP row of 16 lanes.  65536 rows of 768 in 50 us (5.0 TB/s), 43 without
+// One group a DPP row of 16 lanes.  65536 rows of 768 in 48 to 50 us (5.0 to 5.3 TB/s), 43 without
 // the SiLU's arithmetic: memory and the vector units, which overlap in part.  Two
 // or four groups a thread, their loads first: 50 and 52; persistent blocks 51.
 template <typename T, bool VEC>
