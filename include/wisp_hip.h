@@ -300,7 +300,7 @@ int wisp_silu_mul_fp8(const void* h, int dtype, int64_t rows, int inter, int64_t
  * small tiles).
  * E <= 512, N < 2^21, M < 2^31, K a multiple of 8, x, w and their strides 16-byte aligned,
  * an expert's weights below 2 GiB, rows of w less than 16 MiB and of x less than
- * 4 MiB apart.  The kernel goes by E, M, N and K alone (M: the rows of the buffer), and
+ * 4 MiB apart, experts less than 2^50 elements.  The kernel goes by E, M, N and K alone (M: the rows of the buffer), and
  * the order of a row's sum by the kernel and by its expert's number: the same call gives
  * the same bytes, another batch may give the same row other last bits.  No reference
  * counterpart (its experts run over one GPU's pairs). */

@@ -818,3 +818,12 @@ def test_outputs_from_any_element_on(kernel, fp8, dtype, E, per, N, K, at):
         _near(out[part], *O.grouped_mm(x, w, [n], DOT8 if fp8 else 0.0), dtype)
     assert bool((slab[:at] == 7).all()) and bool((out[M - 5:] == 7).all())
     assert bool((slab[at + M * N:] == 7).all())
+
+
+def test_a_single_expert_s_strides_say_nothing():
+    """One expert: weights and block scales any distance from the next."""
+    q, s, w, ws = _case8(20, 1, 40, 64, 90)
+    ends = _ends([18])
+    want = G.grouped_mm_fp8(q, s, w, ws, ends)
+    far = [t.as_strided(t.shape, (2 ** 58, *t.stride()[1:])) for t in (w, ws)]
+    assert torch.equal(G.grouped_mm_fp8(q, s, far[0], far[1], ends), want)

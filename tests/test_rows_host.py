@@ -152,3 +152,17 @@ def test_outputs_between_two_dwords_are_stored_one_by_one(hiplib, fp8, E, M, N, 
             _lib.WISP_GROUPED_TILE_64, _lib.WISP_GROUPED_TILE_128, _lib.WISP_GROUPED_TILE_256)
     if not fp8:
         assert kernel(4, F32) == kernel(0, F32)
+
+
+@pytest.mark.parametrize("elements", [1 << 50, 1 << 60, 1 << 61, 1 << 62, (1 << 63) - 8])
+def test_strides_that_no_address_counts(hiplib, elements):
+    """Strides whose bytes, or those of 512 experts, pass 64 bits are refused as any that
+    are too large."""
+    for x_ld, ws, w_ld in ((elements, 4096, 64), (64, elements, 64), (64, 4096, elements)):
+        assert hiplib.wisp_grouped_mm(P, x_ld, P, ws, w_ld, P, 2, 4, 64, 64, P, BF16, 0,
+                                      None) == UNSUPPORTED
+        assert hiplib.wisp_grouped_mm_fp8(P, x_ld, P, 1, P, ws, w_ld, P, 1, P, 2, 4, 64, 64, P,
+                                          0, None) == UNSUPPORTED
+    for s_ld, ws in ((elements, 1), (1, elements)):
+        assert hiplib.wisp_grouped_mm_fp8(P, 64, P, s_ld, P, 4096, 64, P, ws, P, 2, 4, 64, 64, P,
+                                          0, None) == UNSUPPORTED

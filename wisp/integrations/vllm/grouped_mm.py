@@ -159,7 +159,8 @@ def grouped_mm_fp8(q: torch.Tensor, s: torch.Tensor, w: torch.Tensor, ws: torch.
     if M and N:
         rc = lib().wisp_grouped_mm_fp8(
             q.data_ptr(), q.stride(0) if M > 1 else K, s.data_ptr(), s.stride(0) if M > 1 else G,
-            w.data_ptr(), step, w_ld, ws.data_ptr(), ws.stride(0), ends.data_ptr(), E, M, N, K,
+            w.data_ptr(), step, w_ld, ws.data_ptr(), ws.stride(0) if E > 1 else 0,
+            ends.data_ptr(), E, M, N, K,
             out.data_ptr(), not given, _stream(q))
         if rc:
             check(rc, "grouped_mm_fp8")

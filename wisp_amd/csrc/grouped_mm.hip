@@ -1273,9 +1273,16 @@ int grouped(const Args& a, hipStream_t st) {
   return WISP_OK;
 }
 
+// Elements between experts: 512 times as many fit 64 bits as bytes of any type.
+constexpr int64_t kMostApart = (int64_t)1 << 50;
+
 // What both entry points check; elem: bytes of a column.
 const char* unsupported(int64_t x_ld, int64_t w_ld, int64_t w_stride, int64_t N, int64_t K,
                         int elem, const void* x, const void* w) {
+  // (first, so that no stride's bytes pass 64 bits below, nor a place in the weights)
+  if (x_ld >= (int64_t)1 << 22) return "rows of x 4 MiB apart";
+  if (w_ld >= (int64_t)1 << 24) return "rows of w 16 MiB apart";
+  if (w_stride >= kMostApart) return "experts 2^50 elements apart";
   if (K % (16 / elem)) return "a row of x and of w must be whole 16-byte pieces";
   if (x_ld * elem % 16 || w_ld * elem % 16 || w_stride * elem % 16 || (uintptr_t)x % 16 ||
       (uintptr_t)w % 16)
@@ -1326,6 +1333,8 @@ extern "C" int wisp_grouped_mm_fp8(const uint8_t* q, int64_t q_ld, const float* 
   if (E > kMaxExperts) return refuse(WISP_ERR_UNSUPPORTED, "more than 512 experts", where);
   if (const char* why = unsupported(q_ld, w_ld, w_stride, N, K, 1, q, w))
     return refuse(WISP_ERR_UNSUPPORTED, why, where);
+  if (ws_stride >= kMostApart)
+    return refuse(WISP_ERR_UNSUPPORTED, "block scales 2^50 elements apart", where);
   if (s_ld >= (int64_t)1 << 20)
     return refuse(WISP_ERR_UNSUPPORTED, "scales of x 4 MiB apart", where);
   const Args a = {q, s, w, ws, ends, out, q_ld, w_stride, w_ld, ws_stride, s_ld, E, M, N, K,
