@@ -298,12 +298,14 @@ int wisp_silu_mul_fp8(const void* h, int dtype, int64_t rows, int inter, int64_t
  * [M, N] contiguous from any element on, WISP_BF16 or WISP_F32: float32 sums, rounded
  * once (a bfloat16 out that starts between two dwords is stored value by value, by the
  * small tiles).
- * E <= 512, N < 2^21, M < 2^31, K a multiple of 8, x, w and their strides 16-byte aligned,
- * an expert's weights below 2 GiB, rows of w less than 16 MiB and of x less than
- * 4 MiB apart, experts less than 2^50 elements.  The kernel goes by E, M, N and K alone (M: the rows of the buffer), and
- * the order of a row's sum by the kernel and by its expert's number: the same call gives
- * the same bytes, another batch may give the same row other last bits.  No reference
- * counterpart (its experts run over one GPU's pairs). */
+ * E <= 512, N < 2^21, M < 2^31, K a multiple of 8, x, w and their strides
+ * 16-byte aligned, an expert's weights below 2 GiB, rows of w less than 16 MiB
+ * and of x less than 4 MiB apart, experts less than 2^50 elements.  The kernel
+ * goes by the types, E, M, N, K and out's alignment (M: the rows of the
+ * buffer), never by ends, and the order of a row's sum by the kernel and by its
+ * expert's number: the same call gives the same bytes, another batch may give
+ * the same row other last bits.  No reference counterpart (its experts run over
+ * one GPU's pairs). */
 int wisp_grouped_mm(const void* x, int64_t x_ld, const void* w, int64_t w_stride, int64_t w_ld,
                     const int32_t* ends, int E, int M, int N, int K, void* out, int out_dtype,
                     int zero_tail, wisp_stream_t stream);
@@ -314,17 +316,17 @@ int wisp_grouped_mm(const void* x, int64_t x_ld, const void* w, int64_t w_stride
  * ceil(K / 128)] contiguous.  Per 128 columns
  * acc += dot(q, w) * (s * ws) in float32; the dot is the fp8 matrix
  * instruction's, off by up to some 2^-16 of the sum of its products' sizes on
- * ordinary rows and 2^-12 on codes of the full range.  K a multiple of 16, rows of s less than 4 MiB apart; otherwise
- * as above. */
+ * ordinary rows and 2^-12 on codes of the full range.  K a multiple of 16, rows
+ * of s less than 4 MiB apart; otherwise as above. */
 int wisp_grouped_mm_fp8(const uint8_t* q, int64_t q_ld, const float* s, int64_t s_ld,
                         const uint8_t* w, int64_t w_stride, int64_t w_ld, const float* ws,
                         int64_t ws_stride, const int32_t* ends, int E, int M, int N, int K,
                         void* out, int zero_tail, wisp_stream_t stream);
 
-/* The kernel that the two calls above run for these sizes and this output (a test
- * or a profile names it; fp8: 0 or 1), or -1 for sizes that they refuse or that are
- * empty.  Nothing is read or launched.  Tiles are so many weight rows by 64 rows of x, large ones 256 by
- * so many rows of x. */
+/* The kernel that the two calls above run for these sizes and this output (a
+ * test or a profile names it; fp8: 0 or 1), or -1 for sizes that they refuse or
+ * that are empty.  Nothing is read or launched.  Tiles are so many weight rows
+ * by 64 rows of x, large ones 256 by so many rows of x. */
 #define WISP_GROUPED_FEW 1        /* 16 weight rows a block, the columns shared */
 #define WISP_GROUPED_TILE_64 2
 #define WISP_GROUPED_TILE_128 3
